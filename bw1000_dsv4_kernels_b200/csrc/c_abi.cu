@@ -289,4 +289,62 @@ int launch_w8a8_gemm_ld(const void* A, const void* B, const void* sa, const void
     return gemm_i8(a, cs(stream));
 }
 
+int launch_layernorm(void* res, const void* x, const void* w, const void* b, void* y, void* mean, void* rstd, int M, int N,
+                     float eps, dsv4_stream_t stream) {
+    if (int rc = check_rows("layernorm", M, N)) return rc;
+    if (M == 0) return 0;
+    if (N == 0) return fail(DSV4_ERR_ARG, "layernorm: the row length must be positive");
+    DSV4_REQUIRE_PTR("layernorm", x);
+    DSV4_REQUIRE_PTR("layernorm", w);
+    DSV4_REQUIRE_PTR("layernorm", b);
+    DSV4_REQUIRE_PTR("layernorm", y);
+    DSV4_REQUIRE_PTR("layernorm", mean);
+    DSV4_REQUIRE_PTR("layernorm", rstd);
+    return layernorm(res, x, w, b, y, nullptr, nullptr, mean, rstd, M, N, eps, cs(stream));
+}
+
+int launch_layernorm_quant(void* res, const void* x, const void* w, const void* b, void* q, void* s, void* mean, void* rstd,
+                           int M, int N, float eps, dsv4_stream_t stream) {
+    if (int rc = check_rows("layernorm_quant", M, N)) return rc;
+    if (M == 0) return 0;
+    if (N == 0) return fail(DSV4_ERR_ARG, "layernorm_quant: the row length must be positive");
+    DSV4_REQUIRE_PTR("layernorm_quant", x);
+    DSV4_REQUIRE_PTR("layernorm_quant", w);
+    DSV4_REQUIRE_PTR("layernorm_quant", b);
+    DSV4_REQUIRE_PTR("layernorm_quant", q);
+    DSV4_REQUIRE_PTR("layernorm_quant", s);
+    DSV4_REQUIRE_PTR("layernorm_quant", mean);
+    DSV4_REQUIRE_PTR("layernorm_quant", rstd);
+    return layernorm(res, x, w, b, nullptr, q, s, mean, rstd, M, N, eps, cs(stream));
+}
+
+int64_t dsv4_layernorm_backward_workspace(int M, int N) { return M > 0 && N > 0 ? layernorm_backward_workspace(M, N) : 0; }
+
+int launch_layernorm_backward(const void* dy, const void* x, const void* mean, const void* rstd, const void* w, const void* dres,
+                              void* dx, void* dw, void* db, void* workspace, int64_t workspace_bytes, int M, int N,
+                              dsv4_stream_t stream) {
+    if (int rc = check_rows("layernorm_backward", M, N)) return rc;
+    if (N == 0) return M == 0 ? 0 : fail(DSV4_ERR_ARG, "layernorm_backward: the row length must be positive");
+    DSV4_REQUIRE_PTR("layernorm_backward", dw);
+    DSV4_REQUIRE_PTR("layernorm_backward", db);
+    if (M == 0) {   // sums over no rows
+        if (cudaMemsetAsync(dw, 0, (size_t)N * 4, cs(stream)) != cudaSuccess ||
+            cudaMemsetAsync(db, 0, (size_t)N * 4, cs(stream)) != cudaSuccess) {
+            check_launch("layernorm_backward");
+            return DSV4_ERR_LAUNCH;
+        }
+        return 0;
+    }
+    DSV4_REQUIRE_PTR("layernorm_backward", dy);
+    DSV4_REQUIRE_PTR("layernorm_backward", x);
+    DSV4_REQUIRE_PTR("layernorm_backward", mean);
+    DSV4_REQUIRE_PTR("layernorm_backward", rstd);
+    DSV4_REQUIRE_PTR("layernorm_backward", w);
+    DSV4_REQUIRE_PTR("layernorm_backward", dx);
+    DSV4_REQUIRE_PTR("layernorm_backward", workspace);
+    if (workspace_bytes < layernorm_backward_workspace(M, N) || (reinterpret_cast<uintptr_t>(workspace) & 3))
+        return fail(DSV4_ERR_ARG, "layernorm_backward: the workspace is smaller than dsv4_layernorm_backward_workspace or not 4-byte aligned");
+    return layernorm_backward(dy, x, mean, rstd, w, dres, dx, dw, db, workspace, M, N, cs(stream));
+}
+
 }  // extern "C"

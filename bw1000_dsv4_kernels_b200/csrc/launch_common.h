@@ -67,6 +67,15 @@ int moe_combine_exchange(const void* const* z_ranks, const int* const* slot_rank
                          int topk, int H, cudaStream_t st);
 int moe_push_rows(const int* dst_slot, int T, int topk, int tokens_per_rank, void* const* inbox_ranks, int G, int H,
                   void** row_ptr, cudaStream_t st);
+
+// ---- launchers implemented in layernorm.cu ------------------------------------------
+// res null: no residual; q null: bf16 output y
+int layernorm(void* res, const void* x, const void* w, const void* b, void* y, void* q, void* s, void* mean, void* rstd,
+              int M, int K, float eps, cudaStream_t st);
+int64_t layernorm_backward_workspace(int M, int K);
+int layernorm_backward(const void* dy, const void* x, const void* mean, const void* rstd, const void* w, const void* dres,
+                       void* dx, void* dw, void* db, void* workspace, int M, int K, cudaStream_t st);
+
 int read_device_status(cudaStream_t st, int* out);
 int read_row_status(int* out);  // status word of the row kernels (after the stream was synchronised)
 

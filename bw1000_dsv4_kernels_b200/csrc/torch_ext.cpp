@@ -599,6 +599,93 @@ int64_t device_status() {
     return v;
 }
 
+// ---- layer norm ---------------------------------------------------------------------
+// A workspace that lives only for the launches of one call: allocated on the stream that the launches go to, so that
+// the caching allocator hands it out again only behind them on that stream, whatever torch's current stream is.
+Tensor workspace_on(dsv4_stream_t stream, int64_t bytes, const Tensor& like) {
+    c10::cuda::CUDAStreamGuard on(c10::cuda::getStreamFromExternal(reinterpret_cast<cudaStream_t>(stream), like.device().index()));
+    return torch::empty({bytes}, like.options().dtype(torch::kUInt8));
+}
+
+struct NormShape {
+    int M, N;
+};
+NormShape check_norm(const Tensor& x, const Tensor& w, const Tensor& b, const c10::optional<Tensor>& res) {
+    check_cuda(x, "x", torch::kBFloat16);
+    check_cuda(w, "w", torch::kBFloat16);
+    check_cuda(b, "b", torch::kBFloat16);
+    check_same_device(x, w, "x/w");
+    check_same_device(x, b, "x/b");
+    TORCH_CHECK(x.is_contiguous() && w.is_contiguous() && b.is_contiguous(), "x, w and b must be contiguous");
+    TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "x must have at least one column");
+    TORCH_CHECK(w.numel() == x.size(-1) && b.numel() == x.size(-1), "w and b must have one entry per column of x");
+    if (res.has_value()) {
+        check_cuda(*res, "res", torch::kBFloat16);
+        check_same_device(x, *res, "x/res");
+        TORCH_CHECK(res->is_contiguous(), "res must be contiguous");
+        TORCH_CHECK(res->sizes() == x.sizes(), "res and x must have the same shape");
+    }
+    const Rows r = rows_of(x);
+    return {r.M, r.N};
+}
+
+// -> y, mean, rstd; res (optional) is overwritten with bf16(res + x), and that row is what is normalised
+std::vector<Tensor> layernorm_impl(c10::optional<Tensor> res, Tensor x, Tensor w, Tensor b, double eps, int64_t stream_ptr) {
+    const NormShape n = check_norm(x, w, b, res);
+    c10::cuda::CUDAGuard guard(x.device());
+    auto y = torch::empty_like(x);
+    auto mean = torch::empty({n.M}, x.options().dtype(torch::kFloat32)), rstd = torch::empty_like(mean);
+    check_status(launch_layernorm(res.has_value() ? res->data_ptr() : nullptr, x.data_ptr(), w.data_ptr(), b.data_ptr(),
+                                  y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), n.M, n.N, (float)eps, as_stream(stream_ptr)));
+    return {y, mean, rstd};
+}
+std::vector<Tensor> layernorm_stream(Tensor x, Tensor w, Tensor b, double eps, int64_t stream_ptr) {
+    return layernorm_impl(c10::nullopt, x, w, b, eps, stream_ptr);
+}
+std::vector<Tensor> add_layernorm_stream(Tensor res, Tensor x, Tensor w, Tensor b, double eps, int64_t stream_ptr) {
+    return layernorm_impl(res, x, w, b, eps, stream_ptr);
+}
+
+// -> q, s [M,1], mean, rstd
+std::vector<Tensor> layernorm_quant_impl(c10::optional<Tensor> res, Tensor x, Tensor w, Tensor b, double eps, int64_t stream_ptr) {
+    const NormShape n = check_norm(x, w, b, res);
+    c10::cuda::CUDAGuard guard(x.device());
+    auto q = torch::empty_like(x, x.options().dtype(torch::kInt8));
+    auto s = torch::empty({n.M}, x.options().dtype(torch::kFloat32));
+    auto mean = torch::empty_like(s), rstd = torch::empty_like(s);
+    check_status(launch_layernorm_quant(res.has_value() ? res->data_ptr() : nullptr, x.data_ptr(), w.data_ptr(), b.data_ptr(),
+                                        q.data_ptr(), s.data_ptr(), mean.data_ptr(), rstd.data_ptr(), n.M, n.N, (float)eps,
+                                        as_stream(stream_ptr)));
+    return {q, s.unsqueeze(-1), mean, rstd};
+}
+std::vector<Tensor> layernorm_quant_stream(Tensor x, Tensor w, Tensor b, double eps, int64_t stream_ptr) {
+    return layernorm_quant_impl(c10::nullopt, x, w, b, eps, stream_ptr);
+}
+std::vector<Tensor> add_layernorm_quant_stream(Tensor res, Tensor x, Tensor w, Tensor b, double eps, int64_t stream_ptr) {
+    return layernorm_quant_impl(res, x, w, b, eps, stream_ptr);
+}
+
+// -> dx, dw fp32, db fp32; x is the row that was normalised (the updated residual where there was one)
+std::vector<Tensor> layernorm_backward_stream(Tensor dy, Tensor x, Tensor mean, Tensor rstd, Tensor w,
+                                              c10::optional<Tensor> dres, int64_t stream_ptr) {
+    const NormShape n = check_norm(x, w, w, dres);
+    check_cuda(dy, "dy", torch::kBFloat16);
+    check_same_device(x, dy, "x/dy");
+    TORCH_CHECK(dy.is_contiguous() && dy.sizes() == x.sizes(), "dy must be contiguous with the shape of x");
+    const Tensor& mean_c = flat_scale(mean, n.M, "mean", x);
+    const Tensor& rstd_c = flat_scale(rstd, n.M, "rstd", x);
+    c10::cuda::CUDAGuard guard(x.device());
+    auto dx = torch::empty_like(x);
+    auto dw = torch::empty({n.N}, x.options().dtype(torch::kFloat32)), db = torch::empty_like(dw);
+    const dsv4_stream_t st = as_stream(stream_ptr);
+    const int64_t bytes = dsv4_layernorm_backward_workspace(n.M, n.N);
+    Tensor ws = workspace_on(st, bytes, x);
+    check_status(launch_layernorm_backward(dy.data_ptr(), x.data_ptr(), mean_c.data_ptr(), rstd_c.data_ptr(), w.data_ptr(),
+                                           dres.has_value() ? dres->data_ptr() : nullptr, dx.data_ptr(), dw.data_ptr(),
+                                           db.data_ptr(), ws.data_ptr(), bytes, n.M, n.N, st));
+    return {dx, dw, db};
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -702,6 +789,26 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         w8a8_gemm_allgather_stream(A, B, sa, sb, out, col0, peers, current_stream_ptr());
     });
     m.def("w8a8_gemm_allgather_stream", &w8a8_gemm_allgather_stream);
+    m.def("layernorm", [](Tensor x, Tensor w, Tensor b, double eps) {
+        return layernorm_stream(x, w, b, eps, current_stream_ptr());
+    });
+    m.def("layernorm_stream", &layernorm_stream);
+    m.def("add_layernorm", [](Tensor res, Tensor x, Tensor w, Tensor b, double eps) {
+        return add_layernorm_stream(res, x, w, b, eps, current_stream_ptr());
+    });
+    m.def("add_layernorm_stream", &add_layernorm_stream);
+    m.def("layernorm_quant", [](Tensor x, Tensor w, Tensor b, double eps) {
+        return layernorm_quant_stream(x, w, b, eps, current_stream_ptr());
+    });
+    m.def("layernorm_quant_stream", &layernorm_quant_stream);
+    m.def("add_layernorm_quant", [](Tensor res, Tensor x, Tensor w, Tensor b, double eps) {
+        return add_layernorm_quant_stream(res, x, w, b, eps, current_stream_ptr());
+    });
+    m.def("add_layernorm_quant_stream", &add_layernorm_quant_stream);
+    m.def("layernorm_backward", [](Tensor dy, Tensor x, Tensor mean, Tensor rstd, Tensor w, c10::optional<Tensor> dres) {
+        return layernorm_backward_stream(dy, x, mean, rstd, w, dres, current_stream_ptr());
+    }, py::arg("dy"), py::arg("x"), py::arg("mean"), py::arg("rstd"), py::arg("w"), py::arg("dres") = py::none());
+    m.def("layernorm_backward_stream", &layernorm_backward_stream);
     m.def("device_status", &device_status);
     m.def("abi_version", [] { return dsv4_abi_version(); });
     m.def("set_overlap_previous_kernel", [](bool on) { dsv4_set_overlap_previous_kernel(on ? 1 : 0); },

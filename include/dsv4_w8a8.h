@@ -256,6 +256,25 @@ DSV4_API int launch_grouped_gemm_scatter(const void* A, const void* W, const voi
 DSV4_API int launch_moe_push_rows(const int* dst_slot, int T, int topk, int tokens_per_rank,
                        void* const* inbox_ranks, int num_ranks, int H, void** row_ptr, dsv4_stream_t stream);
 
+/* ---- layer norm (no counterpart in the reference; beside launch_rmsnorm and launch_add_rmsnorm_quant) ----------
+ * a = x, or a = bf16(res + x) with res (bf16 [M,N]) overwritten by it when res is not null;
+ * mean, rstd fp32 [M] of a's rows (rstd = 1/sqrt(var + eps), population variance); y = (a - mean)*rstd*w + b.
+ * w, b bf16 [N].  Statistics are those of the row as it is stored in bf16, which is what the backward pass reads.
+ * launch_layernorm stores y as bf16; launch_layernorm_quant stores the codes and scales of launch_ptq on the
+ * unrounded y.  N must be positive. */
+DSV4_API int launch_layernorm(void* res, const void* x, const void* w, const void* b, void* y, void* mean, void* rstd,
+                       int M, int N, float eps, dsv4_stream_t stream);
+DSV4_API int launch_layernorm_quant(void* res, const void* x, const void* w, const void* b, void* q, void* s, void* mean,
+                       void* rstd, int M, int N, float eps, dsv4_stream_t stream);
+/* Gradients of launch_layernorm: x bf16 [M,N] is the row that was normalised (the updated residual where there was
+ * one), dy bf16 [M,N]; dres bf16 [M,N] or null is the gradient that reaches the same row past the norm and is added.
+ * dx bf16 [M,N]; dw, db fp32 [N], summed over the rows in an order that depends on M, N and the device only.
+ * workspace: dsv4_layernorm_backward_workspace(M, N) bytes of device memory, free again once the launch has run. */
+DSV4_API int64_t dsv4_layernorm_backward_workspace(int M, int N);
+DSV4_API int launch_layernorm_backward(const void* dy, const void* x, const void* mean, const void* rstd, const void* w,
+                       const void* dres, void* dx, void* dw, void* db, void* workspace, int64_t workspace_bytes, int M,
+                       int N, dsv4_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
