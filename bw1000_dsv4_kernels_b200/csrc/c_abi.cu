@@ -289,6 +289,28 @@ int launch_w8a8_gemm_ld(const void* A, const void* B, const void* sa, const void
     return gemm_i8(a, cs(stream));
 }
 
+int launch_w8a8_linear(const void* A, const void* B, const void* sa, const void* sb, const void* bias, int act,
+                       const void* residual, int64_t ldr, void* C, int64_t ldc, int M, int N, int K, dsv4_stream_t stream) {
+    if (act < DSV4_ACT_NONE || act > DSV4_ACT_SILU) return fail(DSV4_ERR_ARG, "w8a8_linear: unknown activation");
+    if (residual != nullptr && ldr < N) return fail(DSV4_ERR_ARG, "w8a8_linear: residual row stride smaller than N");
+    GemmArgs a{};
+    a.A = A; a.B = B; a.sa = static_cast<const float*>(sa); a.sb = static_cast<const float*>(sb); a.C = C;
+    a.offsets = nullptr; a.M = M; a.N = N; a.K = K; a.E = 1; a.ldc = ldc; a.sa_groups = 1; a.out_i32 = 0;
+    a.epilogue = 1; a.bias = bias; a.resid = residual; a.ldr = ldr; a.act = act;
+    return gemm_i8(a, cs(stream));
+}
+
+int launch_w8a8_gated(const void* A, const void* B, const void* sa, const void* sb, const void* bias, int act, void* C,
+                      int64_t ldc, int M, int I, int K, dsv4_stream_t stream) {
+    if (act <= DSV4_ACT_NONE || act > DSV4_ACT_SILU) return fail(DSV4_ERR_ARG, "w8a8_gated: unknown activation");
+    if (I > INT32_MAX / 2) return fail(DSV4_ERR_ARG, "w8a8_gated: 2 * I does not fit in int32");
+    GemmArgs a{};
+    a.A = A; a.B = B; a.sa = static_cast<const float*>(sa); a.sb = static_cast<const float*>(sb); a.C = C;
+    a.offsets = nullptr; a.M = M; a.N = I; a.K = K; a.E = 1; a.ldc = ldc; a.sa_groups = 1; a.out_i32 = 0;
+    a.epilogue = 2; a.bias = bias; a.act = act;
+    return gemm_i8(a, cs(stream));
+}
+
 int launch_layernorm(void* res, const void* x, const void* w, const void* b, void* y, void* mean, void* rstd, int M, int N,
                      float eps, dsv4_stream_t stream) {
     if (int rc = check_rows("layernorm", M, N)) return rc;

@@ -36,6 +36,9 @@ enum WaitSite : int {
     kWaitAccFull = 104,
 };
 
+// What is done with a finished accumulator (see gemm_i8_epilogues.cuh for all but the plain scaling)
+enum Epilogue : int { kEpiPlain = 0, kEpiLinear = 1, kEpiGated = 2 };
+
 struct Params {
     const float* sa;
     const float* sb;
@@ -63,6 +66,13 @@ struct Params {
     // test hook (never set through the public entry points): the producer issues no tile loads, so
     // every consumer wait of the launch runs out and the kernel leaves through its give-up path
     int withhold_loads;
+    // fused epilogues: bias per weight row, activation, residual with row stride ldr; `inter` is the number of gate
+    // rows of a gated weight [2 * inter, K] (N is then inter too)
+    const __nv_bfloat16* bias;
+    const __nv_bfloat16* resid;
+    int64_t ldr;
+    int act;
+    int inter;
 };
 
 template <int BN, int STAGES>
@@ -73,7 +83,8 @@ struct Smem {
     static constexpr int kTilesBytes = STAGES * kStageBytes;
     // after the tiles: one copy of the tile's column scales per drain warp, barriers, tmem slot
     static constexpr int kSbOff = kTilesBytes;
-    static constexpr int kBarOff = kSbOff + 4 * BN * 4;  // 8-byte aligned below
+    static constexpr int kBiasOff = kSbOff + 4 * BN * 4;   // the same for the biases of the fused epilogue
+    static constexpr int kBarOff = kBiasOff + 4 * BN * 4;  // 8-byte aligned below
     static constexpr int kNumBars = 2 * STAGES + 8;  // stage full/empty + up to 4 accumulator full/empty pairs
     static constexpr int kTmemSlotOff = ((kBarOff + 7) & ~7) + kNumBars * 8;
     static constexpr int kAbortOff = kTmemSlotOff + 4;

@@ -171,29 +171,29 @@ int sm_count() {
     return cached;
 }
 
-template <int BN, int STAGES>
+template <int BN, int STAGES, int EPI>
 int launch_variant(const CUtensorMap& tmA, const CUtensorMap& tmB, const Params& p, int max_tiles,
                    cudaStream_t st) {
     using L = Smem<BN, STAGES>;
     static_assert(L::kDynamic <= 227 * 1024, "shared memory limit");
     static bool opted_in[64] = {};
-    if (!opt_in_shared_memory(gemm_i8_kernel<BN, STAGES>, L::kDynamic, opted_in))
+    if (!opt_in_shared_memory(gemm_i8_kernel<BN, STAGES, EPI>, L::kDynamic, opted_in))
         return fail(DSV4_ERR_LAUNCH, "w8a8_gemm: cannot raise the dynamic shared memory limit");
     int grid = sm_count();
     if (grid <= 0) return fail(DSV4_ERR_LAUNCH, "w8a8_gemm: no CUDA device");
     if (max_tiles < grid) grid = max_tiles;
     if (grid < 1) grid = 1;
-    gemm_i8_kernel<BN, STAGES><<<grid, kThreads, L::kDynamic, st>>>(tmA, tmB, p);
+    gemm_i8_kernel<BN, STAGES, EPI><<<grid, kThreads, L::kDynamic, st>>>(tmA, tmB, p);
     return check_launch("w8a8_gemm");
 }
 
-template <int NTOK>
+template <int NTOK, int EPI>
 int launch_stream_variant(const CUtensorMap& tmW, const CUtensorMap& tmX, const Params& p, int n_tiles, int splits,
                           cudaStream_t st) {
     using L = StreamSmem<NTOK>;
     static_assert(L::kDynamic <= 227 * 1024, "shared memory limit");
     static bool opted_in[64] = {};
-    if (!opt_in_shared_memory(gemm_i8_stream_kernel<NTOK>, L::kDynamic, opted_in))
+    if (!opt_in_shared_memory(gemm_i8_stream_kernel<NTOK, EPI>, L::kDynamic, opted_in))
         return fail(DSV4_ERR_LAUNCH, "w8a8_gemm: cannot raise the dynamic shared memory limit");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(n_tiles * splits), 1, 1);
@@ -209,7 +209,7 @@ int launch_stream_variant(const CUtensorMap& tmW, const CUtensorMap& tmX, const 
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = overlap_previous_kernel() ? 2 : 1;
-    const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_stream_kernel<NTOK>, tmW, tmX, p);
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_stream_kernel<NTOK, EPI>, tmW, tmX, p);
     if (err != cudaSuccess) {
         cudaGetLastError();  // clear the sticky launch error
         static thread_local char msg[160];
@@ -238,7 +238,7 @@ int stream_pair_active_clusters(int splits) {
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_stream_pair_kernel, &cfg) != cudaSuccess) {
+        if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_stream_pair_kernel<>, &cfg) != cudaSuccess) {
             cudaGetLastError();
             n = -1;
         }
@@ -247,12 +247,13 @@ int stream_pair_active_clusters(int splits) {
     return cached[dev][splits] > 0 ? cached[dev][splits] : 0;
 }
 
+template <int EPI>
 int launch_stream_pair(const CUtensorMap& tmW, const CUtensorMap& tmX, const Params& p, int n_tiles, int splits,
                        cudaStream_t st) {
     using L = StreamPairSmem;
     static_assert(L::kDynamic <= 227 * 1024, "shared memory limit");
     static bool opted_in[64] = {};
-    if (!opt_in_shared_memory(gemm_i8_stream_pair_kernel, L::kDynamic, opted_in))
+    if (!opt_in_shared_memory(gemm_i8_stream_pair_kernel<EPI>, L::kDynamic, opted_in))
         return fail(DSV4_ERR_LAUNCH, "w8a8_gemm: cannot raise the dynamic shared memory limit");
     // a cluster must fit into one GPC: take the widest K split whose clusters all run in one wave
     while (splits > 1 && stream_pair_active_clusters(splits) < n_tiles) --splits;
@@ -270,7 +271,7 @@ int launch_stream_pair(const CUtensorMap& tmW, const CUtensorMap& tmX, const Par
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = overlap_previous_kernel() ? 2 : 1;
-    const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_stream_pair_kernel, tmW, tmX, p);
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_stream_pair_kernel<EPI>, tmW, tmX, p);
     if (err != cudaSuccess) {
         cudaGetLastError();  // clear the sticky launch error
         static thread_local char msg[160];
@@ -313,20 +314,21 @@ int make_store_map(CUtensorMap* map, void* base, uint64_t rows, uint64_t cols, u
     return 0;
 }
 
-template <int STAGES, bool TMA_STORE>
+template <int STAGES, bool TMA_STORE, int EPI = kEpiPlain>
 int launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap& tmB, const Params& p, const StoreMaps& smaps,
                         cudaStream_t st) {
     using L = PairSmem<STAGES, TMA_STORE>;
     static_assert(L::kDynamic <= 227 * 1024, "shared memory limit");
     static bool opted_in[64] = {};
-    if (!opt_in_shared_memory(gemm_i8_pair_kernel<STAGES, TMA_STORE>, L::kDynamic, opted_in))
+    if (!opt_in_shared_memory(gemm_i8_pair_kernel<STAGES, TMA_STORE, EPI>, L::kDynamic, opted_in))
         return fail(DSV4_ERR_LAUNCH, "w8a8_gemm: cannot raise the dynamic shared memory limit");
-    const int tiles = ((p.M + 255) / 256) * ((p.N + 255) / 256);
+    const int out_cols = EPI == kEpiGated ? 128 : 256;
+    const int tiles = ((p.M + 255) / 256) * ((p.N + out_cols - 1) / out_cols);
     int pairs = sm_count() / 2;
     if (pairs <= 0) return fail(DSV4_ERR_LAUNCH, "w8a8_gemm: no CUDA device");
     if (tiles < pairs) pairs = tiles;
     if (!overlap_previous_kernel()) {
-        gemm_i8_pair_kernel<STAGES, TMA_STORE><<<2 * pairs, kThreads, L::kDynamic, st>>>(tmA, tmB, p, smaps);
+        gemm_i8_pair_kernel<STAGES, TMA_STORE, EPI><<<2 * pairs, kThreads, L::kDynamic, st>>>(tmA, tmB, p, smaps);
         return check_launch("w8a8_gemm");
     }
     cudaLaunchConfig_t cfg = {};
@@ -339,7 +341,7 @@ int launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap& tmB, const Pa
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_pair_kernel<STAGES, TMA_STORE>, tmA, tmB, p, smaps);
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_pair_kernel<STAGES, TMA_STORE, EPI>, tmA, tmB, p, smaps);
     if (err != cudaSuccess) {
         cudaGetLastError();  // clear the sticky launch error
         static thread_local char msg[160];
@@ -347,6 +349,87 @@ int launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap& tmB, const Pa
         return fail(DSV4_ERR_LAUNCH, msg);
     }
     return check_launch("w8a8_gemm");
+}
+
+// Dense problems: the kernel by the number of tokens and tiles.  A gated weight [2 N, K] gives N outputs, and each weight
+// tile takes half its rows from the gates and half from the ups, so its N counts twice.
+template <int EPI>
+int gemm_i8_dense(const GemmArgs& a, const Params& p, int bn, cudaStream_t st) {
+    constexpr bool kGated = EPI == kEpiGated;
+    const int sms = sm_count();
+    const int w_rows = kGated ? 2 * a.N : a.N;
+    CUtensorMap tmA, tmB;
+    // Few tokens: stream the weight once, tokens on the MMA's N axis, K split over a cluster
+    if (a.M <= 256 && a.npeers == 0) {
+        const int k_blocks = (a.K + BK - 1) / BK;
+        if (a.M > 128 && w_rows >= 256) {
+            // 129..256 tokens: CTA pairs halve the token traffic per SM
+            const int pair_tiles = kGated ? (a.N + 127) / 128 : (a.N + 255) / 256;
+            int psplits = sms / (2 * pair_tiles);
+            if (psplits > 4) psplits = 4;
+            if (psplits > k_blocks) psplits = k_blocks;
+            if (psplits < 1) psplits = 1;
+            int rc5 = make_tile_map(&tmA, a.B, (uint64_t)w_rows, (uint64_t)a.K, kGated ? 64 : 128);   // weights
+            if (rc5) return rc5;
+            rc5 = make_tile_map(&tmB, a.A, (uint64_t)a.M, (uint64_t)a.K, 128);  // this CTA's half of the tokens
+            if (rc5) return rc5;
+            return launch_stream_pair<EPI>(tmA, tmB, p, pair_tiles, psplits, st);
+        }
+        const int n_tiles = kGated ? (a.N + 63) / 64 : (a.N + 127) / 128;
+        int splits = sms / n_tiles;
+        if (splits > 8) splits = 8;
+        if (splits > k_blocks) splits = k_blocks;
+        if (splits < 1) splits = 1;
+        const int ntok = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : a.M <= 128 ? 128 : 256;
+        int rc4 = make_tile_map(&tmA, a.B, (uint64_t)w_rows, (uint64_t)a.K, kGated ? 64 : 128);   // weights
+        if (rc4) return rc4;
+        rc4 = make_tile_map(&tmB, a.A, (uint64_t)a.M, (uint64_t)a.K, (uint32_t)ntok);  // tokens
+        if (rc4) return rc4;
+        switch (ntok) {
+            case 16: return launch_stream_variant<16, EPI>(tmA, tmB, p, n_tiles, splits, st);
+            case 32: return launch_stream_variant<32, EPI>(tmA, tmB, p, n_tiles, splits, st);
+            case 64: return launch_stream_variant<64, EPI>(tmA, tmB, p, n_tiles, splits, st);
+            case 128: return launch_stream_variant<128, EPI>(tmA, tmB, p, n_tiles, splits, st);
+            default: return launch_stream_variant<256, EPI>(tmA, tmB, p, n_tiles, splits, st);
+        }
+    }
+    // Dense problems with more than one 128-row tile go to the CTA-pair kernel, gated ones always
+    if (kGated || (a.M > 128 && (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256) >= sms / 4)) {
+        int rc2 = make_tile_map(&tmA, a.A, (uint64_t)a.M, (uint64_t)a.K, BM);
+        if (rc2) return rc2;
+        rc2 = make_tile_map(&tmB, a.B, (uint64_t)w_rows, (uint64_t)a.K, 128);
+        if (rc2) return rc2;
+        StoreMaps smaps;
+        smaps.count = 0;
+        if constexpr (EPI == kEpiPlain) {
+            if (a.npeers > 0) {
+                // fused all-gather: tile stores through tensor maps of this rank's slab and of every peer's
+                rc2 = make_store_map(&smaps.m[0], a.C, (uint64_t)a.M, (uint64_t)a.N, (uint64_t)p.ldc);
+                if (rc2) return rc2;
+                for (int d = 0; d < a.npeers; ++d) {
+                    rc2 = make_store_map(&smaps.m[1 + d], a.peerC[d], (uint64_t)a.M, (uint64_t)a.N, (uint64_t)p.ldc);
+                    if (rc2) return rc2;
+                }
+                smaps.count = 1 + a.npeers;
+                return launch_pair_variant<4, true>(tmA, tmB, p, smaps, st);
+            }
+        }
+        return launch_pair_variant<6, false, EPI>(tmA, tmB, p, smaps, st);
+    }
+    if constexpr (!kGated) {
+        int rc = make_tile_map(&tmA, a.A, (uint64_t)a.M, (uint64_t)a.K, BM);
+        if (rc) return rc;
+        rc = make_tile_map(&tmB, a.B, (uint64_t)w_rows, (uint64_t)a.K, (uint32_t)bn);
+        if (rc) return rc;
+        const int max_tiles = ((a.M + BM - 1) / BM) * ((a.N + bn - 1) / bn);
+        switch (bn) {
+            case 256: return launch_variant<256, 4, EPI>(tmA, tmB, p, max_tiles, st);
+            case 128: return launch_variant<128, 6, EPI>(tmA, tmB, p, max_tiles, st);
+            case 64: return launch_variant<64, 8, EPI>(tmA, tmB, p, max_tiles, st);
+            default: return launch_variant<32, 10, EPI>(tmA, tmB, p, max_tiles, st);
+        }
+    }
+    return 0;
 }
 
 }  // namespace
@@ -394,6 +477,11 @@ int gemm_i8(const GemmArgs& a, cudaStream_t st) {
     p.ldc = a.ldc > 0 ? a.ldc : a.N;
     p.sa_groups = a.sa_groups; p.out_i32 = a.out_i32;
     if (p.ldc < a.N) return fail(DSV4_ERR_ARG, "w8a8_gemm: ldc smaller than N");
+    p.bias = static_cast<const __nv_bfloat16*>(a.bias);
+    p.resid = static_cast<const __nv_bfloat16*>(a.resid);
+    p.ldr = a.ldr; p.act = a.act; p.inter = a.N;
+    if (a.epilogue != kEpiPlain && (grouped || a.out_i32 || a.npeers != 0))
+        return fail(DSV4_ERR_ARG, "w8a8_linear: the fused epilogues exist for the dense GEMM with bf16 output");
     {
         // groups of m-tiles whose rows of A (256 x K bytes each) take at most 32 MB, all about equally large
         const int tiles_m = (a.M + 255) / 256;
@@ -430,8 +518,8 @@ int gemm_i8(const GemmArgs& a, cudaStream_t st) {
     if (bn == 128 && (int64_t)tiles_m_bound * ((a.N + 127) / 128) < sms) bn = 64;
     if (bn == 64 && (int64_t)tiles_m_bound * ((a.N + 63) / 64) < sms) bn = 32;
 
-    CUtensorMap tmA, tmB;
     if (grouped) {
+        CUtensorMap tmB;
         if (a.masked_m != nullptr && (a.offsets != nullptr || a.max_m <= 0 || (int64_t)a.E * a.max_m != a.M))
             return fail(DSV4_ERR_ARG, "grouped_gemm_masked: needs max_m > 0, M == E * max_m and no expert_offsets");
         if (a.out_i32) return fail(DSV4_ERR_ARG, "grouped_gemm: raw accumulators exist only for the dense GEMM");
@@ -451,71 +539,10 @@ int gemm_i8(const GemmArgs& a, cudaStream_t st) {
         if (a.sa_groups == 1 && (a.row_ptr != nullptr || short_k)) return launch_wt_variant<false, true>(tmB, xmaps, p, st);
         return a.sa_groups != 1 ? launch_wt_variant<true>(tmB, xmaps, p, st) : launch_wt_variant<false>(tmB, xmaps, p, st);
     }
-    // Few tokens: stream the weight once, tokens on the MMA's N axis, K split over a cluster
-    if (a.M <= 256 && a.npeers == 0) {
-        const int k_blocks = (a.K + BK - 1) / BK;
-        if (a.M > 128 && a.N >= 256) {
-            // 129..256 tokens: CTA pairs halve the token traffic per SM
-            const int pair_tiles = (a.N + 255) / 256;
-            int psplits = sms / (2 * pair_tiles);
-            if (psplits > 4) psplits = 4;
-            if (psplits > k_blocks) psplits = k_blocks;
-            if (psplits < 1) psplits = 1;
-            int rc5 = make_tile_map(&tmA, a.B, b_rows, (uint64_t)a.K, 128);   // weights
-            if (rc5) return rc5;
-            rc5 = make_tile_map(&tmB, a.A, (uint64_t)a.M, (uint64_t)a.K, 128);  // this CTA's half of the tokens
-            if (rc5) return rc5;
-            return launch_stream_pair(tmA, tmB, p, pair_tiles, psplits, st);
-        }
-        const int n_tiles = (a.N + 127) / 128;
-        int splits = sms / n_tiles;
-        if (splits > 8) splits = 8;
-        if (splits > k_blocks) splits = k_blocks;
-        if (splits < 1) splits = 1;
-        const int ntok = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : a.M <= 128 ? 128 : 256;
-        int rc4 = make_tile_map(&tmA, a.B, b_rows, (uint64_t)a.K, 128);   // weights
-        if (rc4) return rc4;
-        rc4 = make_tile_map(&tmB, a.A, (uint64_t)a.M, (uint64_t)a.K, (uint32_t)ntok);  // tokens
-        if (rc4) return rc4;
-        switch (ntok) {
-            case 16: return launch_stream_variant<16>(tmA, tmB, p, n_tiles, splits, st);
-            case 32: return launch_stream_variant<32>(tmA, tmB, p, n_tiles, splits, st);
-            case 64: return launch_stream_variant<64>(tmA, tmB, p, n_tiles, splits, st);
-            case 128: return launch_stream_variant<128>(tmA, tmB, p, n_tiles, splits, st);
-            default: return launch_stream_variant<256>(tmA, tmB, p, n_tiles, splits, st);
-        }
-    }
-    // Dense problems with more than one 128-row tile go to the CTA-pair kernel
-    if (a.M > 128 && (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256) >= sms / 4) {
-        int rc2 = make_tile_map(&tmA, a.A, (uint64_t)a.M, (uint64_t)a.K, BM);
-        if (rc2) return rc2;
-        rc2 = make_tile_map(&tmB, a.B, b_rows, (uint64_t)a.K, 128);
-        if (rc2) return rc2;
-        StoreMaps smaps;
-        smaps.count = 0;
-        if (a.npeers > 0) {
-            // fused all-gather: tile stores through tensor maps of this rank's slab and of every peer's
-            rc2 = make_store_map(&smaps.m[0], a.C, (uint64_t)a.M, (uint64_t)a.N, (uint64_t)p.ldc);
-            if (rc2) return rc2;
-            for (int d = 0; d < a.npeers; ++d) {
-                rc2 = make_store_map(&smaps.m[1 + d], a.peerC[d], (uint64_t)a.M, (uint64_t)a.N, (uint64_t)p.ldc);
-                if (rc2) return rc2;
-            }
-            smaps.count = 1 + a.npeers;
-            return launch_pair_variant<4, true>(tmA, tmB, p, smaps, st);
-        }
-        return launch_pair_variant<6, false>(tmA, tmB, p, smaps, st);
-    }
-    int rc = make_tile_map(&tmA, a.A, (uint64_t)a.M, (uint64_t)a.K, BM);
-    if (rc) return rc;
-    rc = make_tile_map(&tmB, a.B, b_rows, (uint64_t)a.K, (uint32_t)bn);
-    if (rc) return rc;
-    const int max_tiles = tiles_m_bound * ((a.N + bn - 1) / bn);
-    switch (bn) {
-        case 256: return launch_variant<256, 4>(tmA, tmB, p, max_tiles, st);
-        case 128: return launch_variant<128, 6>(tmA, tmB, p, max_tiles, st);
-        case 64: return launch_variant<64, 8>(tmA, tmB, p, max_tiles, st);
-        default: return launch_variant<32, 10>(tmA, tmB, p, max_tiles, st);
+    switch (a.epilogue) {
+        case kEpiLinear: return gemm_i8_dense<kEpiLinear>(a, p, bn, st);
+        case kEpiGated: return gemm_i8_dense<kEpiGated>(a, p, bn, st);
+        default: return gemm_i8_dense<kEpiPlain>(a, p, bn, st);
     }
 }
 

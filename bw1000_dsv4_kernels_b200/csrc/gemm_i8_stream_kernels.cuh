@@ -4,6 +4,7 @@
 #define W8A8_GEMM_I8_STREAM_KERNELS_CUH
 
 #include "gemm_i8_common.cuh"
+#include "gemm_i8_epilogues.cuh"
 
 namespace w8a8 {
 namespace {
@@ -107,8 +108,8 @@ struct StreamSmem {
     static constexpr int kTilesBytes = kStages * kStageBytes;
     static constexpr int kPartialBytes = NTOK * 128 * 4;
     static_assert(kPartialBytes <= kTilesBytes, "the partial tile reuses the stage ring");
-    static constexpr int kScaleOff = kTilesBytes;             // token scales [256], then the tile's 128 channel scales
-    static constexpr int kBarOff = kScaleOff + (256 + 128) * 4;
+    static constexpr int kScaleOff = kTilesBytes;             // token scales [256], the tile's 128 channel scales and biases
+    static constexpr int kBarOff = kScaleOff + (256 + 128 + 128) * 4;
     static constexpr int kNumBars = 2 * kStages + 1;
     static constexpr int kTmemSlotOff = kBarOff + kNumBars * 8;
     static constexpr int kAbortOff = kTmemSlotOff + 4;
@@ -118,15 +119,36 @@ struct StreamSmem {
 
 // The drain warps (threads 64..191) have nothing to do while the weight streams: they fetch the scales the
 // epilogue needs.  Activation scales may come from the kernel before this one, hence the dependency wait.
+template <int EPI>
 __device__ __forceinline__ void stage_scales(const Params& p, float* sa_s, float* sb_s, int ntok, int n0) {
     ptx::grid_dependency_wait();
     if (p.out_i32) return;
     const int t = threadIdx.x - 64;
     for (int i = t; i < ntok; i += kDrainThreads) sa_s[i] = i < p.M ? __ldg(p.sa + i) : 0.0f;
-    for (int j = t; j < 128; j += kDrainThreads) sb_s[j] = n0 + j < p.N ? __ldg(p.sb + n0 + j) : 0.0f;
+    if constexpr (EPI == kEpiPlain) {
+        for (int j = t; j < 128; j += kDrainThreads) sb_s[j] = n0 + j < p.N ? __ldg(p.sb + n0 + j) : 0.0f;
+    } else {
+        // a gated tile is 64 gate rows, then the 64 up rows of the same outputs
+        float* bias_s = sb_s + 128;
+        for (int j = t; j < 128; j += kDrainThreads) {
+            const bool up = EPI == kEpiGated && j >= 64;
+            const int c = up ? p.inter + n0 + (j - 64) : n0 + j;
+            const bool ok = c < (up ? 2 * p.inter : p.N);
+            sb_s[j] = ok ? __ldg(p.sb + c) : 0.0f;
+            bias_s[j] = ok && p.bias != nullptr ? __bfloat162float(p.bias[c]) : 0.0f;
+        }
+    }
 }
 
-template <int NTOK>
+// The weight rows of a tile: 128 consecutive ones, or (gated) 64 gate rows and the 64 up rows of the same outputs, which
+// take two loads; the tensor map's box has that many rows.
+template <int EPI>
+__device__ __forceinline__ void load_weight_tile(uint32_t dst, const CUtensorMap* tmW, int k, int n0, int inter, uint32_t bar) {
+    ptx::tma_load_2d(dst, tmW, k, n0, bar);
+    if constexpr (EPI == kEpiGated) ptx::tma_load_2d(dst + 64 * BK, tmW, k, inter + n0, bar);
+}
+
+template <int NTOK, int EPI = kEpiPlain>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                       const Params p) {
@@ -152,7 +174,7 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
     const int S = (int)ptx::cluster_nctarank();
     const int split = (int)ptx::cluster_ctarank();
     const int nt = blockIdx.x / S;
-    const int n0 = nt * 128;
+    const int n0 = nt * (EPI == kEpiGated ? 64 : 128);
     constexpr uint32_t kTmemCols = NTOK < 32 ? 32 : NTOK;
 
     // this CTA's share of the K blocks
@@ -177,7 +199,7 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
         // this kernel was launched to overlap its predecessor).
         for (int i = 0; i < prologue; ++i) {
             ptx::mbar_arrive_expect_tx(full_bar(i), L::kStageBytes);
-            ptx::tma_load_2d(tiles_base + i * L::kStageBytes, &tmW, (kb0 + i) * BK, n0, full_bar(i));
+            load_weight_tile<EPI>(tiles_base + i * L::kStageBytes, &tmW, (kb0 + i) * BK, n0, p.inter, full_bar(i));
         }
         ptx::grid_dependency_wait();
         for (int i = 0; i < prologue; ++i)
@@ -204,7 +226,7 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
                 }
                 const uint32_t w_dst = tiles_base + stage * L::kStageBytes;
                 ptx::mbar_arrive_expect_tx(full_bar(stage), L::kStageBytes);
-                ptx::tma_load_2d(w_dst, &tmW, kb * BK, n0, full_bar(stage));
+                load_weight_tile<EPI>(w_dst, &tmW, kb * BK, n0, p.inter, full_bar(stage));
                 ptx::tma_load_2d(w_dst + L::kWBytes, &tmX, kb * BK, 0, full_bar(stage));
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
@@ -236,7 +258,7 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
         }
     } else {
         // drain warps: the epilogue's scales first, then accumulator -> shared partial
-        stage_scales(p, sa_s, sb_s, NTOK, n0);
+        stage_scales<EPI>(p, sa_s, sb_s, NTOK, n0);
         const int quarter = warp & 3;
         const int wrow = quarter * 32 + lane;  // weight row inside the tile = TMEM lane
         if (kb1 > kb0) {
@@ -291,7 +313,11 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
         uint32_t peer_base[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) peer_base[r] = ptx::map_to_cta(my_partial, r < S ? r : 0);
-        reduce_partials_and_store<8, 4>(p, peer_base, S, cols_lo, cols_hi, n0, threadIdx.x, kThreads, sa_s, sb_s);
+        if constexpr (EPI == kEpiPlain)
+            reduce_partials_and_store<8, 4>(p, peer_base, S, cols_lo, cols_hi, n0, threadIdx.x, kThreads, sa_s, sb_s);
+        else
+            reduce_partials_fused<8, EPI == kEpiGated ? 2 : 4, EPI == kEpiGated>(p, peer_base, S, cols_lo, cols_hi, n0,
+                                                                                 threadIdx.x, kThreads, sa_s, sb_s, sb_s + 128);
     }
 
     // nobody leaves while a peer may still read its shared memory
@@ -322,8 +348,8 @@ struct StreamPairSmem {
     static constexpr int kTilesBytes = kStages * kStageBytes;
     static constexpr int kPartialBytes = 256 * 128 * 4;
     static_assert(kPartialBytes <= kTilesBytes, "the partial tile reuses the stage ring");
-    static constexpr int kScaleOff = kTilesBytes;             // token scales [256], then the tile's 128 channel scales
-    static constexpr int kBarOff = kScaleOff + (256 + 128) * 4;
+    static constexpr int kScaleOff = kTilesBytes;             // token scales [256], the tile's 128 channel scales and biases
+    static constexpr int kBarOff = kScaleOff + (256 + 128 + 128) * 4;
     static constexpr int kNumBars = 2 * kStages + 1;
     static constexpr int kTmemSlotOff = kBarOff + kNumBars * 8;
     static constexpr int kAbortOff = kTmemSlotOff + 4;
@@ -331,6 +357,7 @@ struct StreamPairSmem {
     static constexpr int kDynamic = kTotal + 1024;
 };
 
+template <int EPI = kEpiPlain>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_i8_stream_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                            const Params p) {
@@ -359,7 +386,12 @@ gemm_i8_stream_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
     const uint32_t leader = (uint32_t)(crank & ~1);
     const uint16_t pair_mask = (uint16_t)(0x3u << leader);
     const int nt = blockIdx.x / csize;
-    const int n0 = nt * 256 + half * 128;         // this CTA's weight rows
+    // this CTA's outputs: 128 weight rows, or the 64 gates and 64 ups of 64 gated outputs
+    const int n0 = EPI == kEpiGated ? nt * 128 + half * 64 : nt * 256 + half * 128;
+    auto load_weights = [&](uint32_t dst, int k, uint32_t bar) {
+        ptx::tma_load_2d_pair(dst, &tmW, k, n0, bar);
+        if constexpr (EPI == kEpiGated) ptx::tma_load_2d_pair(dst + 64 * BK, &tmW, k, p.inter + n0, bar);
+    };
     constexpr uint32_t kTmemCols = NTOK;
 
     const int k_blocks = (p.K + BK - 1) / BK;
@@ -396,7 +428,7 @@ gemm_i8_stream_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
             for (int i = 0; i < prologue; ++i) {
                 const uint32_t leader_full = ptx::map_to_cta(full_bar(i), leader);
                 if (half == 0) ptx::mbar_arrive_expect_tx(full_bar(i), 2 * L::kStageBytes);
-                ptx::tma_load_2d_pair(tiles_base + i * L::kStageBytes, &tmW, (kb0 + i) * BK, n0, leader_full);
+                load_weights(tiles_base + i * L::kStageBytes, (kb0 + i) * BK, leader_full);
             }
             ptx::grid_dependency_wait();
             for (int i = 0; i < prologue; ++i)
@@ -413,7 +445,7 @@ gemm_i8_stream_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
                 const uint32_t w_dst = tiles_base + stage * L::kStageBytes;
                 const uint32_t leader_full = ptx::map_to_cta(full_bar(stage), leader);
                 if (half == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * L::kStageBytes);
-                ptx::tma_load_2d_pair(w_dst, &tmW, kb * BK, n0, leader_full);
+                load_weights(w_dst, kb * BK, leader_full);
                 ptx::tma_load_2d_pair(w_dst + L::kWBytes, &tmX, kb * BK, half * 128, leader_full);
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
@@ -446,7 +478,7 @@ gemm_i8_stream_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
     } else {
         // drain warps of both CTAs: the epilogue's scales first, then the accumulator of this CTA's 128 weight
         // rows -> shared partial
-        stage_scales(p, sa_s, sb_s, NTOK, n0);
+        stage_scales<EPI>(p, sa_s, sb_s, NTOK, n0);
         const int quarter = warp & 3;
         const int wrow = quarter * 32 + lane;
         if (kb1 > kb0) {
@@ -490,7 +522,11 @@ gemm_i8_stream_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
         uint32_t peer_base[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) peer_base[r] = ptx::map_to_cta(my_partial, (uint32_t)(2 * (r < S ? r : 0) + half));
-        reduce_partials_and_store<4, 8>(p, peer_base, S, cols_lo, cols_hi, n0, threadIdx.x, kThreads, sa_s, sb_s);
+        if constexpr (EPI == kEpiPlain)
+            reduce_partials_and_store<4, 8>(p, peer_base, S, cols_lo, cols_hi, n0, threadIdx.x, kThreads, sa_s, sb_s);
+        else
+            reduce_partials_fused<4, EPI == kEpiGated ? 4 : 8, EPI == kEpiGated>(p, peer_base, S, cols_lo, cols_hi, n0,
+                                                                                 threadIdx.x, kThreads, sa_s, sb_s, sb_s + 128);
     }
 
     // nobody leaves while a peer may still read its shared memory

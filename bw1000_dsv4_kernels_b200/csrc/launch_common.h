@@ -42,6 +42,12 @@ struct GemmArgs {
     void* const* row_ptr = nullptr;  // grouped GEMM, per-token scales: device array, one destination row per result row (C unused)
     void* peerC[7];       // fused all-gather: the other ranks' mapped output slabs
     int npeers;           // 0 = none
+    // fused epilogue (enum Epilogue in gemm_i8_common.cuh): 1 linear, 2 gated (B is [2 N, K], gates first)
+    int epilogue = 0;
+    const void* bias = nullptr;    // bf16, one per row of B
+    const void* resid = nullptr;   // bf16 [M, N] with row stride ldr
+    int64_t ldr = 0;
+    int act = 0;                   // enum Activation in activations.cuh
     // Test hook, zero through every public entry point: the tile producers of the launch issue no
     // loads and every bounded wait gives up after test_wait_limit_ns, so the kernel's give-up path runs.
     int test_withhold_loads = 0;

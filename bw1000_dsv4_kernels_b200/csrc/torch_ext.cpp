@@ -599,6 +599,68 @@ int64_t device_status() {
     return v;
 }
 
+// ---- fused linear and gated projection ------------------------------------------------
+int activation_of(const std::string& name) {
+    static const char* const names[] = {"none", "relu", "gelu", "gelu_tanh", "silu"};
+    for (int i = 0; i < 5; ++i)
+        if (name == names[i]) return i;
+    TORCH_CHECK(false, "unknown activation '", name, "': none, relu, gelu, gelu_tanh or silu");
+}
+const void* bias_ptr(const c10::optional<Tensor>& bias, int64_t n, const Tensor& operand) {
+    if (!bias.has_value()) return nullptr;
+    check_cuda(*bias, "bias", torch::kBFloat16);
+    check_same_device(*bias, operand, "bias");
+    TORCH_CHECK(bias->is_contiguous() && bias->numel() == n, "bias must be contiguous with ", n, " entries");
+    return bias->data_ptr();
+}
+// row stride of a bf16 [m, n] tensor whose rows are dense
+int64_t row_stride(const Tensor& t, const char* name, int64_t m, int64_t n, const Tensor& operand) {
+    check_cuda(t, name, torch::kBFloat16);
+    check_same_device(t, operand, name);
+    TORCH_CHECK(t.dim() == 2 && t.size(0) == m && t.size(1) == n, name, " must be [", m, ", ", n, "]");
+    TORCH_CHECK(n <= 1 || t.stride(1) == 1, name, " must have unit stride in the last dimension");
+    TORCH_CHECK(m <= 1 || t.stride(0) >= n, name, " must not have overlapping or broadcast rows");
+    return m <= 1 ? n : t.stride(0);
+}
+
+Tensor w8a8_linear_stream(Tensor A, Tensor B, Tensor sa, Tensor sb, c10::optional<Tensor> bias, const std::string& act,
+                          c10::optional<Tensor> residual, int64_t stream_ptr) {
+    const GemmShape g = check_gemm_operands(A, B);
+    const Tensor& sa_c = flat_scale(sa, g.M, "sa", A);
+    const Tensor& sb_c = flat_scale(sb, g.N, "sb", A);
+    const void* bp = bias_ptr(bias, g.N, A);
+    const int act_id = activation_of(act);
+    const int64_t ldr = residual.has_value() ? row_stride(*residual, "residual", g.M, g.N, A) : 0;
+    c10::cuda::CUDAGuard guard(A.device());
+    auto C = torch::empty({g.M, g.N}, A.options().dtype(torch::kBFloat16));
+    check_status(launch_w8a8_linear(A.data_ptr(), B.data_ptr(), sa_c.data_ptr(), sb_c.data_ptr(), bp, act_id,
+                                    residual.has_value() ? residual->data_ptr() : nullptr, ldr, C.data_ptr(), g.N, g.M, g.N,
+                                    g.K, as_stream(stream_ptr)));
+    return C;
+}
+
+int gated_act(const std::string& act) {
+    const int id = activation_of(act);
+    TORCH_CHECK(id != DSV4_ACT_NONE, "a gated projection needs an activation: relu, gelu, gelu_tanh or silu");
+    return id;
+}
+
+// W13 int8 [2*I, K], the I gate rows first -> act(gate) * up, bf16 [M, I]
+Tensor w8a8_gated_stream(Tensor A, Tensor W13, Tensor sa, Tensor s13, c10::optional<Tensor> bias, const std::string& act,
+                         int64_t stream_ptr) {
+    const GemmShape g = check_gemm_operands(A, W13);
+    TORCH_CHECK(g.N % 2 == 0, "W13 must hold as many up rows as gate rows, got ", g.N, " rows");
+    const Tensor& sa_c = flat_scale(sa, g.M, "sa", A);
+    const Tensor& sb_c = flat_scale(s13, g.N, "s13", A);
+    const void* bp = bias_ptr(bias, g.N, A);
+    const int act_id = gated_act(act);
+    c10::cuda::CUDAGuard guard(A.device());
+    auto C = torch::empty({g.M, g.N / 2}, A.options().dtype(torch::kBFloat16));
+    check_status(launch_w8a8_gated(A.data_ptr(), W13.data_ptr(), sa_c.data_ptr(), sb_c.data_ptr(), bp, act_id, C.data_ptr(),
+                                   g.N / 2, g.M, g.N / 2, g.K, as_stream(stream_ptr)));
+    return C;
+}
+
 // ---- layer norm ---------------------------------------------------------------------
 // A workspace that lives only for the launches of one call: allocated on the stream that the launches go to, so that
 // the caching allocator hands it out again only behind them on that stream, whatever torch's current stream is.
@@ -789,6 +851,16 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         w8a8_gemm_allgather_stream(A, B, sa, sb, out, col0, peers, current_stream_ptr());
     });
     m.def("w8a8_gemm_allgather_stream", &w8a8_gemm_allgather_stream);
+    m.def("w8a8_linear", [](Tensor A, Tensor B, Tensor sa, Tensor sb, c10::optional<Tensor> bias, const std::string& act,
+                            c10::optional<Tensor> residual) {
+        return w8a8_linear_stream(A, B, sa, sb, bias, act, residual, current_stream_ptr());
+    }, py::arg("A"), py::arg("B"), py::arg("sa"), py::arg("sb"), py::arg("bias") = py::none(), py::arg("act") = "none",
+       py::arg("residual") = py::none());
+    m.def("w8a8_linear_stream", &w8a8_linear_stream);
+    m.def("w8a8_gated", [](Tensor A, Tensor W13, Tensor sa, Tensor s13, c10::optional<Tensor> bias, const std::string& act) {
+        return w8a8_gated_stream(A, W13, sa, s13, bias, act, current_stream_ptr());
+    }, py::arg("A"), py::arg("W13"), py::arg("sa"), py::arg("s13"), py::arg("bias") = py::none(), py::arg("act") = "silu");
+    m.def("w8a8_gated_stream", &w8a8_gated_stream);
     m.def("layernorm", [](Tensor x, Tensor w, Tensor b, double eps) {
         return layernorm_stream(x, w, b, eps, current_stream_ptr());
     });

@@ -256,6 +256,19 @@ DSV4_API int launch_grouped_gemm_scatter(const void* A, const void* W, const voi
 DSV4_API int launch_moe_push_rows(const int* dst_slot, int T, int topk, int tokens_per_rank,
                        void* const* inbox_ranks, int num_ranks, int H, void** row_ptr, dsv4_stream_t stream);
 
+/* ---- fused W8A8 linear and gated projection (no counterpart in the reference; beside launch_w8a8_gemm) ----------
+ * z = (float(A B^T) * sa[row]) * sb[channel] + bias[channel] in fp32; bias bf16 or null; A int8 [M,K], B int8, K % 16 == 0,
+ * A and B 16-byte aligned.
+ * launch_w8a8_linear: B [N,K]; C bf16 [M, ldc] = act(z) + residual, residual bf16 with row stride ldr or null; C and
+ *   residual may be the same array with the same stride.  Without bias, activation and residual: the bits of
+ *   launch_w8a8_gemm.
+ * launch_w8a8_gated: B [2*I,K], the I gate rows first; C bf16 [M, ldc >= I] = act(z[:, :I]) * z[:, I:], one kernel. */
+enum { DSV4_ACT_NONE = 0, DSV4_ACT_RELU = 1, DSV4_ACT_GELU = 2, DSV4_ACT_GELU_TANH = 3, DSV4_ACT_SILU = 4 };
+DSV4_API int launch_w8a8_linear(const void* A, const void* B, const void* sa, const void* sb, const void* bias, int act,
+                       const void* residual, int64_t ldr, void* C, int64_t ldc, int M, int N, int K, dsv4_stream_t stream);
+DSV4_API int launch_w8a8_gated(const void* A, const void* B, const void* sa, const void* sb, const void* bias, int act,
+                       void* C, int64_t ldc, int M, int I, int K, dsv4_stream_t stream);
+
 /* ---- layer norm (no counterpart in the reference; beside launch_rmsnorm and launch_add_rmsnorm_quant) ----------
  * a = x, or a = bf16(res + x) with res (bf16 [M,N]) overwritten by it when res is not null;
  * mean, rstd fp32 [M] of a's rows (rstd = 1/sqrt(var + eps), population variance); y = (a - mean)*rstd*w + b.
