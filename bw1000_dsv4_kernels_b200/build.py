@@ -20,10 +20,10 @@ LIB_NAME = "libdsv4_w8a8.so"
 LIB_PATH = os.path.join(HERE, LIB_NAME)
 EXT_PATH = os.path.join(HERE, "dsv4_native_ext" + sysconfig.get_config_var("EXT_SUFFIX"))
 
-CUDA_SOURCES = ["rowwise_quant.cu", "gemm_i8_sm100.cu", "moe_segments.cu", "layernorm.cu", "c_abi.cu"]
+CUDA_SOURCES = ["rowwise_quant.cu", "gemm_i8_sm100.cu", "moe_segments.cu", "layernorm.cu", "w8a8_backward.cu", "c_abi.cu"]
 CUDA_HEADERS = ["w8a8_arith.cuh", "sm100_ptx.cuh", "launch_common.h", "gemm_i8_common.cuh", "gemm_i8_tile_kernel.cuh",
                 "gemm_i8_pair_kernel.cuh", "gemm_i8_wt_kernel.cuh", "gemm_i8_stream_kernels.cuh",
-                "gemm_i8_epilogues.cuh", "activations.cuh"]
+                "gemm_i8_epilogues.cuh", "gemm_i8_grad_kernel.cuh", "gradient_digits.cuh", "activations.cuh"]
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -53,7 +53,7 @@ def build_cuda_lib(force: bool = False, verbose: bool = False, ptxas_info: bool 
     # -fmad=false: a multiply and an add that the sources write as two rounded steps must stay two
     # instructions (fused forms are written explicitly where they are meant)
     cmd = [nvcc, *ARCH_FLAGS, "-lineinfo", "-O3", "-fmad=false", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
-           "-Xcompiler", "-fvisibility=hidden", "--threads", "4", "-o", LIB_PATH, *srcs]
+           "-Xcompiler", "-fvisibility=hidden", "--threads", "0", "--split-compile", "0", "-o", LIB_PATH, *srcs]
     if ptxas_info:
         cmd[1:1] = ["-Xptxas", "-v"]
     _run(cmd, verbose)

@@ -311,6 +311,65 @@ int launch_w8a8_gated(const void* A, const void* B, const void* sa, const void* 
     return gemm_i8(a, cs(stream));
 }
 
+int64_t dsv4_w8a8_backward_workspace(int M, int weight_rows, int act, int want_dbias) {
+    if (M <= 0 || weight_rows <= 0) return 0;
+    return w8a8_backward_workspace(M, weight_rows, act != DSV4_ACT_NONE, want_dbias != 0);
+}
+
+static int backward_entry(const char* op, bool gated, const void* dy, int64_t ldy, const void* A, const void* B, const void* sa,
+                          const void* sb, const void* bias, int act, void* dx, void* dbias, void* workspace,
+                          int64_t workspace_bytes, int M, int N, int K, dsv4_stream_t stream) {
+    char msg[160];
+    auto bad = [&](const char* what) {
+        std::snprintf(msg, sizeof msg, "%s: %s", op, what);
+        return fail(DSV4_ERR_ARG, msg);
+    };
+    if (M < 0 || N < 0 || K < 0) return bad("negative size");
+    if (act < DSV4_ACT_NONE || act > DSV4_ACT_SILU || (gated && act == DSV4_ACT_NONE)) return bad("unknown activation");
+    if (N == 0) {   // no weight rows: nothing reaches the activations
+        if (M == 0 || K == 0) return 0;
+        if (dx == nullptr) return bad("null pointer dx");
+        if (cudaMemsetAsync(dx, 0, (size_t)M * K * 2, cs(stream)) != cudaSuccess) { check_launch(op); return DSV4_ERR_LAUNCH; }
+        return 0;
+    }
+    if (M == 0) {   // sums over no rows
+        if (dbias != nullptr && cudaMemsetAsync(dbias, 0, (size_t)N * 4, cs(stream)) != cudaSuccess)
+            { check_launch(op); return DSV4_ERR_LAUNCH; }
+        return 0;
+    }
+    if (K == 0 || K % 16 != 0) return bad("K must be a positive multiple of 16 (TMA row stride)");
+    if (N > 131071) return bad("more than 131071 weight rows");
+    if (dy == nullptr || B == nullptr || sb == nullptr || dx == nullptr || workspace == nullptr) return bad("null pointer");
+    if (act != DSV4_ACT_NONE && (A == nullptr || sa == nullptr)) return bad("null pointer A or sa");
+    if ((reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(B) & 15)) return bad("A and B must be 16-byte aligned");
+    if (ldy < (gated ? N / 2 : N)) return bad("gradient row stride smaller than its row");
+    if ((int64_t)2 * M > INT32_MAX) return bad("too many rows");
+    if (workspace_bytes < w8a8_backward_workspace(M, N, act != DSV4_ACT_NONE, dbias != nullptr) ||
+        (reinterpret_cast<uintptr_t>(workspace) & 15))
+        return bad("the workspace is smaller than dsv4_w8a8_backward_workspace or not 16-byte aligned");
+    BackwardArgs a;
+    a.dy = dy; a.ldy = ldy; a.A = A; a.B = B;
+    a.sa = static_cast<const float*>(sa); a.sb = static_cast<const float*>(sb);
+    a.bias = bias; a.act = act; a.gated = gated; a.dx = dx; a.dbias = static_cast<float*>(dbias);
+    a.M = M; a.N = N; a.K = K;
+    return w8a8_backward(a, workspace, cs(stream));
+}
+
+int launch_w8a8_linear_backward(const void* dy, int64_t ldy, const void* A, const void* B, const void* sa, const void* sb,
+                                const void* bias, int act, void* dx, void* dbias, void* workspace, int64_t workspace_bytes,
+                                int M, int N, int K, dsv4_stream_t stream) {
+    return backward_entry("w8a8_linear_backward", false, dy, ldy, A, B, sa, sb, bias, act, dx, dbias, workspace,
+                          workspace_bytes, M, N, K, stream);
+}
+
+int launch_w8a8_gated_backward(const void* dh, int64_t ldh, const void* A, const void* B, const void* sa, const void* sb,
+                               const void* bias, int act, void* dx, void* dbias, void* workspace, int64_t workspace_bytes,
+                               int M, int I, int K, dsv4_stream_t stream) {
+    if (I > INT32_MAX / 2) return fail(DSV4_ERR_ARG, "w8a8_gated_backward: 2 * I does not fit in int32");
+    return backward_entry("w8a8_gated_backward", true, dh, ldh, A, B, sa, sb, bias, act, dx, dbias, workspace,
+                          workspace_bytes, M, 2 * I, K, stream);
+}
+
 int launch_layernorm(void* res, const void* x, const void* w, const void* b, void* y, void* mean, void* rstd, int M, int N,
                      float eps, dsv4_stream_t stream) {
     if (int rc = check_rows("layernorm", M, N)) return rc;

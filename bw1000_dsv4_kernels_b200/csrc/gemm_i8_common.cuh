@@ -37,7 +37,8 @@ enum WaitSite : int {
 };
 
 // What is done with a finished accumulator (see gemm_i8_epilogues.cuh for all but the plain scaling)
-enum Epilogue : int { kEpiPlain = 0, kEpiLinear = 1, kEpiGated = 2 };
+enum Epilogue : int { kEpiPlain = 0, kEpiLinear = 1, kEpiGated = 2, kEpiLinearGrad = 3, kEpiGatedGrad = 4 };
+__host__ __device__ constexpr bool is_gated(int epi) { return epi == kEpiGated || epi == kEpiGatedGrad; }
 
 struct Params {
     const float* sa;
@@ -73,6 +74,9 @@ struct Params {
     int64_t ldr;
     int act;
     int inter;
+    // gradient epilogues: resid is the incoming gradient (dy or dh), C the fp32 gradient of z with row stride ldc, and
+    // row_top[row] collects the largest |dz * sb| of the row as the bits of a non-negative float
+    unsigned* row_top;
 };
 
 template <int BN, int STAGES>

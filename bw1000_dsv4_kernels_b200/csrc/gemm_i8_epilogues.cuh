@@ -3,6 +3,9 @@
 //   linear       z = (acc * sa) * sb + bias;  y = act(z) + residual            -> bf16
 //   gated        the tile holds a block of gate columns and the same block of up columns (two loads of weight rows, I
 //                rows apart), so one thread has g and u of the same output: h = act(zg) * zu   -> bf16
+//   gradients    z is computed again from the same codes and scales: dz = dy * act'(z), or dg = dh * zu * act'(zg) and
+//                du = dh * act(zg), stored in fp32, together with each row's largest |dz * sb| (the scale of the
+//                fixed-point form in which the gradient product takes it)
 //
 // Without bias, activation and residual, linear gives the bits of the plain epilogue.
 #ifndef W8A8_GEMM_I8_EPILOGUES_CUH
@@ -140,6 +143,90 @@ __device__ __forceinline__ void drain_gated(const Params& p, uint32_t t_lane, co
         });
         store_row32(static_cast<__nv_bfloat16*>(p.C) + (int64_t)row * p.ldc + n, out, p.N - n, vec_ok);
     }
+}
+
+__device__ __forceinline__ void store_f32x2(float* p, float a, float b, int n_left, bool vec) {
+    if (vec) {   // n_left is even then
+        if (n_left >= 2) *reinterpret_cast<float2*>(p) = make_float2(a, b);
+    } else {
+        if (n_left >= 1) p[0] = a;
+        if (n_left >= 2) p[1] = b;
+    }
+}
+// larger magnitude, as bits: unlike fmaxf it keeps a NaN, which then reaches the whole row of the result
+__device__ __forceinline__ unsigned top_bits(unsigned top, float v) { return max(top, __float_as_uint(v) & 0x7fffffffu); }
+
+template <int NCOLS>
+__device__ __forceinline__ void drain_linear_grad(const Params& p, uint32_t t_lane, const float* sbs, const float* bias_s,
+                                                  int row, bool row_ok, int n0) {
+    const float sa = row_ok ? __ldg(p.sa + row) : 0.0f;
+    const bool dy_vec = row_vector_ok(p.resid, p.ldr), z_vec = p.ldc % 4 == 0;
+    unsigned top = 0;
+#pragma unroll 1
+    for (int cc = 0; cc < NCOLS / 32; ++cc) {
+        uint32_t r[32];
+        const int n = n0 + cc * 32, left = p.N - n;
+        Row32 dy = {};
+        if (row_ok && left > 0) load_row32(dy, p.resid + (int64_t)row * p.ldr + n, left, dy_vec);
+        __syncwarp();
+        ptx::tmem_ld_32x32b_x32(t_lane + cc * 32, r);
+        ptx::tmem_ld_wait();
+        if (!row_ok || left <= 0) continue;
+        float* out = static_cast<float*>(p.C) + (int64_t)row * p.ldc + n;
+        with_act(p.act, [&](auto a) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+                float dz[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int e = j + k, c = cc * 32 + e;
+                    dz[k] = row32_at(dy, e) * act_value_slope<decltype(a)::value>(scaled(r[e], sa, sbs[c], bias_s[c])).y;
+                    if (e < left) top = top_bits(top, dz[k] * sbs[c]);
+                }
+                store_f32x2(out + j, dz[0], dz[1], left - j, z_vec);
+            }
+        });
+    }
+    if (row_ok && top != 0) atomicMax(p.row_top + row, top);
+}
+
+__device__ __forceinline__ void drain_gated_grad(const Params& p, uint32_t t_lane, const float* sbs, const float* bias_s,
+                                                 int row, bool row_ok, int n0) {
+    const float sa = row_ok ? __ldg(p.sa + row) : 0.0f;
+    const bool dh_vec = row_vector_ok(p.resid, p.ldr), z_vec = p.ldc % 4 == 0 && p.inter % 2 == 0;
+    unsigned top = 0;
+#pragma unroll 1
+    for (int cc = 0; cc < 4; ++cc) {
+        uint32_t g[32], u[32];
+        const int n = n0 + cc * 32, left = p.N - n;
+        Row32 dh = {};
+        if (row_ok && left > 0) load_row32(dh, p.resid + (int64_t)row * p.ldr + n, left, dh_vec);
+        __syncwarp();
+        ptx::tmem_ld_32x32b_x32(t_lane + cc * 32, g);
+        ptx::tmem_ld_32x32b_x32(t_lane + 128 + cc * 32, u);
+        ptx::tmem_ld_wait();
+        if (!row_ok || left <= 0) continue;
+        float* out_g = static_cast<float*>(p.C) + (int64_t)row * p.ldc + n;
+        float* out_u = out_g + p.inter;
+        with_act(p.act, [&](auto a) {
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+                float dg[2], du[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int e = j + k, c = cc * 32 + e;
+                    const float2 vs = act_value_slope<decltype(a)::value>(scaled(g[e], sa, sbs[c], bias_s[c]));
+                    const float zu = scaled(u[e], sa, sbs[128 + c], bias_s[128 + c]), d = row32_at(dh, e);
+                    dg[k] = d * zu * vs.y;
+                    du[k] = d * vs.x;
+                    if (e < left) top = top_bits(top_bits(top, dg[k] * sbs[c]), du[k] * sbs[128 + c]);
+                }
+                store_f32x2(out_g + j, dg[0], dg[1], left - j, z_vec);
+                store_f32x2(out_u + j, du[0], du[1], left - j, z_vec);
+            }
+        });
+    }
+    if (row_ok && top != 0) atomicMax(p.row_top + row, top);
 }
 
 // Split-K epilogues of the weight-streaming kernels (see reduce_partials_and_store): the item's partials come through

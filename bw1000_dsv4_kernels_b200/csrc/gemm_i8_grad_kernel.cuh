@@ -1,0 +1,203 @@
+// Private part of gemm_i8_sm100.cu: the gradient product through a frozen int8 weight,
+//
+//   dx[m, k] = sum_n t[m, n] * W[n, k],   t = dz * sb (fp32),   W int8 [N, K] as the forward has it.
+//
+// W is int8 and a gradient needs more than eight bits, so each row of t is put into 16-bit fixed point relative to its
+// largest magnitude and cut into two int8 digits: t = s * (256 hi + lo), s = top / 32639.  Both digits go through the
+// int8 tensor cores with exact int32 sums, hi in one accumulator and lo in another (256 + 256 columns are the whole
+// tensor memory), and dx = s * (256 sum_hi + sum_lo).  A digit pass costs what an int8 GEMM costs, the pair what a bf16
+// GEMM of that size costs, but W needs neither a bf16 copy nor a conversion on its way, and the step of t is 2^-16 of
+// the row's top (bf16 would round every element to 2^-8 of itself).
+//
+// The sum runs over W's rows, so W is the operand whose memory runs along its N axis: its 128 x 128-byte boxes are used
+// as they lie in memory (an MN-major operand); no transposed copy of the weight exists.
+//
+// Pairs of CTAs, tiles of 256 x 256, pipeline and barriers as in gemm_i8_pair_kernel; a tile walks the K blocks twice.
+// With both accumulators taken by one tile, the drain does not overlap the next tile's MMAs (its loads do): about 4 %
+// at N = 8192.
+#ifndef W8A8_GEMM_I8_GRAD_KERNEL_CUH
+#define W8A8_GEMM_I8_GRAD_KERNEL_CUH
+
+#include "gemm_i8_common.cuh"
+#include "gemm_i8_epilogues.cuh"
+#include "gemm_i8_pair_kernel.cuh"
+#include "gradient_digits.cuh"
+
+namespace w8a8 {
+namespace {
+
+struct GradParams {
+    const unsigned* row_top;   // [M] largest |t| of the row, as float bits
+    __nv_bfloat16* dx;         // [M, K]
+    int M, N, K;               // N: length of the sum
+    int group_m;
+    unsigned long long wait_limit_ns;
+};
+
+template <int STAGES>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+gemm_i8_grad_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmW, const GradParams p) {
+    using L = PairSmem<STAGES, false>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kTmemSlotOff);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kAbortOff);
+    const uint32_t tiles_base = ptx::smem_u32(smem);
+    const uint32_t bar_base = ptx::smem_u32(bars);
+    auto full_bar = [&](int s) { return bar_base + 8u * s; };
+    auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
+    const uint32_t acc_full_bar = bar_base + 8u * (2 * STAGES), acc_empty_bar = bar_base + 8u * (2 * STAGES + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = ptx::cluster_ctarank();
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            ptx::mbar_init(full_bar(s), 1);
+            ptx::mbar_init(empty_bar(s), 1);
+        }
+        ptx::mbar_init(acc_full_bar, 1);
+        ptx::mbar_init(acc_empty_bar, 2 * (kDrainThreads / 32));
+        *abort_flag = 0;
+        ptx::fence_barrier_init();
+        ptx::fence_proxy_async_smem();
+        ptx::prefetch_tensormap(&tmD);
+        ptx::prefetch_tensormap(&tmW);
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc_pair(ptx::smem_u32(tmem_slot), 512);
+        ptx::tmem_relinquish_pair();
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::cluster_sync();  // the peer's barriers exist before anything arrives on them
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+
+    const int tiles_m = (p.M + 255) / 256, tiles_k = (p.K + 255) / 256;
+    const int total = tiles_m * tiles_k;
+    const PairTileOrder order{tiles_m, tiles_k, p.group_m};
+    const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+    const int blocks = (p.N + BK - 1) / BK;
+
+    if (warp == 0) {
+        // ---------------- TMA producer (both CTAs) ----------------
+        if (ptx::elect_one()) {
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = pair; t < total && ok; t += npairs) {
+                int mt, kt;
+                order.at(t, mt, kt);
+                for (int digit = 0; digit < 2 && ok; ++digit) {
+                    const int row0 = digit * p.M + mt * 256 + (int)rank * 128;   // rows past the hi block belong to no output
+                    for (int nb = 0; nb < blocks; ++nb) {
+                        if (!ptx::mbar_wait_bounded(empty_bar(stage), phase ^ 1u, p.wait_limit_ns) || *abort_flag) {
+                            report_wait_failure(kWaitEmptyStage);
+                            *abort_flag = 1;
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t a_dst = tiles_base + stage * L::kStageBytes;
+                        const uint32_t leader_full = ptx::map_to_cta(full_bar(stage), 0);
+                        if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * L::kStageBytes);
+                        ptx::tma_load_2d_pair(a_dst, &tmD, nb * BK, row0, leader_full);
+                        ptx::tma_load_2d_pair(a_dst + L::kABytes, &tmW, kt * 256 + (int)rank * 128, nb * BK, leader_full);
+                        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                    }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (even CTA only) ----------------
+        if (rank == 0 && ptx::elect_one()) {
+            constexpr uint32_t idesc = ptx::idesc_i8_b_mn(256, 256);
+            int stage = 0;
+            uint32_t phase = 0, acc_phase = 0;
+            bool ok = true;
+            for (int t = pair; t < total && ok; t += npairs) {
+                if (!ptx::mbar_wait_bounded(acc_empty_bar, acc_phase ^ 1u, p.wait_limit_ns) || *abort_flag) {
+                    report_wait_failure(kWaitAccEmpty);
+                    *abort_flag = 1;
+                    break;
+                }
+                ptx::tc_fence_after_sync();
+                for (int digit = 0; digit < 2 && ok; ++digit) {
+                    for (int nb = 0; nb < blocks; ++nb) {
+                        if (!ptx::mbar_wait_bounded(full_bar(stage), phase, p.wait_limit_ns) || *abort_flag) {
+                            report_wait_failure(kWaitFullStage);
+                            *abort_flag = 1;
+                            ok = false;
+                            break;
+                        }
+                        ptx::tc_fence_after_sync();
+                        const uint32_t a_src = tiles_base + stage * L::kStageBytes;
+                        const uint64_t adesc = ptx::smem_desc_k_sw128(a_src);
+                        const uint64_t bdesc = ptx::smem_desc_mn_sw128(a_src + L::kABytes);
+#pragma unroll
+                        for (int k = 0; k < BK / UMMA_K; ++k)
+                            ptx::mma_i8_ss_pair(tmem_base + digit * 256, adesc + 2u * k, bdesc + (4096u >> 4) * k, idesc,
+                                                (nb | k) != 0 ? 1u : 0u);
+                        ptx::tc_commit_pair(empty_bar(stage), 0x3);
+                        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                    }
+                }
+                if (!ok) break;
+                ptx::tc_commit_pair(acc_full_bar, 0x3);
+                acc_phase ^= 1u;
+            }
+        }
+    } else {
+        // ---------------- drain warps (both CTAs) ----------------
+        const int quarter = warp & 3;
+        uint32_t acc_phase = 0;
+        const bool vec = p.K % 8 == 0 && (reinterpret_cast<uintptr_t>(p.dx) & 15) == 0;
+        const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+        for (int t = pair; t < total; t += npairs) {
+            int mt, kt;
+            order.at(t, mt, kt);
+            const int row = mt * 256 + (int)rank * 128 + quarter * 32 + lane;
+            const float s = row < p.M ? digit_scale(__uint_as_float(__ldg(p.row_top + row))) : 0.0f;
+            __syncwarp();
+            if (!ptx::mbar_wait_bounded(acc_full_bar, acc_phase, p.wait_limit_ns) || *abort_flag) {
+                report_wait_failure(kWaitAccFull);
+                *abort_flag = 1;
+                break;
+            }
+            ptx::tc_fence_after_sync();
+#pragma unroll 1
+            for (int cc = 0; cc < 8; ++cc) {
+                uint32_t hi[32], lo[32];
+                __syncwarp();
+                ptx::tmem_ld_32x32b_x32(t_lane + cc * 32, hi);
+                ptx::tmem_ld_32x32b_x32(t_lane + 256 + cc * 32, lo);
+                ptx::tmem_ld_wait();
+                const int k = kt * 256 + cc * 32;
+                if (row >= p.M || k >= p.K) continue;
+                Row32 out;
+#pragma unroll
+                for (int j = 0; j < 16; ++j)
+                    out.w[j] = pack_bf16x2_rn(digit_value((int)hi[2 * j], (int)lo[2 * j], s),
+                                              digit_value((int)hi[2 * j + 1], (int)lo[2 * j + 1], s));
+                store_row32(p.dx + (int64_t)row * p.K + k, out, p.K - k, vec);
+            }
+            ptx::tc_fence_before_sync();
+            if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_cta(acc_empty_bar, 0));
+            acc_phase ^= 1u;
+        }
+    }
+
+    // ---------------- teardown ----------------
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::cluster_sync();  // neither CTA leaves while the other may still touch its memory
+    if (warp == 1) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc_pair(tmem_base, 512);
+    }
+}
+
+}  // namespace
+}  // namespace w8a8
+
+#endif  // W8A8_GEMM_I8_GRAD_KERNEL_CUH

@@ -77,7 +77,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     static_assert(EPI == kEpiPlain || !TMA_STORE, "the fused epilogues store from registers");
     constexpr int PBN = 256;  // tile width of the pair
     // a gated tile is 128 gate rows (the even CTA's) and the 128 up rows of the same outputs (the odd CTA's)
-    constexpr bool kGated = EPI == kEpiGated;
+    constexpr bool kGated = is_gated(EPI);
     constexpr int kOutCols = kGated ? 128 : PBN;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -249,7 +249,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             order.at(t, mt, nt);
             const int n0 = nt * kOutCols;
             __syncwarp();
-            if constexpr (EPI == kEpiLinear) {
+            if constexpr (EPI == kEpiLinear || EPI == kEpiLinearGrad) {
                 stage_columns(p, sbs, bias_s, lane, 128, n0, n0 + 128, p.N, p.N);
             } else if constexpr (kGated) {
                 stage_columns(p, sbs, bias_s, lane, 128, n0, p.inter + n0, p.inter, 2 * p.inter);
@@ -270,6 +270,10 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * PBN;
             if constexpr (EPI == kEpiLinear) {
                 drain_linear<PBN>(p, t_lane, sbs, bias_s, row, row < p.M, n0, vec_ok);
+            } else if constexpr (EPI == kEpiLinearGrad) {
+                drain_linear_grad<PBN>(p, t_lane, sbs, bias_s, row, row < p.M, n0);
+            } else if constexpr (EPI == kEpiGatedGrad) {
+                drain_gated_grad(p, t_lane, sbs, bias_s, row, row < p.M, n0);
             } else if constexpr (kGated) {
                 drain_gated(p, t_lane, sbs, bias_s, row, row < p.M, n0, vec_ok);
             } else if constexpr (!TMA_STORE) {

@@ -36,6 +36,7 @@
 #include "gemm_i8_pair_kernel.cuh"
 #include "gemm_i8_stream_kernels.cuh"
 #include "gemm_i8_wt_kernel.cuh"
+#include "gemm_i8_grad_kernel.cuh"
 
 namespace w8a8 {
 
@@ -322,7 +323,7 @@ int launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap& tmB, const Pa
     static bool opted_in[64] = {};
     if (!opt_in_shared_memory(gemm_i8_pair_kernel<STAGES, TMA_STORE, EPI>, L::kDynamic, opted_in))
         return fail(DSV4_ERR_LAUNCH, "w8a8_gemm: cannot raise the dynamic shared memory limit");
-    const int out_cols = EPI == kEpiGated ? 128 : 256;
+    const int out_cols = is_gated(EPI) ? 128 : 256;
     const int tiles = ((p.M + 255) / 256) * ((p.N + out_cols - 1) / out_cols);
     int pairs = sm_count() / 2;
     if (pairs <= 0) return fail(DSV4_ERR_LAUNCH, "w8a8_gemm: no CUDA device");
@@ -355,12 +356,13 @@ int launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap& tmB, const Pa
 // tile takes half its rows from the gates and half from the ups, so its N counts twice.
 template <int EPI>
 int gemm_i8_dense(const GemmArgs& a, const Params& p, int bn, cudaStream_t st) {
-    constexpr bool kGated = EPI == kEpiGated;
+    constexpr bool kGated = is_gated(EPI);
+    constexpr bool kGrad = EPI == kEpiLinearGrad || EPI == kEpiGatedGrad;
     const int sms = sm_count();
     const int w_rows = kGated ? 2 * a.N : a.N;
     CUtensorMap tmA, tmB;
     // Few tokens: stream the weight once, tokens on the MMA's N axis, K split over a cluster
-    if (a.M <= 256 && a.npeers == 0) {
+    if constexpr (!kGrad) if (a.M <= 256 && a.npeers == 0) {
         const int k_blocks = (a.K + BK - 1) / BK;
         if (a.M > 128 && w_rows >= 256) {
             // 129..256 tokens: CTA pairs halve the token traffic per SM
@@ -393,8 +395,8 @@ int gemm_i8_dense(const GemmArgs& a, const Params& p, int bn, cudaStream_t st) {
             default: return launch_stream_variant<256, EPI>(tmA, tmB, p, n_tiles, splits, st);
         }
     }
-    // Dense problems with more than one 128-row tile go to the CTA-pair kernel, gated ones always
-    if (kGated || (a.M > 128 && (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256) >= sms / 4)) {
+    // Dense problems with more than one 128-row tile go to the CTA-pair kernel, gated ones and gradients always
+    if (kGated || kGrad || (a.M > 128 && (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256) >= sms / 4)) {
         int rc2 = make_tile_map(&tmA, a.A, (uint64_t)a.M, (uint64_t)a.K, BM);
         if (rc2) return rc2;
         rc2 = make_tile_map(&tmB, a.B, (uint64_t)w_rows, (uint64_t)a.K, 128);
@@ -416,7 +418,7 @@ int gemm_i8_dense(const GemmArgs& a, const Params& p, int bn, cudaStream_t st) {
         }
         return launch_pair_variant<6, false, EPI>(tmA, tmB, p, smaps, st);
     }
-    if constexpr (!kGated) {
+    if constexpr (!kGated && !kGrad) {
         int rc = make_tile_map(&tmA, a.A, (uint64_t)a.M, (uint64_t)a.K, BM);
         if (rc) return rc;
         rc = make_tile_map(&tmB, a.B, (uint64_t)w_rows, (uint64_t)a.K, (uint32_t)bn);
@@ -479,7 +481,7 @@ int gemm_i8(const GemmArgs& a, cudaStream_t st) {
     if (p.ldc < a.N) return fail(DSV4_ERR_ARG, "w8a8_gemm: ldc smaller than N");
     p.bias = static_cast<const __nv_bfloat16*>(a.bias);
     p.resid = static_cast<const __nv_bfloat16*>(a.resid);
-    p.ldr = a.ldr; p.act = a.act; p.inter = a.N;
+    p.ldr = a.ldr; p.act = a.act; p.inter = a.N; p.row_top = a.row_top;
     if (a.epilogue != kEpiPlain && (grouped || a.out_i32 || a.npeers != 0))
         return fail(DSV4_ERR_ARG, "w8a8_linear: the fused epilogues exist for the dense GEMM with bf16 output");
     {
@@ -542,8 +544,39 @@ int gemm_i8(const GemmArgs& a, cudaStream_t st) {
     switch (a.epilogue) {
         case kEpiLinear: return gemm_i8_dense<kEpiLinear>(a, p, bn, st);
         case kEpiGated: return gemm_i8_dense<kEpiGated>(a, p, bn, st);
+        case kEpiLinearGrad: return gemm_i8_dense<kEpiLinearGrad>(a, p, bn, st);
+        case kEpiGatedGrad: return gemm_i8_dense<kEpiGatedGrad>(a, p, bn, st);
         default: return gemm_i8_dense<kEpiPlain>(a, p, bn, st);
     }
+}
+
+// dx = dz_scaled W for digits that split_gradient wrote (see gemm_i8_grad_kernel.cuh)
+int gemm_i8_gradient(const void* digits, const unsigned* row_top, const void* W, void* dx, int M, int N, int K, int pitch,
+                     cudaStream_t st) {
+    using L = PairSmem<6, false>;
+    static bool opted_in[64] = {};
+    if (!opt_in_shared_memory(gemm_i8_grad_kernel<6>, L::kDynamic, opted_in))
+        return fail(DSV4_ERR_LAUNCH, "w8a8 backward: cannot raise the dynamic shared memory limit");
+    GradParams p;
+    p.row_top = row_top;
+    p.dx = static_cast<__nv_bfloat16*>(dx);
+    p.M = M; p.N = N; p.K = K;
+    p.wait_limit_ns = ptx::kWaitLimitNs;
+    // groups of m-tiles whose two digits take at most 32 MB, as in gemm_i8
+    const int tiles_m = (M + 255) / 256;
+    int gm_max = (int)((int64_t)32 * 1024 * 1024 / ((int64_t)512 * pitch));
+    if (gm_max < 1) gm_max = 1;
+    const int groups = (tiles_m + gm_max - 1) / gm_max;
+    p.group_m = (tiles_m + groups - 1) / groups;
+    CUtensorMap tmD, tmW;
+    if (int rc = make_tile_map(&tmD, digits, (uint64_t)2 * M, (uint64_t)pitch, BM)) return rc;
+    if (int rc = make_tile_map(&tmW, W, (uint64_t)N, (uint64_t)K, 128)) return rc;
+    const int64_t tiles = (int64_t)tiles_m * ((K + 255) / 256);
+    int pairs = sm_count() / 2;
+    if (pairs <= 0) return fail(DSV4_ERR_LAUNCH, "w8a8 backward: no CUDA device");
+    if (tiles < pairs) pairs = (int)tiles;
+    gemm_i8_grad_kernel<6><<<2 * pairs, kThreads, L::kDynamic, st>>>(tmD, tmW, p);
+    return check_launch("w8a8 backward");
 }
 
 // ------------------------------------------------------------------------------------

@@ -48,12 +48,15 @@ struct GemmArgs {
     const void* resid = nullptr;   // bf16 [M, N] with row stride ldr
     int64_t ldr = 0;
     int act = 0;                   // enum Activation in activations.cuh
+    unsigned* row_top = nullptr;   // gradient epilogues (3 linear, 4 gated; resid is the incoming gradient, C is fp32)
     // Test hook, zero through every public entry point: the tile producers of the launch issue no
     // loads and every bounded wait gives up after test_wait_limit_ns, so the kernel's give-up path runs.
     int test_withhold_loads = 0;
     unsigned long long test_wait_limit_ns = 0;
 };
 int gemm_i8(const GemmArgs& a, cudaStream_t st);
+int gemm_i8_gradient(const void* digits, const unsigned* row_top, const void* W, void* dx, int M, int N, int K, int pitch,
+                     cudaStream_t st);
 int scale_convert(const void* acc, const void* sa, const void* sb, void* out, int M, int N,
                   cudaStream_t st);
 
@@ -81,6 +84,24 @@ int layernorm(void* res, const void* x, const void* w, const void* b, void* y, v
 int64_t layernorm_backward_workspace(int M, int K);
 int layernorm_backward(const void* dy, const void* x, const void* mean, const void* rstd, const void* w, const void* dres,
                        void* dx, void* dw, void* db, void* workspace, int M, int K, cudaStream_t st);
+
+// ---- launchers implemented in w8a8_backward.cu ----------------------------------------
+struct BackwardArgs {
+    const void* dy;        // bf16 [M, N], or [M, N / 2] when gated; row stride ldy
+    int64_t ldy;
+    const void* A;         // int8 [M, K]: the forward's codes
+    const void* B;         // int8 [N, K]
+    const float* sa;
+    const float* sb;
+    const void* bias;      // bf16 [N] or null
+    int act;
+    bool gated;
+    void* dx;              // bf16 [M, K]
+    float* dbias;          // fp32 [N] or null
+    int M, N, K;
+};
+int64_t w8a8_backward_workspace(int M, int N, bool recompute, bool dbias);
+int w8a8_backward(const BackwardArgs& a, void* workspace, cudaStream_t st);
 
 int read_device_status(cudaStream_t st, int* out);
 int read_row_status(int* out);  // status word of the row kernels (after the stream was synchronised)

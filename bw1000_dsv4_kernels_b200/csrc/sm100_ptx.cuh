@@ -326,6 +326,14 @@ __device__ __forceinline__ uint64_t smem_desc_k_sw128(uint32_t smem_addr) {
     return d;
 }
 
+// The same for a tile whose 128-byte rows run along the operand's M or N axis ("MN-major", 128 8-bit elements) and
+// follow one another along K: eight rows of K are one 1024-byte swizzle atom, the stride byte offset steps over them,
+// and one atom covers the 128 elements, so the other offset is not used (it is given the same value).  Stepping K by
+// 32 rows adds 4096 bytes.
+__device__ __forceinline__ uint64_t smem_desc_mn_sw128(uint32_t smem_addr) {
+    return smem_desc_k_sw128(smem_addr) | (static_cast<uint64_t>(1024 >> 4) << 16);
+}
+
 // Instruction descriptor for kind::i8: D int32 (c_format 2 at bit 4), A and B signed
 // 8-bit (format 1 at bits 7 and 10), both K-major (bits 15, 16 clear), N/8 at bit 17,
 // M/16 at bit 24.
@@ -333,6 +341,8 @@ __host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
     return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) |
            (static_cast<uint32_t>(m >> 4) << 24);
 }
+// B is MN-major (bit 16 set)
+__host__ __device__ constexpr uint32_t idesc_i8_b_mn(int m, int n) { return idesc_i8(m, n) | (1u << 16); }
 
 }  // namespace ptx
 }  // namespace w8a8

@@ -599,6 +599,13 @@ int64_t device_status() {
     return v;
 }
 
+// A workspace that lives only for the launches of one call: allocated on the stream that the launches go to, so that
+// the caching allocator hands it out again only behind them on that stream, whatever torch's current stream is.
+Tensor workspace_on(dsv4_stream_t stream, int64_t bytes, const Tensor& like) {
+    c10::cuda::CUDAStreamGuard on(c10::cuda::getStreamFromExternal(reinterpret_cast<cudaStream_t>(stream), like.device().index()));
+    return torch::empty({bytes}, like.options().dtype(torch::kUInt8));
+}
+
 // ---- fused linear and gated projection ------------------------------------------------
 int activation_of(const std::string& name) {
     static const char* const names[] = {"none", "relu", "gelu", "gelu_tanh", "silu"};
@@ -661,14 +668,39 @@ Tensor w8a8_gated_stream(Tensor A, Tensor W13, Tensor sa, Tensor s13, c10::optio
     return C;
 }
 
-// ---- layer norm ---------------------------------------------------------------------
-// A workspace that lives only for the launches of one call: allocated on the stream that the launches go to, so that
-// the caching allocator hands it out again only behind them on that stream, whatever torch's current stream is.
-Tensor workspace_on(dsv4_stream_t stream, int64_t bytes, const Tensor& like) {
-    c10::cuda::CUDAStreamGuard on(c10::cuda::getStreamFromExternal(reinterpret_cast<cudaStream_t>(stream), like.device().index()));
-    return torch::empty({bytes}, like.options().dtype(torch::kUInt8));
+// -> dx bf16 [M, K], dbias fp32 (None without a bias)
+std::vector<c10::optional<Tensor>> w8a8_backward_impl(bool gated, Tensor dy, Tensor A, Tensor B, Tensor sa, Tensor sb,
+                                                      c10::optional<Tensor> bias, const std::string& act, int64_t stream_ptr) {
+    const GemmShape g = check_gemm_operands(A, B);
+    TORCH_CHECK(!gated || g.N % 2 == 0, "W13 must hold as many up rows as gate rows, got ", g.N, " rows");
+    const Tensor& sa_c = flat_scale(sa, g.M, "sa", A);
+    const Tensor& sb_c = flat_scale(sb, g.N, gated ? "s13" : "sb", A);
+    const void* bp = bias_ptr(bias, g.N, A);
+    const int act_id = gated ? gated_act(act) : activation_of(act);
+    const int64_t ldy = row_stride(dy, gated ? "dh" : "dy", g.M, gated ? g.N / 2 : g.N, A);
+    c10::cuda::CUDAGuard guard(A.device());
+    auto dx = torch::empty({g.M, g.K}, A.options().dtype(torch::kBFloat16));
+    c10::optional<Tensor> db;
+    if (bias.has_value()) db = torch::empty({g.N}, A.options().dtype(torch::kFloat32));
+    const dsv4_stream_t st = as_stream(stream_ptr);
+    const int64_t bytes = dsv4_w8a8_backward_workspace(g.M, g.N, act_id, bias.has_value());
+    Tensor ws = workspace_on(st, bytes, A);
+    auto launch = gated ? launch_w8a8_gated_backward : launch_w8a8_linear_backward;
+    check_status(launch(dy.data_ptr(), ldy, A.data_ptr(), B.data_ptr(), sa_c.data_ptr(), sb_c.data_ptr(), bp, act_id,
+                        dx.data_ptr(), db.has_value() ? db->data_ptr() : nullptr, ws.data_ptr(), bytes, g.M,
+                        gated ? g.N / 2 : g.N, g.K, st));
+    return {dx, db};
+}
+std::vector<c10::optional<Tensor>> w8a8_linear_backward_stream(Tensor dy, Tensor A, Tensor B, Tensor sa, Tensor sb,
+                                                               c10::optional<Tensor> bias, const std::string& act, int64_t stream_ptr) {
+    return w8a8_backward_impl(false, dy, A, B, sa, sb, bias, act, stream_ptr);
+}
+std::vector<c10::optional<Tensor>> w8a8_gated_backward_stream(Tensor dh, Tensor A, Tensor W13, Tensor sa, Tensor s13,
+                                                              c10::optional<Tensor> bias, const std::string& act, int64_t stream_ptr) {
+    return w8a8_backward_impl(true, dh, A, W13, sa, s13, bias, act, stream_ptr);
 }
 
+// ---- layer norm ---------------------------------------------------------------------
 struct NormShape {
     int M, N;
 };
@@ -861,6 +893,18 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         return w8a8_gated_stream(A, W13, sa, s13, bias, act, current_stream_ptr());
     }, py::arg("A"), py::arg("W13"), py::arg("sa"), py::arg("s13"), py::arg("bias") = py::none(), py::arg("act") = "silu");
     m.def("w8a8_gated_stream", &w8a8_gated_stream);
+    m.def("w8a8_linear_backward", [](Tensor dy, Tensor A, Tensor B, Tensor sa, Tensor sb, c10::optional<Tensor> bias,
+                                     const std::string& act) {
+        return w8a8_linear_backward_stream(dy, A, B, sa, sb, bias, act, current_stream_ptr());
+    }, py::arg("dy"), py::arg("A"), py::arg("B"), py::arg("sa"), py::arg("sb"), py::arg("bias") = py::none(),
+       py::arg("act") = "none");
+    m.def("w8a8_linear_backward_stream", &w8a8_linear_backward_stream);
+    m.def("w8a8_gated_backward", [](Tensor dh, Tensor A, Tensor W13, Tensor sa, Tensor s13, c10::optional<Tensor> bias,
+                                    const std::string& act) {
+        return w8a8_gated_backward_stream(dh, A, W13, sa, s13, bias, act, current_stream_ptr());
+    }, py::arg("dh"), py::arg("A"), py::arg("W13"), py::arg("sa"), py::arg("s13"), py::arg("bias") = py::none(),
+       py::arg("act") = "silu");
+    m.def("w8a8_gated_backward_stream", &w8a8_gated_backward_stream);
     m.def("layernorm", [](Tensor x, Tensor w, Tensor b, double eps) {
         return layernorm_stream(x, w, b, eps, current_stream_ptr());
     });

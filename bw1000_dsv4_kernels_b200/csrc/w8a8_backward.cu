@@ -1,0 +1,200 @@
+// Backward pass of the fused W8A8 linear and of the gated projection, through the frozen int8 weight:
+//
+//   dz    = dy * act'(z)   (gated: dg = dh * zu * act'(zg), du = dh * act(zg)), z computed again from the forward's codes
+//   dx    = (dz * sb) W                      the gradient of the dequantised activations
+//   dbias = sum over rows of dz              fp32
+//
+// Three steps: the forward's GEMM with a gradient epilogue writes dz in fp32 and each row's largest |dz * sb|
+// (gemm_i8_epilogues.cuh); split_gradient_kernel puts dz * sb into two int8 digits per element and sums the columns;
+// gemm_i8_grad_kernel multiplies the digits with W.  The codes and scales of the forward are all that has to be kept for
+// it.  Without an activation dz is dy itself: the first step is a pass over dy for the rows' largest magnitudes.
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <cstdint>
+
+#include "activations.cuh"
+#include "gradient_digits.cuh"
+#include "launch_common.h"
+#include "w8a8_arith.cuh"
+
+namespace w8a8 {
+namespace {
+
+__device__ __forceinline__ unsigned top_bits(unsigned top, float v) { return max(top, __float_as_uint(v) & 0x7fffffffu); }
+
+// eight consecutive gradients of one row as fp32; those at or beyond `left` are zero
+__device__ __forceinline__ void load8(const float* p, int left, bool vec, float (&v)[8]) {
+    if (vec && left >= 8) {
+        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : 0.0f;
+    }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, int left, bool vec, float (&v)[8]) {
+    if (vec && left >= 8) {
+        const uint4 q = *reinterpret_cast<const uint4*>(p);
+        v[0] = bf16lo_to_f32(q.x); v[1] = bf16hi_to_f32(q.x); v[2] = bf16lo_to_f32(q.y); v[3] = bf16hi_to_f32(q.y);
+        v[4] = bf16lo_to_f32(q.z); v[5] = bf16hi_to_f32(q.z); v[6] = bf16lo_to_f32(q.w); v[7] = bf16hi_to_f32(q.w);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < left ? __bfloat162float(p[j]) : 0.0f;
+    }
+}
+
+// row_top[row] = largest |dy * sb| of the row, as float bits: one CTA per row
+__global__ void __launch_bounds__(256) row_top_kernel(const __nv_bfloat16* dy, int64_t ldy, const float* __restrict__ sb, int N,
+                                                      bool vec, unsigned* row_top) {
+    __shared__ unsigned part[8];
+    const __nv_bfloat16* row = dy + (int64_t)blockIdx.x * ldy;
+    unsigned top = 0;
+    for (int c = threadIdx.x * 8; c < N; c += 256 * 8) {
+        float v[8];
+        load8(row + c, N - c, vec, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (c + j < N) top = top_bits(top, v[j] * __ldg(sb + c + j));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int w = 1; w < 8; ++w) top = max(top, part[w]);
+        row_top[blockIdx.x] = top;
+    }
+}
+
+// dz [M, N] -> digits int8 [2][M][pitch] (hi, then lo; zero beyond N), and per block of rows the column sums of dz.
+// A thread owns eight columns and walks the block's rows.
+constexpr int kSplitThreads = 128;
+constexpr int kSplitCols = kSplitThreads * 8;
+template <typename T, bool SUM>
+__global__ void __launch_bounds__(kSplitThreads) split_gradient_kernel(const T* dz, int64_t ld, const float* __restrict__ sb,
+                                                                       const unsigned* __restrict__ row_top, int M, int N,
+                                                                       int pitch, int rows_per_block, bool vec, int8_t* digits,
+                                                                       float* partial) {
+    const int c = blockIdx.x * kSplitCols + threadIdx.x * 8;
+    if (c >= pitch) return;
+    const int left = N - c;
+    float scale[8], sum[8] = {};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) scale[j] = j < left ? __ldg(sb + c + j) : 0.0f;
+    const int r0 = blockIdx.y * rows_per_block, r1 = min(M, r0 + rows_per_block);
+    const int64_t plane = (int64_t)M * pitch;
+#pragma unroll 4
+    for (int r = r0; r < r1; ++r) {
+        float v[8];
+        load8(dz + (int64_t)r * ld + c, left, vec, v);
+        const float inv = digit_inverse(__uint_as_float(__ldg(row_top + r)));
+        uint32_t hi[2], lo[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            int d[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (SUM) sum[4 * h + j] += v[4 * h + j];
+                d[j] = digits_of(v[4 * h + j] * scale[4 * h + j], inv);
+            }
+            hi[h] = pack_i8x4(digit_hi(d[0]), digit_hi(d[1]), digit_hi(d[2]), digit_hi(d[3]));
+            lo[h] = pack_i8x4(digit_lo(d[0]), digit_lo(d[1]), digit_lo(d[2]), digit_lo(d[3]));
+        }
+        int8_t* out = digits + (int64_t)r * pitch + c;
+        *reinterpret_cast<uint2*>(out) = make_uint2(hi[0], hi[1]);
+        *reinterpret_cast<uint2*>(out + plane) = make_uint2(lo[0], lo[1]);
+    }
+    if constexpr (SUM) {
+        float* o = partial + (int64_t)blockIdx.y * N + c;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j < left) o[j] = sum[j];
+    }
+}
+
+// column sums over the row blocks, eight slices of them, each in order: 32 columns per CTA
+__global__ void __launch_bounds__(256) gradient_column_sum_kernel(const float* __restrict__ partial, int parts, int N,
+                                                                  float* __restrict__ out) {
+    __shared__ float sh[8][33];
+    const int col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
+    float v = 0.0f;
+    if (col < N)
+        for (int i = slice; i < parts; i += 8) v += partial[(int64_t)i * N + col];
+    sh[slice][threadIdx.x & 31] = v;
+    __syncthreads();
+    if (slice == 0 && col < N) {
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) s += sh[k][threadIdx.x & 31];
+        out[col] = s;
+    }
+}
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+struct Layout {
+    int pitch, rows_per_block, row_blocks;
+    int64_t digits, dz, row_top, partial, total;   // offsets and size in bytes
+};
+Layout layout(int M, int N, bool recompute, bool dbias) {
+    auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
+    Layout l;
+    l.pitch = (int)(((int64_t)N + 15) / 16 * 16);
+    l.rows_per_block = M >= 2048 ? 32 : 16;
+    l.row_blocks = (M + l.rows_per_block - 1) / l.rows_per_block;
+    l.digits = 0;
+    l.dz = l.digits + up((int64_t)2 * M * l.pitch);
+    l.row_top = l.dz + (recompute ? up((int64_t)4 * M * N) : 0);
+    l.partial = l.row_top + up((int64_t)4 * M);
+    l.total = l.partial + (dbias ? up((int64_t)4 * l.row_blocks * N) : 0);
+    return l;
+}
+
+template <typename T>
+int split(const T* dz, int64_t ld, const BackwardArgs& a, const Layout& l, const unsigned* row_top, int8_t* digits,
+          float* partial, cudaStream_t st) {
+    const bool vec = (ld * sizeof(T)) % 16 == 0 && aligned16(dz);
+    const dim3 grid((l.pitch + kSplitCols - 1) / kSplitCols, l.row_blocks);
+    if (a.dbias != nullptr) {
+        split_gradient_kernel<T, true><<<grid, kSplitThreads, 0, st>>>(dz, ld, a.sb, row_top, a.M, a.N, l.pitch,
+                                                                       l.rows_per_block, vec, digits, partial);
+        if (int rc = check_launch("w8a8 backward")) return rc;
+        gradient_column_sum_kernel<<<(a.N + 31) / 32, 256, 0, st>>>(partial, l.row_blocks, a.N, a.dbias);
+    } else {
+        split_gradient_kernel<T, false><<<grid, kSplitThreads, 0, st>>>(dz, ld, a.sb, row_top, a.M, a.N, l.pitch,
+                                                                        l.rows_per_block, vec, digits, partial);
+    }
+    return check_launch("w8a8 backward");
+}
+
+}  // namespace
+
+int64_t w8a8_backward_workspace(int M, int N, bool recompute, bool dbias) { return layout(M, N, recompute, dbias).total; }
+
+int w8a8_backward(const BackwardArgs& a, void* workspace, cudaStream_t st) {
+    const bool recompute = a.act != kActNone;
+    const Layout l = layout(a.M, a.N, recompute, a.dbias != nullptr);
+    char* ws = static_cast<char*>(workspace);
+    int8_t* digits = reinterpret_cast<int8_t*>(ws + l.digits);
+    unsigned* row_top = reinterpret_cast<unsigned*>(ws + l.row_top);
+    float* partial = reinterpret_cast<float*>(ws + l.partial);
+    const __nv_bfloat16* dy = static_cast<const __nv_bfloat16*>(a.dy);
+    if (recompute) {
+        float* dz = reinterpret_cast<float*>(ws + l.dz);
+        if (cudaMemsetAsync(row_top, 0, (size_t)a.M * 4, st) != cudaSuccess) return check_launch("w8a8 backward");
+        GemmArgs g{};
+        g.A = a.A; g.B = a.B; g.sa = a.sa; g.sb = a.sb; g.C = dz;
+        g.M = a.M; g.N = a.gated ? a.N / 2 : a.N; g.K = a.K; g.E = 1; g.ldc = a.N; g.sa_groups = 1;
+        g.epilogue = a.gated ? 4 : 3; g.bias = a.bias; g.resid = a.dy; g.ldr = a.ldy; g.act = a.act; g.row_top = row_top;
+        if (int rc = gemm_i8(g, st)) return rc;
+        if (int rc = split(dz, (int64_t)a.N, a, l, row_top, digits, partial, st)) return rc;
+    } else {
+        row_top_kernel<<<a.M, 256, 0, st>>>(dy, a.ldy, a.sb, a.N, a.ldy % 8 == 0 && aligned16(dy), row_top);
+        if (int rc = check_launch("w8a8 backward")) return rc;
+        if (int rc = split(dy, a.ldy, a, l, row_top, digits, partial, st)) return rc;
+    }
+    return gemm_i8_gradient(digits, row_top, a.B, a.dx, a.M, a.N, a.K, l.pitch, st);
+}
+
+}  // namespace w8a8

@@ -269,6 +269,23 @@ DSV4_API int launch_w8a8_linear(const void* A, const void* B, const void* sa, co
 DSV4_API int launch_w8a8_gated(const void* A, const void* B, const void* sa, const void* sb, const void* bias, int act,
                        void* C, int64_t ldc, int M, int I, int K, dsv4_stream_t stream);
 
+/* Gradients of the two through the frozen int8 weight.  A, sa: the codes and scales that the forward pass took (all that
+ * it has to keep); z is computed again from them.  dy bf16 [M, N] (gated: [M, I]) with row stride ldy.
+ * dx bf16 [M,K]: the gradient of the dequantised activations A * sa (the quantiser is passed straight through);
+ * dbias fp32 [N] (gated: [2*I]) or null: sums of dz over the rows.  The residual's gradient is dy itself.
+ * Inside, each row of dz * sb is in 16-bit fixed point relative to its largest magnitude (a row that holds an infinity or
+ * a NaN therefore gives a row of NaN); dz, the sums and the scales are fp32.  With DSV4_ACT_NONE A and sa are not read
+ * and may be null.  At most 131071 weight rows.  Every result depends on the inputs, sizes and device only.
+ * workspace: dsv4_w8a8_backward_workspace(M, weight rows, act, dbias != null) bytes of device memory, 16-byte aligned,
+ * free again once the launches have run. */
+DSV4_API int64_t dsv4_w8a8_backward_workspace(int M, int weight_rows, int act, int want_dbias);
+DSV4_API int launch_w8a8_linear_backward(const void* dy, int64_t ldy, const void* A, const void* B, const void* sa,
+                       const void* sb, const void* bias, int act, void* dx, void* dbias, void* workspace,
+                       int64_t workspace_bytes, int M, int N, int K, dsv4_stream_t stream);
+DSV4_API int launch_w8a8_gated_backward(const void* dh, int64_t ldh, const void* A, const void* B, const void* sa,
+                       const void* sb, const void* bias, int act, void* dx, void* dbias, void* workspace,
+                       int64_t workspace_bytes, int M, int I, int K, dsv4_stream_t stream);
+
 /* ---- layer norm (no counterpart in the reference; beside launch_rmsnorm and launch_add_rmsnorm_quant) ----------
  * a = x, or a = bf16(res + x) with res (bf16 [M,N]) overwritten by it when res is not null;
  * mean, rstd fp32 [M] of a's rows (rstd = 1/sqrt(var + eps), population variance); y = (a - mean)*rstd*w + b.

@@ -1,0 +1,200 @@
+"""Gradients of the fused W8A8 linear and of the gated projection against 64 bits on the CPU.
+
+Tolerances.  dz: the recomputed z is off by 4 * 2^-24 of its size, slopes of at most 1.13 (their own slope at most 1.2)
+and the fast exponential's 2^-18 make that 2^-17 of the terms' magnitude at most.  dx: every row of t = dz * sb is in
+fixed point with a step of top / 32639, off by half of it, so a sum of N terms is off by at most
+(step / 2) * sum |W[n, k]|, plus dz's own error times |W|, plus the two conversions, plus half a bf16 step of the
+result.  dbias: dz's error, and the fp32 additions of a column (rows of a block, then the blocks' slices)."""
+import pytest
+import torch
+
+from tests import ffn_reference as ref
+from tests import workloads as wl
+
+pytestmark = pytest.mark.gpu
+U = ref.U32
+DZ = 2.0 ** -17
+
+
+def cuda(*ts):
+    return [None if t is None else t.cuda() for t in ts]
+
+
+def check_dx(dx, dx64, t, t_err, w):
+    step = t.abs().amax(1, keepdim=True).clamp_min(1e-30) / 32639
+    wsum = w.double().abs().sum(0, keepdim=True)
+    slack = step / 2 * 1.01 * wsum + t_err @ w.double().abs() + 4 * U * (t.abs() @ w.double().abs())
+    err = (dx.cpu().double() - dx64).abs()
+    assert (err <= ref.UBF * (dx64.abs() + slack) + slack).all(), float((err - ref.UBF * dx64.abs() - slack).max())
+    # the fixed point is worth more than bf16: the rounding of the result dominates
+    if dx64.abs().max() > 0:
+        assert err.norm() <= 4e-3 * dx64.norm()
+
+
+def check_db(db, db64, dz, dz_err):
+    m = dz.shape[0]
+    slack = dz_err.sum(0) + U * (40 + m // 16) * dz.abs().sum(0) + 1e-30
+    assert db.dtype == torch.float32 and ((db.cpu().double() - db64).abs() <= slack).all()
+
+
+SHAPES = [(1, 8, 16), (3, 40, 48), (17, 127, 128), (64, 128, 144), (100, 257, 272), (129, 320, 1040), (256, 256, 256),
+          (257, 1000, 400), (300, 129, 2064), (513, 600, 528), (700, 2305, 784)]
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("act,bias", [("none", False), ("none", True), ("gelu", True), ("silu", False), ("gelu_tanh", True),
+                                      ("relu", True)])
+def test_linear_backward(ext, m, n, k, act, bias):
+    (a, sa), (w, sw) = ref.tokens(m, k, m), ref.weight(n, k, n)
+    b = ref.bf16((n,), 3) if bias else None
+    dy = ref.bf16((m, n + 3), 4)[:, 1:n + 1]
+    dx64, db64, t, dz = ref.linear_backward(dy, a, sa, w, sw, b, act)
+    dyd = torch.zeros((m, n + 3), dtype=torch.bfloat16, device="cuda")[:, 1:n + 1]   # strided rows at odd addresses
+    dyd.copy_(dy)
+    ad, wd, sad, swd, bd = cuda(a, w, sa, sw, b)
+    dx, db = ext.w8a8_linear_backward(dyd, ad, wd, sad, swd, bd, act)
+    assert dx.dtype == torch.bfloat16 and dx.shape == (m, k)
+    z, size = ref.project(a, sa, w, sw, b)
+    dz_err = (dy.double().abs() * (DZ + 1.2 * 4 * U * size)) if act != "none" else torch.zeros_like(dz)
+    if act == "relu":   # where z is within its rounding of zero the kernel may take either side
+        dz_err = torch.where(z.abs() <= 4 * U * size, dy.double().abs(), 0 * dz)
+    check_dx(dx, dx64, t, dz_err * sw.double(), w)
+    assert (db is None) == (not bias)
+    if bias:
+        check_db(db, db64, dz, dz_err)
+    dx2, db2 = ext.w8a8_linear_backward(dyd.contiguous(), ad, wd, sad, swd, bd, act)   # aligned rows: the same bits
+    assert torch.equal(dx.view(torch.int16), dx2.view(torch.int16)) and (not bias or torch.equal(db, db2))
+
+
+@pytest.mark.parametrize("m,i,k", SHAPES)
+@pytest.mark.parametrize("act,bias", [("silu", False), ("silu", True), ("gelu", False), ("gelu_tanh", True), ("relu", False)])
+def test_gated_backward(ext, m, i, k, act, bias):
+    i = max(1, i // 2)
+    (a, sa), (w, sw) = ref.tokens(m, k, m), ref.weight(2 * i, k, i)
+    b = ref.bf16((2 * i,), 3) if bias else None
+    dh = ref.bf16((m, i), 4)
+    dx64, db64, t, dz = ref.gated_backward(dh, a, sa, w, sw, b, act)
+    dx, db = ext.w8a8_gated_backward(dh.cuda(), *cuda(a, w, sa, sw, b), act)
+    z, size = ref.project(a, sa, w, sw, b)
+    g, u, size_g, size_u = z[:, :i], z[:, i:], size[:, :i], size[:, i:]
+    d = dh.double().abs()
+    err_g = d * u.abs() * (DZ + 1.2 * 4 * U * size_g) + d * 1.13 * 4 * U * size_u
+    err_u = d * (DZ * (ref.act(g, act).abs() + 1e-6) + 1.13 * 4 * U * size_g)
+    if act == "relu":
+        near = g.abs() <= 4 * U * size_g
+        err_g = torch.where(near, d * u.abs() * 1.01, d * 1.13 * 4 * U * size_u + U * d * u.abs())
+    err = torch.cat([err_g, err_u], 1) + 4 * U * dz.abs()
+    check_dx(dx, dx64, t, err * sw.double(), w)
+    assert (db is None) == (not bias)
+    if bias:
+        check_db(db, db64, dz, err)
+
+
+def test_the_gradient_product_takes_every_weight_row_and_column(ext):
+    """unit scales and gradients of small integers, then one row of the weight per row of the result"""
+    m, n, k = 300, 640, 432
+    g = torch.Generator().manual_seed(1)
+    dy = torch.randint(-8, 9, (m, n), generator=g).float()
+    dy[:, 0] = 8.0
+    dy = dy.to(torch.bfloat16)
+    w = torch.randint(-127, 128, (n, k), generator=g, dtype=torch.int8)
+    (a, sa) = ref.tokens(m, k, 2)
+    dx, _ = ext.w8a8_linear_backward(dy.cuda(), a.cuda(), w.cuda(), sa.cuda(), torch.ones(n).cuda())
+    want = dy.double() @ w.double()
+    step = 8.0 / 32639
+    bound = step / 2 * w.double().abs().sum(0)
+    assert ((dx.cpu().double() - want).abs() <= ref.UBF * (want.abs() + bound) + bound).all()
+    # one row of the weight at a time comes back as itself
+    one = torch.zeros((m, n), dtype=torch.bfloat16)
+    one[torch.arange(m), torch.arange(m) % n] = 1.0
+    dx, _ = ext.w8a8_linear_backward(one.cuda(), a.cuda(), w.cuda(), sa.cuda(), torch.ones(n).cuda())
+    assert ((dx.cpu().double() - w[torch.arange(m) % n].double()).abs() <= 127 * 2.0 ** -15).all()
+
+
+def test_rows_are_scaled_by_themselves(ext):
+    """rows of very different size, rows of zeros, and rows with a NaN or an infinity do not touch one another"""
+    m, n, k = 12, 96, 64
+    (a, sa), (w, sw) = ref.tokens(m, k, 1), ref.weight(n, k, 2)
+    dy = ref.bf16((m, n), 3).float() * (10.0 ** torch.arange(-24, 24, 4).float()).unsqueeze(1)
+    dy[5] = 0.0
+    dy[7, 11] = float("nan")
+    dy[8, 12] = float("inf")
+    dy = dy.to(torch.bfloat16)
+    for act in ("none", "silu"):
+        dx, db = ext.w8a8_linear_backward(dy.cuda(), *cuda(a, w, sa, sw, torch.zeros(n, dtype=torch.bfloat16)), act)
+        dx = dx.cpu().double()
+        assert (dx[5] == 0).all() and dx[7].isnan().all() and not dx[8].isfinite().any()
+        fine = [r for r in range(m) if r not in (5, 7, 8)]
+        want = ref.linear_backward(dy[fine], a[fine], sa[fine], w, sw, None, act)[0]
+        assert ((dx[fine] - want).norm(dim=1) <= 4e-3 * want.norm(dim=1)).all()
+        assert db.cpu()[11].isnan() and not db.cpu()[12].isfinite()
+
+
+def test_directional_difference_of_the_forward(ext):
+    """dx and dbias of the kernels against central differences of the 64-bit forward, in the dequantised activations"""
+    m, i, k, h = 9, 40, 96, 1e-5
+    (a, sa), (w, sw) = ref.tokens(m, k, 1), ref.weight(2 * i, k, 2)
+    b, dh = ref.bf16((2 * i,), 3), ref.bf16((m, i), 4)
+    x, wd = a.double() * sa.double(), w.double() * sw.double()[:, None]
+    v, vb = torch.randn(m, k, dtype=torch.float64), torch.randn(2 * i, dtype=torch.float64)
+    for act in ref.GATED_ACTS[:3]:
+        def f(t):
+            z = (x + t * v) @ wd.T + b.double() + t * vb
+            return (ref.act(z[:, :i], act) * z[:, i:] * dh.double()).sum()
+        dx, db = ext.w8a8_gated_backward(dh.cuda(), *cuda(a, w, sa, sw, b), act)
+        got = (dx.cpu().double() * v).sum() + (db.cpu().double() * vb).sum()
+        assert (got - (f(h) - f(-h)) / (2 * h)).abs() <= 2 * ref.UBF * (dx.cpu().double() * v).abs().sum() + 1e-4
+
+
+def test_empty_batches_and_refusals(ext):
+    (a, sa), (w, sw) = ref.tokens(4, 64, 1), ref.weight(32, 64, 2)
+    a, sa, w, sw = cuda(a, sa, w, sw)
+    b = torch.zeros(32, dtype=torch.bfloat16, device="cuda")
+    dy = torch.zeros((4, 32), dtype=torch.bfloat16, device="cuda")
+    dx, db = ext.w8a8_linear_backward(dy[:0], a[:0], w, sa[:0], sw, b, "gelu")
+    assert dx.shape == (0, 64) and (db == 0).all() and db.shape == (32,)
+    dx, db = ext.w8a8_linear_backward(dy, a, w, sa, sw, b, "none")
+    assert (dx == 0).all() and (db == 0).all()
+    for bad in (dy[:, :16], dy[:3], dy.float(), dy.cpu(), dy[0].expand(4, 32)):
+        with pytest.raises(RuntimeError):
+            ext.w8a8_linear_backward(bad, a, w, sa, sw)
+    with pytest.raises(RuntimeError):
+        ext.w8a8_gated_backward(dy, a, w, sa, sw)            # [4, 16] wanted
+    with pytest.raises(RuntimeError, match="activation"):
+        ext.w8a8_gated_backward(dy[:, :16], a, w, sa, sw, None, "none")
+
+
+def test_two_runs_other_streams_and_captured_replays(ext):
+    m, i, k = 200, 136, 272
+    (a, sa), (w, sw) = ref.tokens(m, k, 1), ref.weight(2 * i, k, 2)
+    b = ref.bf16((2 * i,), 3)
+    a, sa, w, sw, b = cuda(a, sa, w, sw, b)
+    dh = ref.bf16((m, i), 4).cuda()
+    want = ext.w8a8_gated_backward(dh, a, w, sa, sw, b)
+    again = ext.w8a8_gated_backward(dh, a, w, sa, sw, b)
+    assert all(torch.equal(p, q) for p, q in zip(want, again))
+    torch.cuda.synchronize()
+    side, outs = torch.cuda.Stream(), []
+    for _ in range(10):
+        outs.append(ext.w8a8_gated_backward_stream(dh, a, w, sa, sw, b, "silu", side.cuda_stream))
+        torch.full((8 << 20,), 77, dtype=torch.uint8, device="cuda")   # would land in a workspace freed to this stream
+    side.synchronize()
+    assert all(torch.equal(p, q) for o in outs for p, q in zip(want, o))
+    graphs = []
+    for _ in range(2):   # two graphs alive at once, replayed alternately
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ext.w8a8_gated_backward(dh, a, w, sa, sw, b)
+            lin = ext.w8a8_linear_backward(dh, a, w[:i], sa, sw[:i], b[:i], "none")
+        graphs.append((graph, out, lin))
+    for seed in (11, 12, 13):
+        dh.copy_(ref.bf16((m, i), seed))
+        for graph, _, _ in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        want = ext.w8a8_gated_backward(dh, a, w, sa, sw, b)
+        lin64 = ext.w8a8_linear_backward(dh, a, w[:i], sa, sw[:i], b[:i], "none")
+        for _, out, lin in graphs:
+            assert all(torch.equal(p, q) for p, q in zip(want, out))
+            assert all(torch.equal(p, q) for p, q in zip(lin64, lin))
+    assert ext.device_status() == 0
