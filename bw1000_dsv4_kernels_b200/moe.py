@@ -23,6 +23,9 @@ experts.  Two ways to put the rows together:
     rounding, not bit for bit; integer codes, scales and accumulators per expert are identical.
   * ExchangeW8A8MoE: the combine pulls the expert rows from peer memory and pushes the finished bf16
     rows to every rank in one kernel; the result is bit-identical to the single-GPU forward.
+
+A shared expert (`shared`: a ffn.W8A8GatedFFN or ffn.W8A8FFN that every rank holds in full) runs on every token; the
+routed result goes in as the residual of its down projection, so adding it takes no pass of its own.
 """
 from dataclasses import dataclass
 from typing import Optional
@@ -59,7 +62,7 @@ class W8A8MoE:
     """
 
     def __init__(self, w13, w13_scale, w2, w2_scale, num_experts: int, expert_lo: int = 0,
-                 group_scaled: bool = True, process_group=None):
+                 group_scaled: bool = True, process_group=None, shared=None):
         self.w13, self.w13_scale, self.w2, self.w2_scale = w13, w13_scale, w2, w2_scale
         self.e_local = w13.shape[0]
         self.inter = w2.shape[2]
@@ -68,6 +71,7 @@ class W8A8MoE:
         self.num_experts, self.expert_lo = num_experts, expert_lo
         self.group_scaled = group_scaled
         self.pg = process_group
+        self.shared = shared
         self.last_trace: Optional[MoeTrace] = None
 
     def local_partial(self, x, topk_ids, topk_w, out_f32: bool, keep_trace: bool = False):
@@ -89,18 +93,21 @@ class W8A8MoE:
             self.last_trace = MoeTrace(off, src_row, dst_slot, a_q, a_s, y, h_q, h_s, z)
         return out
 
+    def _add_shared(self, x, routed):
+        return routed if self.shared is None else self.shared.forward(x, residual=routed)
+
     def forward(self, x, topk_ids, topk_w, keep_trace: bool = False):
         """x bf16 [T,H], topk_ids int32 [T,topk], topk_w fp32 [T,topk] -> bf16 [T,H]."""
         single = self.pg is None and self.e_local == self.num_experts
         if single:
-            return self.local_partial(x, topk_ids, topk_w, out_f32=False, keep_trace=keep_trace)
+            return self._add_shared(x, self.local_partial(x, topk_ids, topk_w, out_f32=False, keep_trace=keep_trace))
         import torch.distributed as dist
         if self.pg is None and not dist.is_initialized():
             raise RuntimeError("W8A8MoE.forward: this rank holds an expert shard but there is no process group to sum the "
                                "ranks' partial results over; call local_partial() if the partial sum is what you want")
         part = self.local_partial(x, topk_ids, topk_w, out_f32=True, keep_trace=keep_trace)
         dist.all_reduce(part, group=self.pg)
-        return part.to(torch.bfloat16)
+        return self._add_shared(x, part.to(torch.bfloat16))
 
 
 def token_range(rank: int, world: int, tokens: int):
@@ -122,10 +129,10 @@ class ExchangeW8A8MoE(W8A8MoE):
     """
 
     def __init__(self, w13, w13_scale, w2, w2_scale, num_experts: int, rank: int, world: int, t_max: int, topk: int,
-                 device, group_scaled: bool = True, process_group=None):
+                 device, group_scaled: bool = True, process_group=None, shared=None):
         per = num_experts // world
         assert per * world == num_experts and w13.shape[0] == per
-        super().__init__(w13, w13_scale, w2, w2_scale, num_experts, rank * per, group_scaled, process_group)
+        super().__init__(w13, w13_scale, w2, w2_scale, num_experts, rank * per, group_scaled, process_group, shared)
         import torch.distributed as dist
         import torch.distributed._symmetric_memory as symm_mem
         self.rank, self.world, self.t_max, self.topk = rank, world, t_max, topk
@@ -162,7 +169,7 @@ class ExchangeW8A8MoE(W8A8MoE):
         _ext().moe_combine_exchange(self.z_ptrs, self.slot_ptrs, topk_ids, topk_w, self.out_ptrs,
                                     self.num_experts // self.world, t0, t1, self.hidden)
         self.handle.barrier(channel=1)      # every rank's rows have landed everywhere
-        return self.out[:t]
+        return self._add_shared(x, self.out[:t])
 
 
 class PushExchangeW8A8MoE(W8A8MoE):
@@ -178,10 +185,10 @@ class PushExchangeW8A8MoE(W8A8MoE):
     """
 
     def __init__(self, w13, w13_scale, w2, w2_scale, num_experts: int, rank: int, world: int, t_max: int, topk: int,
-                 device, group_scaled: bool = True, process_group=None):
+                 device, group_scaled: bool = True, process_group=None, shared=None):
         per = num_experts // world
         assert per * world == num_experts and w13.shape[0] == per
-        super().__init__(w13, w13_scale, w2, w2_scale, num_experts, rank * per, group_scaled, process_group)
+        super().__init__(w13, w13_scale, w2, w2_scale, num_experts, rank * per, group_scaled, process_group, shared)
         import torch.distributed as dist
         import torch.distributed._symmetric_memory as symm_mem
         self.rank, self.world, self.t_max, self.topk = rank, world, t_max, topk
@@ -227,7 +234,7 @@ class PushExchangeW8A8MoE(W8A8MoE):
         ext.moe_combine_exchange(inbox, slots, topk_ids, topk_w, self.out_ptrs, self.num_experts // self.world,
                                  t0, t1, self.hidden)
         self.handle.barrier(channel=1)      # every rank's output rows have landed everywhere, inboxes are free again
-        return self.out[:t]
+        return self._add_shared(x, self.out[:t])
 
 
 def route(router_logits: torch.Tensor, topk: int):
