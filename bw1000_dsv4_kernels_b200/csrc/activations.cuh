@@ -1,6 +1,6 @@
-// Activations of the fused linear and gated epilogues and their derivatives, fp32.  exp and erfc are CUDA's own; the
-// sigmoid takes the fast exponential, whose relative error (about 2^-21 at the arguments where the result still
-// matters) is far below the bf16 step of every output that it reaches.
+// Activations of the fused linear and gated epilogues and their derivatives, fp32.  They take CUDA's fast exponential and
+// reciprocal, whose relative error (about 2^-21 at the arguments where the result still matters) is far below the bf16
+// step of every output that they reach.
 #pragma once
 #include <cuda_runtime.h>
 
@@ -16,13 +16,27 @@ constexpr float kGeluCubic = 0.044715f;
 
 __device__ __forceinline__ float sigmoid_fast(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
 
-// erfc(-z / sqrt 2) rather than 1 + erf: it keeps its relative accuracy where the normal distribution's tail is small
-__device__ __forceinline__ float normal_cdf(float z) { return 0.5f * erfcf(-z * kSqrtHalf); }
+// Phi(z), the normal distribution function, and exp(-z^2 / 2), which Phi's formula needs anyway and the density is made of.
+// 0.5 * erfc(|z| / sqrt 2) by Abramowitz and Stegun, Handbook of Mathematical Functions, formula 7.1.26: a polynomial of
+// degree five in 1 / (1 + 0.3275911 x) times exp(-x^2), off by at most 0.75e-7.  erfcf is exact to the last bits but takes
+// four times the instructions and branches on its argument, which made the drain of a 7168-deep tile longer than its
+// tensor-core work.
+__device__ __forceinline__ float2 normal_cdf_exp(float z) {
+    const float x = fabsf(z) * kSqrtHalf;
+    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
+    const float e = __expf(-x * x);
+    float q = fmaf(t, 1.061405429f, -1.453152027f);
+    q = fmaf(t, q, 1.421413741f);
+    q = fmaf(t, q, -0.284496736f);
+    q = fmaf(t, q, 0.254829592f);
+    q = q * t * e * 0.5f;
+    return make_float2(z > 0.0f ? 1.0f - q : q, e);
+}
 
 template <int ACT>
 __device__ __forceinline__ float act_value(float z) {
     if constexpr (ACT == kActRelu) return z > 0.0f ? z : (z != z ? z : 0.0f);
-    if constexpr (ACT == kActGelu) return z * normal_cdf(z);
+    if constexpr (ACT == kActGelu) return z * normal_cdf_exp(z).x;
     if constexpr (ACT == kActGeluTanh) return z * sigmoid_fast(kGeluTanhC * fmaf(kGeluCubic * z * z, z, z));
     if constexpr (ACT == kActSilu) return z * sigmoid_fast(z);
     return z;
@@ -33,8 +47,8 @@ template <int ACT>
 __device__ __forceinline__ float2 act_value_slope(float z) {
     if constexpr (ACT == kActRelu) return make_float2(act_value<kActRelu>(z), z > 0.0f ? 1.0f : 0.0f);
     if constexpr (ACT == kActGelu) {
-        const float p = normal_cdf(z);
-        return make_float2(z * p, fmaf(z * kInvSqrt2Pi, __expf(-0.5f * z * z), p));
+        const float2 p = normal_cdf_exp(z);
+        return make_float2(z * p.x, fmaf(z * kInvSqrt2Pi, p.y, p.x));
     }
     if constexpr (ACT == kActGeluTanh) {
         const float z2 = z * z;

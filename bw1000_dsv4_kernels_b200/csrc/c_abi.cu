@@ -311,9 +311,9 @@ int launch_w8a8_gated(const void* A, const void* B, const void* sa, const void* 
     return gemm_i8(a, cs(stream));
 }
 
-int64_t dsv4_w8a8_backward_workspace(int M, int weight_rows, int act, int want_dbias) {
+int64_t dsv4_w8a8_backward_workspace(int M, int weight_rows, int gated, int act, int want_dbias) {
     if (M <= 0 || weight_rows <= 0) return 0;
-    return w8a8_backward_workspace(M, weight_rows, act != DSV4_ACT_NONE, want_dbias != 0);
+    return w8a8_backward_workspace(M, weight_rows, gated != 0, act != DSV4_ACT_NONE, want_dbias != 0);
 }
 
 static int backward_entry(const char* op, bool gated, const void* dy, int64_t ldy, const void* A, const void* B, const void* sa,
@@ -344,7 +344,7 @@ static int backward_entry(const char* op, bool gated, const void* dy, int64_t ld
     if ((reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(B) & 15)) return bad("A and B must be 16-byte aligned");
     if (ldy < (gated ? N / 2 : N)) return bad("gradient row stride smaller than its row");
     if ((int64_t)2 * M > INT32_MAX) return bad("too many rows");
-    if (workspace_bytes < w8a8_backward_workspace(M, N, act != DSV4_ACT_NONE, dbias != nullptr) ||
+    if (workspace_bytes < w8a8_backward_workspace(M, N, gated, act != DSV4_ACT_NONE, dbias != nullptr) ||
         (reinterpret_cast<uintptr_t>(workspace) & 15))
         return bad("the workspace is smaller than dsv4_w8a8_backward_workspace or not 16-byte aligned");
     BackwardArgs a;

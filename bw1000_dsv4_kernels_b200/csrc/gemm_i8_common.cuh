@@ -74,9 +74,13 @@ struct Params {
     int64_t ldr;
     int act;
     int inter;
-    // gradient epilogues: resid is the incoming gradient (dy or dh), C the fp32 gradient of z with row stride ldc, and
-    // row_top[row] collects the largest |dz * sb| of the row as the bits of a non-negative float
+    // gradient epilogues: resid is the incoming gradient (dy or dh), C the fp32 gradient of z with row stride ldc (a
+    // multiple of four; a gated problem's ups start at column `up_col`), and row_top[row] collects the largest |dz * sb| of
+    // the row as the bits of a non-negative float
     unsigned* row_top;
+    int up_col;
+    // fused CTA-pair kernel: rows of B per tile, gates and ups together (a multiple of 32, of 64 when gated)
+    int tile_n;
 };
 
 template <int BN, int STAGES>

@@ -61,172 +61,178 @@ __device__ __forceinline__ float scaled(uint32_t acc, float sa, float sb, float 
     return __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn((int)acc), sa), sb), bias);
 }
 
-// Column scales and biases of a tile -> this warp's shared copy.  Columns [0, half) of the tile come from output column
-// n0 on, columns [half, 2 half) from `second` on (a gated tile's up rows, or simply the next columns).
-__device__ __forceinline__ void stage_columns(const Params& p, float* sbs, float* bias_s, int lane, int half, int first,
-                                              int second, int first_end, int second_end) {
-    for (int j = lane; j < 2 * half; j += 32) {
-        const int c = j < half ? first + j : second + (j - half);
-        const bool ok = c < (j < half ? first_end : second_end);
-        sbs[j] = ok ? __ldg(p.sb + c) : 0.0f;
-        bias_s[j] = ok && p.bias != nullptr ? __bfloat162float(p.bias[c]) : 0.0f;
+// A warp's 32 x 32 block of a bf16 array, one row per lane.  Rows that are 16-byte aligned move as four 16-byte accesses
+// per lane.  Otherwise (odd widths, odd addresses) an access per element and lane would touch 32 lines each, 32 times;
+// the block goes through the warp's shared memory instead, where lane = column makes each row one access.
+constexpr int kStagePitch = 17;                        // words per row: 16 plus one against bank conflicts
+constexpr int kBlockBytes = 32 * kStagePitch * 4;
+struct RowBlock {
+    int rows;     // valid rows of the block (lane r owns row r)
+    int cols;     // valid columns
+    bool vec;     // rows are 16-byte aligned
+};
+__device__ __forceinline__ Row32 load_block(const __nv_bfloat16* block, int64_t ld, const RowBlock& b, uint32_t* stage, int lane) {
+    Row32 r = {};
+    if (b.vec && b.cols >= 32) {
+        if (lane < b.rows) load_row32(r, block + lane * ld, 32, true);
+        return r;
+    }
+    __syncwarp();
+    uint16_t* s16 = reinterpret_cast<uint16_t*>(stage);
+    const uint16_t* src = reinterpret_cast<const uint16_t*>(block) + lane;
+#pragma unroll 8
+    for (int i = 0; i < 32; ++i)
+        s16[i * (2 * kStagePitch) + lane] = i < b.rows && lane < b.cols ? src[i * ld] : (uint16_t)0;
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) r.w[j] = stage[lane * kStagePitch + j];
+    return r;
+}
+__device__ __forceinline__ void store_block(__nv_bfloat16* block, int64_t ld, const Row32& r, const RowBlock& b, uint32_t* stage,
+                                            int lane) {
+    if (b.vec && b.cols >= 32) {
+        if (lane < b.rows) store_row32(block + lane * ld, r, 32, true);
+        return;
+    }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < 16; ++j) stage[lane * kStagePitch + j] = r.w[j];
+    __syncwarp();
+    const uint16_t* s16 = reinterpret_cast<const uint16_t*>(stage);
+    uint16_t* dst = reinterpret_cast<uint16_t*>(block) + lane;
+    if (lane < b.cols) {
+#pragma unroll 8
+        for (int i = 0; i < 32; ++i)
+            if (i < b.rows) dst[i * ld] = s16[i * (2 * kStagePitch) + lane];
     }
 }
 
-// One finished accumulator of NCOLS columns: this thread owns tile row `row`.  The residual of the next 32 columns is
-// requested before the current ones are worked on.
+// larger magnitude, as bits: unlike fmaxf it keeps a NaN, which then reaches the whole row of the result
+__device__ __forceinline__ unsigned top_bits(unsigned top, float v) { return max(top, __float_as_uint(v) & 0x7fffffffu); }
+
+// 32 columns of scales or biases in this warp's shared memory
+struct Cols32 {
+    const float* p;
+    __device__ __forceinline__ float operator[](int e) const { return p[e]; }
+};
+
+// Column scales and biases of a tile -> a warp's shared copy (one CTA per tile kernel)
+__device__ __forceinline__ void stage_columns(const Params& p, float* sbs, float* bias_s, int lane, int count, int first) {
+    for (int j = lane; j < count; j += 32) {
+        const int c = first + j;
+        sbs[j] = c < p.N ? __ldg(p.sb + c) : 0.0f;
+        bias_s[j] = c < p.N && p.bias != nullptr ? __bfloat162float(p.bias[c]) : 0.0f;
+    }
+}
+
+// y of 32 columns from the accumulators of one row
+template <int ACT>
+__device__ __forceinline__ Row32 linear_values(const uint32_t (&r)[32], float sa, Cols32 sb, Cols32 bias, bool has_res,
+                                               const Row32& res) {
+    Row32 out;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        float y[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int e = 2 * j + h;
+            y[h] = act_value<ACT>(scaled(r[e], sa, sb[e], bias[e]));
+            if (has_res) y[h] = __fadd_rn(y[h], row32_at(res, e));
+        }
+        out.w[j] = pack_bf16x2_rn(y[0], y[1]);
+    }
+    return out;
+}
+
+// One finished accumulator of NCOLS columns (one CTA per tile kernel): this thread owns tile row `row`.
 template <int NCOLS>
 __device__ __forceinline__ void drain_linear(const Params& p, uint32_t t_lane, const float* sbs, const float* bias_s, int row,
                                              bool row_ok, int n0, bool vec_ok) {
     const float sa = row_ok ? __ldg(p.sa + row) : 0.0f;
     const bool has_res = p.resid != nullptr && row_ok;
     const bool res_vec = row_vector_ok(p.resid, p.ldr);
-    const __nv_bfloat16* rrow = p.resid + (int64_t)row * p.ldr;
-    Row32 res = {};
-    if (has_res && n0 < p.N) load_row32(res, rrow + n0, p.N - n0, res_vec);
 #pragma unroll 1
     for (int cc = 0; cc < NCOLS / 32; ++cc) {
+        const int n = n0 + cc * 32;
+        Row32 res = {};
+        if (has_res && n < p.N) load_row32(res, p.resid + (int64_t)row * p.ldr + n, p.N - n, res_vec);
         uint32_t r[32];
         __syncwarp();  // tcgen05.ld is warp-collective: reconverge after the stores
         ptx::tmem_ld_32x32b_x32(t_lane + cc * 32, r);
-        const int n = n0 + cc * 32;
-        Row32 next = {};
-        if (has_res && cc + 1 < NCOLS / 32 && n + 32 < p.N) load_row32(next, rrow + n + 32, p.N - n - 32, res_vec);
         ptx::tmem_ld_wait();
         if (row_ok && n < p.N) {
             Row32 out;
             with_act(p.act, [&](auto a) {
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    float y[2];
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int e = 2 * j + h;
-                        y[h] = act_value<decltype(a)::value>(scaled(r[e], sa, sbs[cc * 32 + e], bias_s[cc * 32 + e]));
-                        if (has_res) y[h] = __fadd_rn(y[h], row32_at(res, e));
-                    }
-                    out.w[j] = pack_bf16x2_rn(y[0], y[1]);
-                }
+                out = linear_values<decltype(a)::value>(r, sa, {sbs + cc * 32}, {bias_s + cc * 32}, has_res, res);
             });
             store_row32(static_cast<__nv_bfloat16*>(p.C) + (int64_t)row * p.ldc + n, out, p.N - n, vec_ok);
         }
-        res = next;
     }
 }
 
-// A gated tile: accumulator columns [0, 128) are gates, [128, 256) the ups of the same 128 outputs.
-__device__ __forceinline__ void drain_gated(const Params& p, uint32_t t_lane, const float* sbs, const float* bias_s, int row,
-                                            bool row_ok, int n0, bool vec_ok) {
-    const float sa = row_ok ? __ldg(p.sa + row) : 0.0f;
-#pragma unroll 1
-    for (int cc = 0; cc < 4; ++cc) {
-        uint32_t g[32], u[32];
-        __syncwarp();
-        ptx::tmem_ld_32x32b_x32(t_lane + cc * 32, g);
-        ptx::tmem_ld_32x32b_x32(t_lane + 128 + cc * 32, u);
-        ptx::tmem_ld_wait();
-        const int n = n0 + cc * 32;
-        if (!row_ok || n >= p.N) continue;
-        Row32 out;
-        with_act(p.act, [&](auto a) {
+// h of 32 outputs from the accumulators of their gates and ups
+template <int ACT>
+__device__ __forceinline__ Row32 gated_values(const uint32_t (&g)[32], const uint32_t (&u)[32], float sa, Cols32 sg, Cols32 bg,
+                                              Cols32 su, Cols32 bu) {
+    Row32 out;
 #pragma unroll
-            for (int j = 0; j < 16; ++j) {
-                float h[2];
+    for (int j = 0; j < 16; ++j) {
+        float h[2];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int e = 2 * j + k, c = cc * 32 + e;
-                    h[k] = act_value<decltype(a)::value>(scaled(g[e], sa, sbs[c], bias_s[c])) *
-                           scaled(u[e], sa, sbs[128 + c], bias_s[128 + c]);
-                }
-                out.w[j] = pack_bf16x2_rn(h[0], h[1]);
-            }
-        });
-        store_row32(static_cast<__nv_bfloat16*>(p.C) + (int64_t)row * p.ldc + n, out, p.N - n, vec_ok);
+        for (int k = 0; k < 2; ++k) {
+            const int e = 2 * j + k;
+            h[k] = act_value<ACT>(scaled(g[e], sa, sg[e], bg[e])) * scaled(u[e], sa, su[e], bu[e]);
+        }
+        out.w[j] = pack_bf16x2_rn(h[0], h[1]);
     }
+    return out;
 }
 
-__device__ __forceinline__ void store_f32x2(float* p, float a, float b, int n_left, bool vec) {
-    if (vec) {   // n_left is even then
-        if (n_left >= 2) *reinterpret_cast<float2*>(p) = make_float2(a, b);
-    } else {
-        if (n_left >= 1) p[0] = a;
-        if (n_left >= 2) p[1] = b;
-    }
-}
-// larger magnitude, as bits: unlike fmaxf it keeps a NaN, which then reaches the whole row of the result
-__device__ __forceinline__ unsigned top_bits(unsigned top, float v) { return max(top, __float_as_uint(v) & 0x7fffffffu); }
-
-template <int NCOLS>
-__device__ __forceinline__ void drain_linear_grad(const Params& p, uint32_t t_lane, const float* sbs, const float* bias_s,
-                                                  int row, bool row_ok, int n0) {
-    const float sa = row_ok ? __ldg(p.sa + row) : 0.0f;
-    const bool dy_vec = row_vector_ok(p.resid, p.ldr), z_vec = p.ldc % 4 == 0;
-    unsigned top = 0;
-#pragma unroll 1
-    for (int cc = 0; cc < NCOLS / 32; ++cc) {
-        uint32_t r[32];
-        const int n = n0 + cc * 32, left = p.N - n;
-        Row32 dy = {};
-        if (row_ok && left > 0) load_row32(dy, p.resid + (int64_t)row * p.ldr + n, left, dy_vec);
-        __syncwarp();
-        ptx::tmem_ld_32x32b_x32(t_lane + cc * 32, r);
-        ptx::tmem_ld_wait();
-        if (!row_ok || left <= 0) continue;
-        float* out = static_cast<float*>(p.C) + (int64_t)row * p.ldc + n;
-        with_act(p.act, [&](auto a) {
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-                float dz[2];
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int e = j + k, c = cc * 32 + e;
-                    dz[k] = row32_at(dy, e) * act_value_slope<decltype(a)::value>(scaled(r[e], sa, sbs[c], bias_s[c])).y;
-                    if (e < left) top = top_bits(top, dz[k] * sbs[c]);
-                }
-                store_f32x2(out + j, dz[0], dz[1], left - j, z_vec);
-            }
-        });
-    }
-    if (row_ok && top != 0) atomicMax(p.row_top + row, top);
+__device__ __forceinline__ void store4f(float* p, const float (&v)[4]) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
 }
 
-__device__ __forceinline__ void drain_gated_grad(const Params& p, uint32_t t_lane, const float* sbs, const float* bias_s,
-                                                 int row, bool row_ok, int n0) {
-    const float sa = row_ok ? __ldg(p.sa + row) : 0.0f;
-    const bool dh_vec = row_vector_ok(p.resid, p.ldr), z_vec = p.ldc % 4 == 0 && p.inter % 2 == 0;
-    unsigned top = 0;
-#pragma unroll 1
-    for (int cc = 0; cc < 4; ++cc) {
-        uint32_t g[32], u[32];
-        const int n = n0 + cc * 32, left = p.N - n;
-        Row32 dh = {};
-        if (row_ok && left > 0) load_row32(dh, p.resid + (int64_t)row * p.ldr + n, left, dh_vec);
-        __syncwarp();
-        ptx::tmem_ld_32x32b_x32(t_lane + cc * 32, g);
-        ptx::tmem_ld_32x32b_x32(t_lane + 128 + cc * 32, u);
-        ptx::tmem_ld_wait();
-        if (!row_ok || left <= 0) continue;
-        float* out_g = static_cast<float*>(p.C) + (int64_t)row * p.ldc + n;
-        float* out_u = out_g + p.inter;
-        with_act(p.act, [&](auto a) {
+// dz of 32 columns -> dz (16-byte aligned); returns the largest |dz * sb| as bits, together with `top`
+template <int ACT>
+__device__ __forceinline__ unsigned linear_gradients(const uint32_t (&r)[32], float sa, Cols32 sb, Cols32 bias, const Row32& dy,
+                                                     float* dz, bool store, unsigned top) {
 #pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-                float dg[2], du[2];
+    for (int j = 0; j < 32; j += 4) {
+        float v[4];
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int e = j + k, c = cc * 32 + e;
-                    const float2 vs = act_value_slope<decltype(a)::value>(scaled(g[e], sa, sbs[c], bias_s[c]));
-                    const float zu = scaled(u[e], sa, sbs[128 + c], bias_s[128 + c]), d = row32_at(dh, e);
-                    dg[k] = d * zu * vs.y;
-                    du[k] = d * vs.x;
-                    if (e < left) top = top_bits(top_bits(top, dg[k] * sbs[c]), du[k] * sbs[128 + c]);
-                }
-                store_f32x2(out_g + j, dg[0], dg[1], left - j, z_vec);
-                store_f32x2(out_u + j, du[0], du[1], left - j, z_vec);
-            }
-        });
+        for (int k = 0; k < 4; ++k) {
+            const int e = j + k;
+            v[k] = row32_at(dy, e) * act_value_slope<ACT>(scaled(r[e], sa, sb[e], bias[e])).y;
+            top = top_bits(top, v[k] * sb[e]);
+        }
+        if (store) store4f(dz + j, v);
     }
-    if (row_ok && top != 0) atomicMax(p.row_top + row, top);
+    return top;
+}
+
+// dg and du of 32 outputs
+template <int ACT>
+__device__ __forceinline__ unsigned gated_gradients(const uint32_t (&g)[32], const uint32_t (&u)[32], float sa, Cols32 sg,
+                                                    Cols32 bg, Cols32 su, Cols32 bu, const Row32& dh, float* dg, float* du,
+                                                    bool store, unsigned top) {
+#pragma unroll
+    for (int j = 0; j < 32; j += 4) {
+        float vg[4], vu[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int e = j + k;
+            const float2 vs = act_value_slope<ACT>(scaled(g[e], sa, sg[e], bg[e]));
+            const float d = row32_at(dh, e);
+            vg[k] = d * scaled(u[e], sa, su[e], bu[e]) * vs.y;
+            vu[k] = d * vs.x;
+            top = top_bits(top_bits(top, vg[k] * sg[e]), vu[k] * su[e]);
+        }
+        if (store) {
+            store4f(dg + j, vg);
+            store4f(du + j, vu);
+        }
+    }
+    return top;
 }
 
 // Split-K epilogues of the weight-streaming kernels (see reduce_partials_and_store): the item's partials come through
@@ -284,43 +290,51 @@ __device__ __forceinline__ void reduce_partials_fused(const Params& p, const uin
                 }
             }
         }
+        float z[U][kHalves][4];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int it = it0 + u * nthreads;
-            if (it >= items) break;
-            const int c = cols_lo + (it >> kShift), g = it & (kGroups - 1);
-            const int n = n0 + g * 4;
-            if (n >= p.N) continue;
+            const bool ok = it < items;
+            const int c = ok ? cols_lo + (it >> kShift) : 0, g = it & (kGroups - 1);
             const float sa = sa_s[c];
-            float z[kHalves][4];
 #pragma unroll
             for (int h = 0; h < kHalves; ++h) {
                 int a[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int r = 0; r < MAXS; ++r) {
-                    if (r < S) {
+                    if (ok && r < S) {
                         a[0] += (int)v[u][h][r].x; a[1] += (int)v[u][h][r].y; a[2] += (int)v[u][h][r].z; a[3] += (int)v[u][h][r].w;
                     }
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    z[h][j] = scaled((uint32_t)a[j], sa, sb_s[h * 64 + g * 4 + j], bias_s[h * 64 + g * 4 + j]);
+                    z[u][h][j] = scaled((uint32_t)a[j], sa, sb_s[h * 64 + g * 4 + j], bias_s[h * 64 + g * 4 + j]);
             }
-            float y[4];
-            with_act(p.act, [&](auto act) {
+        }
+        // one choice of the activation for all items: a tile's epilogue runs once, so its instructions are fetched cold
+        with_act(p.act, [&](auto act) {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    y[j] = act_value<decltype(act)::value>(z[0][j]);
-                    if constexpr (GATED) y[j] *= z[kHalves - 1][j];
+                    z[u][0][j] = act_value<decltype(act)::value>(z[u][0][j]);
+                    if constexpr (GATED) z[u][0][j] *= z[u][kHalves - 1][j];
                 }
-            });
-            if (!GATED && p.resid != nullptr) {
-                y[0] = __fadd_rn(y[0], bf16lo_to_f32(res[u].x));
-                y[1] = __fadd_rn(y[1], bf16hi_to_f32(res[u].x));
-                y[2] = __fadd_rn(y[2], bf16lo_to_f32(res[u].y));
-                y[3] = __fadd_rn(y[3], bf16hi_to_f32(res[u].y));
             }
-            store4(p, c, n, y, vec_store);
+        });
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int it = it0 + u * nthreads;
+            if (it >= items) break;
+            const int c = cols_lo + (it >> kShift), n = n0 + (it & (kGroups - 1)) * 4;
+            if (n >= p.N) continue;
+            if (!GATED && p.resid != nullptr) {
+                z[u][0][0] = __fadd_rn(z[u][0][0], bf16lo_to_f32(res[u].x));
+                z[u][0][1] = __fadd_rn(z[u][0][1], bf16hi_to_f32(res[u].x));
+                z[u][0][2] = __fadd_rn(z[u][0][2], bf16lo_to_f32(res[u].y));
+                z[u][0][3] = __fadd_rn(z[u][0][3], bf16hi_to_f32(res[u].y));
+            }
+            store4(p, c, n, z[u][0], vec_store);
         }
     }
 }

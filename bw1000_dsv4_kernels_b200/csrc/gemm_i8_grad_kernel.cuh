@@ -20,7 +20,7 @@
 
 #include "gemm_i8_common.cuh"
 #include "gemm_i8_epilogues.cuh"
-#include "gemm_i8_pair_kernel.cuh"
+#include "gemm_i8_fused_pair_kernel.cuh"
 #include "gradient_digits.cuh"
 
 namespace w8a8 {
@@ -29,15 +29,18 @@ namespace {
 struct GradParams {
     const unsigned* row_top;   // [M] largest |t| of the row, as float bits
     __nv_bfloat16* dx;         // [M, K]
-    int M, N, K;               // N: length of the sum
+    int M, K;
+    // the sum runs over `parts` ranges of part_rows rows of W (gates and ups of a gated weight); a digit row holds them at
+    // columns that are multiples of part_blocks * 128, with zeros behind each
+    int parts, part_rows, part_blocks;
     int group_m;
     unsigned long long wait_limit_ns;
 };
 
-template <int STAGES>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFusedThreads, 1)
 gemm_i8_grad_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmW, const GradParams p) {
-    using L = PairSmem<STAGES, false>;
+    using L = FusedPairSmem;
+    constexpr int STAGES = L::kStages;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
@@ -57,7 +60,7 @@ gemm_i8_grad_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
             ptx::mbar_init(empty_bar(s), 1);
         }
         ptx::mbar_init(acc_full_bar, 1);
-        ptx::mbar_init(acc_empty_bar, 2 * (kDrainThreads / 32));
+        ptx::mbar_init(acc_empty_bar, 2 * kFusedDrainWarps);
         *abort_flag = 0;
         ptx::fence_barrier_init();
         ptx::fence_proxy_async_smem();
@@ -78,7 +81,7 @@ gemm_i8_grad_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     const int total = tiles_m * tiles_k;
     const PairTileOrder order{tiles_m, tiles_k, p.group_m};
     const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
-    const int blocks = (p.N + BK - 1) / BK;
+    const int blocks = p.parts * p.part_blocks;
 
     if (warp == 0) {
         // ---------------- TMA producer (both CTAs) ----------------
@@ -102,7 +105,9 @@ gemm_i8_grad_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
                         const uint32_t leader_full = ptx::map_to_cta(full_bar(stage), 0);
                         if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * L::kStageBytes);
                         ptx::tma_load_2d_pair(a_dst, &tmD, nb * BK, row0, leader_full);
-                        ptx::tma_load_2d_pair(a_dst + L::kABytes, &tmW, kt * 256 + (int)rank * 128, nb * BK, leader_full);
+                        const int part = nb >= p.part_blocks ? 1 : 0;
+                        ptx::tma_load_2d_pair(a_dst + L::kABytes, &tmW, kt * 256 + (int)rank * 128,
+                                              part * p.part_rows + (nb - part * p.part_blocks) * BK, leader_full);
                         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                     }
                 }
@@ -149,15 +154,16 @@ gemm_i8_grad_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
         }
     } else {
         // ---------------- drain warps (both CTAs) ----------------
-        const int quarter = warp & 3;
+        const int quarter = warp & 3, turn = (warp - 2) >> 2;
+        uint32_t* stage = reinterpret_cast<uint32_t*>(smem + L::kTransposeOff + (warp - 2) * kBlockBytes);
         uint32_t acc_phase = 0;
         const bool vec = p.K % 8 == 0 && (reinterpret_cast<uintptr_t>(p.dx) & 15) == 0;
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         for (int t = pair; t < total; t += npairs) {
             int mt, kt;
             order.at(t, mt, kt);
-            const int row = mt * 256 + (int)rank * 128 + quarter * 32 + lane;
-            const float s = row < p.M ? digit_scale(__uint_as_float(__ldg(p.row_top + row))) : 0.0f;
+            const int row0 = mt * 256 + (int)rank * 128 + quarter * 32, rows = min(32, p.M - row0);
+            const float s = lane < rows ? digit_scale(__uint_as_float(__ldg(p.row_top + row0 + lane))) : 0.0f;
             __syncwarp();
             if (!ptx::mbar_wait_bounded(acc_full_bar, acc_phase, p.wait_limit_ns) || *abort_flag) {
                 report_wait_failure(kWaitAccFull);
@@ -166,22 +172,23 @@ gemm_i8_grad_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
             }
             ptx::tc_fence_after_sync();
 #pragma unroll 1
-            for (int cc = 0; cc < 8; ++cc) {
+            for (int cc = turn; cc < 8; cc += 2) {
                 uint32_t hi[32], lo[32];
                 __syncwarp();
                 ptx::tmem_ld_32x32b_x32(t_lane + cc * 32, hi);
                 ptx::tmem_ld_32x32b_x32(t_lane + 256 + cc * 32, lo);
                 ptx::tmem_ld_wait();
                 const int k = kt * 256 + cc * 32;
-                if (row >= p.M || k >= p.K) continue;
+                if (rows <= 0 || k >= p.K) continue;
                 Row32 out;
 #pragma unroll
                 for (int j = 0; j < 16; ++j)
                     out.w[j] = pack_bf16x2_rn(digit_value((int)hi[2 * j], (int)lo[2 * j], s),
                                               digit_value((int)hi[2 * j + 1], (int)lo[2 * j + 1], s));
-                store_row32(p.dx + (int64_t)row * p.K + k, out, p.K - k, vec);
+                store_block(p.dx + (int64_t)row0 * p.K + k, p.K, out, {rows, p.K - k, vec}, stage, lane);
             }
             ptx::tc_fence_before_sync();
+            __syncwarp();
             if (lane == 0) ptx::mbar_arrive_cluster(ptx::map_to_cta(acc_empty_bar, 0));
             acc_phase ^= 1u;
         }

@@ -4,7 +4,6 @@
 #define W8A8_GEMM_I8_PAIR_KERNEL_CUH
 
 #include "gemm_i8_common.cuh"
-#include "gemm_i8_epilogues.cuh"
 
 namespace w8a8 {
 namespace {
@@ -35,8 +34,7 @@ struct PairSmem {
     static constexpr int kOutOff = kTilesBytes;
     static constexpr int kOutBytes = TMA_STORE ? kOutSlots * kOutSlabBytes : 0;
     static constexpr int kSbOff = kOutOff + kOutBytes;          // 4 warps x 256 column scales
-    static constexpr int kBiasOff = kSbOff + 4 * 256 * 4;       // 4 warps x 256 biases (not beside the output staging)
-    static constexpr int kBarOff = kBiasOff + (TMA_STORE ? 0 : 4 * 256 * 4);  // 8-byte aligned
+    static constexpr int kBarOff = kSbOff + 4 * 256 * 4;        // 8-byte aligned
     static constexpr int kNumBars = 2 * STAGES + 4;
     static constexpr int kTmemSlotOff = kBarOff + kNumBars * 8;
     static constexpr int kAbortOff = kTmemSlotOff + 4;
@@ -69,16 +67,12 @@ struct StoreMaps {
     int count;
 };
 
-template <int STAGES, bool TMA_STORE, int EPI = kEpiPlain>
+template <int STAGES, bool TMA_STORE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const Params p, const __grid_constant__ StoreMaps smaps) {
     using L = PairSmem<STAGES, TMA_STORE>;
-    static_assert(EPI == kEpiPlain || !TMA_STORE, "the fused epilogues store from registers");
     constexpr int PBN = 256;  // tile width of the pair
-    // a gated tile is 128 gate rows (the even CTA's) and the 128 up rows of the same outputs (the odd CTA's)
-    constexpr bool kGated = is_gated(EPI);
-    constexpr int kOutCols = kGated ? 128 : PBN;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     float* sb_tile = reinterpret_cast<float*>(smem + L::kSbOff);
@@ -124,7 +118,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const uint32_t tmem_base = *tmem_slot;
 
     const int tiles_m = (p.M + 255) / 256;
-    const int tiles_n = (p.N + kOutCols - 1) / kOutCols;
+    const int tiles_n = (p.N + PBN - 1) / PBN;
     const int total = tiles_m * tiles_n;
     const PairTileOrder order{tiles_m, tiles_n, p.pair_group_m};
     const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
@@ -151,7 +145,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             for (Cursor c = c0; first < STAGES && c.t < total; ++first, advance(c)) {
                 int mt, nt;
                 order.at(c.t, mt, nt);
-                const int b_row0 = kGated ? nt * 128 + (int)rank * p.inter : nt * PBN + (int)rank * 128;
+                const int b_row0 = nt * PBN + (int)rank * 128;
                 if (rank == 0) ptx::mbar_arrive_expect_tx(full_bar(first), 2 * L::kStageBytes);
                 ptx::tma_load_2d_pair(tiles_base + first * L::kStageBytes + L::kABytes, &tmB, c.kb * BK, b_row0,
                                       ptx::map_to_cta(full_bar(first), 0));
@@ -171,7 +165,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
                 int mt, nt;
                 order.at(c.t, mt, nt);
                 const int a_row0 = mt * 256 + (int)rank * 128;
-                const int b_row0 = kGated ? nt * 128 + (int)rank * p.inter : nt * PBN + (int)rank * 128;
+                const int b_row0 = nt * PBN + (int)rank * 128;
                 for (; c.kb < k_blocks; ++c.kb) {
                     if (!ptx::mbar_wait_bounded(empty_bar(stage), phase ^ 1u, p.wait_limit_ns) || *abort_flag) {
                         report_wait_failure(kWaitEmptyStage);
@@ -239,7 +233,6 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         ptx::grid_dependency_wait();  // before reading activation scales or writing C
         const int quarter = warp & 3;
         float* sbs = sb_tile + (warp - 2) * PBN;
-        [[maybe_unused]] float* bias_s = reinterpret_cast<float*>(smem + L::kBiasOff) + (warp - 2) * PBN;
         int acc = 0;
         uint32_t acc_phase = 0;
         int out_slot = 0;  // next slab of the output staging ring (fused all-gather epilogue)
@@ -247,13 +240,9 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         for (int t = pair; t < total; t += npairs) {
             int mt, nt;
             order.at(t, mt, nt);
-            const int n0 = nt * kOutCols;
+            const int n0 = nt * PBN;
             __syncwarp();
-            if constexpr (EPI == kEpiLinear || EPI == kEpiLinearGrad) {
-                stage_columns(p, sbs, bias_s, lane, 128, n0, n0 + 128, p.N, p.N);
-            } else if constexpr (kGated) {
-                stage_columns(p, sbs, bias_s, lane, 128, n0, p.inter + n0, p.inter, 2 * p.inter);
-            } else if (!p.out_i32) {
+            if (!p.out_i32) {
                 for (int j = lane; j < PBN; j += 32) sbs[j] = (n0 + j < p.N) ? __ldg(p.sb + n0 + j) : 0.0f;
             }
             __syncwarp();
@@ -268,15 +257,7 @@ gemm_i8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
             ptx::tc_fence_after_sync();
             const int row = mt * 256 + (int)rank * 128 + quarter * 32 + lane;
             const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * PBN;
-            if constexpr (EPI == kEpiLinear) {
-                drain_linear<PBN>(p, t_lane, sbs, bias_s, row, row < p.M, n0, vec_ok);
-            } else if constexpr (EPI == kEpiLinearGrad) {
-                drain_linear_grad<PBN>(p, t_lane, sbs, bias_s, row, row < p.M, n0);
-            } else if constexpr (EPI == kEpiGatedGrad) {
-                drain_gated_grad(p, t_lane, sbs, bias_s, row, row < p.M, n0);
-            } else if constexpr (kGated) {
-                drain_gated(p, t_lane, sbs, bias_s, row, row < p.M, n0, vec_ok);
-            } else if constexpr (!TMA_STORE) {
+            if constexpr (!TMA_STORE) {
                 drain_accumulator<PBN>(p, t_lane, sbs, row, row < p.M, n0, vec_ok);
             } else {
                 // Fused all-gather epilogue: the bf16 tile goes through shared memory one 64-column slab

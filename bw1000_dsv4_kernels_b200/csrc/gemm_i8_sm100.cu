@@ -34,6 +34,7 @@
 #include "gemm_i8_common.cuh"
 #include "gemm_i8_tile_kernel.cuh"
 #include "gemm_i8_pair_kernel.cuh"
+#include "gemm_i8_fused_pair_kernel.cuh"
 #include "gemm_i8_stream_kernels.cuh"
 #include "gemm_i8_wt_kernel.cuh"
 #include "gemm_i8_grad_kernel.cuh"
@@ -315,21 +316,20 @@ int make_store_map(CUtensorMap* map, void* base, uint64_t rows, uint64_t cols, u
     return 0;
 }
 
-template <int STAGES, bool TMA_STORE, int EPI = kEpiPlain>
+template <int STAGES, bool TMA_STORE>
 int launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap& tmB, const Params& p, const StoreMaps& smaps,
                         cudaStream_t st) {
     using L = PairSmem<STAGES, TMA_STORE>;
     static_assert(L::kDynamic <= 227 * 1024, "shared memory limit");
     static bool opted_in[64] = {};
-    if (!opt_in_shared_memory(gemm_i8_pair_kernel<STAGES, TMA_STORE, EPI>, L::kDynamic, opted_in))
+    if (!opt_in_shared_memory(gemm_i8_pair_kernel<STAGES, TMA_STORE>, L::kDynamic, opted_in))
         return fail(DSV4_ERR_LAUNCH, "w8a8_gemm: cannot raise the dynamic shared memory limit");
-    const int out_cols = is_gated(EPI) ? 128 : 256;
-    const int tiles = ((p.M + 255) / 256) * ((p.N + out_cols - 1) / out_cols);
+    const int tiles = ((p.M + 255) / 256) * ((p.N + 255) / 256);
     int pairs = sm_count() / 2;
     if (pairs <= 0) return fail(DSV4_ERR_LAUNCH, "w8a8_gemm: no CUDA device");
     if (tiles < pairs) pairs = tiles;
     if (!overlap_previous_kernel()) {
-        gemm_i8_pair_kernel<STAGES, TMA_STORE, EPI><<<2 * pairs, kThreads, L::kDynamic, st>>>(tmA, tmB, p, smaps);
+        gemm_i8_pair_kernel<STAGES, TMA_STORE><<<2 * pairs, kThreads, L::kDynamic, st>>>(tmA, tmB, p, smaps);
         return check_launch("w8a8_gemm");
     }
     cudaLaunchConfig_t cfg = {};
@@ -342,7 +342,7 @@ int launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap& tmB, const Pa
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_pair_kernel<STAGES, TMA_STORE, EPI>, tmA, tmB, p, smaps);
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_pair_kernel<STAGES, TMA_STORE>, tmA, tmB, p, smaps);
     if (err != cudaSuccess) {
         cudaGetLastError();  // clear the sticky launch error
         static thread_local char msg[160];
@@ -350,6 +350,60 @@ int launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap& tmB, const Pa
         return fail(DSV4_ERR_LAUNCH, msg);
     }
     return check_launch("w8a8_gemm");
+}
+
+// Width of the fused pair kernel's tiles (rows of B, multiples of `unit` up to 256) for tiles_m rows of tiles, `rows` rows of
+// B and `pairs` CTA pairs: the width with the least rounds x time of a round.
+int fused_tile_n(int tiles_m, int rows, int unit, int pairs) {
+    int best = 256;
+    int64_t best_cost = INT64_MAX;
+    for (int w = 256; w >= unit; w -= unit) {
+        const int64_t tiles = (int64_t)tiles_m * ((rows + w - 1) / w);
+        const int64_t cost = (tiles + pairs - 1) / pairs * (256 + w);
+        if (cost < best_cost) {
+            best_cost = cost;
+            best = w;
+        }
+    }
+    return best;
+}
+
+template <int EPI, int ACT>
+int launch_fused_pair(const GemmArgs& a, Params p, cudaStream_t st) {
+    using L = FusedPairSmem;
+    static_assert(L::kDynamic <= 227 * 1024, "shared memory limit");
+    static bool opted_in[64] = {};
+    if (!opt_in_shared_memory(gemm_i8_fused_pair_kernel<EPI, ACT>, L::kDynamic, opted_in))
+        return fail(DSV4_ERR_LAUNCH, "w8a8_linear: cannot raise the dynamic shared memory limit");
+    int pairs = sm_count() / 2;
+    if (pairs <= 0) return fail(DSV4_ERR_LAUNCH, "w8a8_linear: no CUDA device");
+    const int w_rows = is_gated(EPI) ? 2 * a.N : a.N, tiles_m = (a.M + 255) / 256;
+    p.tile_n = fused_tile_n(tiles_m, w_rows, is_gated(EPI) ? 64 : 32, pairs);
+    const int out_n = is_gated(EPI) ? p.tile_n / 2 : p.tile_n;
+    CUtensorMap tmA, tmB;
+    if (int rc = make_tile_map(&tmA, a.A, (uint64_t)a.M, (uint64_t)a.K, BM)) return rc;
+    if (int rc = make_tile_map(&tmB, a.B, (uint64_t)w_rows, (uint64_t)a.K, (uint32_t)(p.tile_n / 2))) return rc;
+    const int64_t tiles = (int64_t)tiles_m * ((a.N + out_n - 1) / out_n);
+    if (tiles > INT32_MAX) return fail(DSV4_ERR_ARG, "w8a8_linear: too many tiles");
+    if (tiles < pairs) pairs = (int)tiles;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(2 * pairs), 1, 1);
+    cfg.blockDim = dim3(kFusedThreads, 1, 1);
+    cfg.dynamicSmemBytes = L::kDynamic;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = overlap_previous_kernel() ? 1 : 0;
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_fused_pair_kernel<EPI, ACT>, tmA, tmB, p);
+    if (err != cudaSuccess) {
+        cudaGetLastError();  // clear the sticky launch error
+        static thread_local char msg[160];
+        snprintf(msg, sizeof msg, "w8a8_linear (CTA pairs): %s", cudaGetErrorString(err));
+        return fail(DSV4_ERR_LAUNCH, msg);
+    }
+    return check_launch("w8a8_linear");
 }
 
 // Dense problems: the kernel by the number of tokens and tiles.  A gated weight [2 N, K] gives N outputs, and each weight
@@ -396,27 +450,35 @@ int gemm_i8_dense(const GemmArgs& a, const Params& p, int bn, cudaStream_t st) {
         }
     }
     // Dense problems with more than one 128-row tile go to the CTA-pair kernel, gated ones and gradients always
-    if (kGated || kGrad || (a.M > 128 && (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256) >= sms / 4)) {
+    if constexpr (EPI != kEpiPlain) if (kGated || kGrad || (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256) >= sms / 4)
+        switch (a.act) {
+            case kActRelu: return launch_fused_pair<EPI, kActRelu>(a, p, st);
+            case kActGelu: return launch_fused_pair<EPI, kActGelu>(a, p, st);
+            case kActGeluTanh: return launch_fused_pair<EPI, kActGeluTanh>(a, p, st);
+            case kActSilu: return launch_fused_pair<EPI, kActSilu>(a, p, st);
+            default:   // the entry points refuse a gated projection without an activation, and a gradient of none needs no z
+                if constexpr (EPI == kEpiLinear) return launch_fused_pair<EPI, kActNone>(a, p, st);
+                return fail(DSV4_ERR_ARG, "w8a8_linear: unknown activation");
+        }
+    if constexpr (EPI == kEpiPlain) if ((a.M > 128 && (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256) >= sms / 4)) {
         int rc2 = make_tile_map(&tmA, a.A, (uint64_t)a.M, (uint64_t)a.K, BM);
         if (rc2) return rc2;
         rc2 = make_tile_map(&tmB, a.B, (uint64_t)w_rows, (uint64_t)a.K, 128);
         if (rc2) return rc2;
         StoreMaps smaps;
         smaps.count = 0;
-        if constexpr (EPI == kEpiPlain) {
-            if (a.npeers > 0) {
-                // fused all-gather: tile stores through tensor maps of this rank's slab and of every peer's
-                rc2 = make_store_map(&smaps.m[0], a.C, (uint64_t)a.M, (uint64_t)a.N, (uint64_t)p.ldc);
+        if (a.npeers > 0) {
+            // fused all-gather: tile stores through tensor maps of this rank's slab and of every peer's
+            rc2 = make_store_map(&smaps.m[0], a.C, (uint64_t)a.M, (uint64_t)a.N, (uint64_t)p.ldc);
+            if (rc2) return rc2;
+            for (int d = 0; d < a.npeers; ++d) {
+                rc2 = make_store_map(&smaps.m[1 + d], a.peerC[d], (uint64_t)a.M, (uint64_t)a.N, (uint64_t)p.ldc);
                 if (rc2) return rc2;
-                for (int d = 0; d < a.npeers; ++d) {
-                    rc2 = make_store_map(&smaps.m[1 + d], a.peerC[d], (uint64_t)a.M, (uint64_t)a.N, (uint64_t)p.ldc);
-                    if (rc2) return rc2;
-                }
-                smaps.count = 1 + a.npeers;
-                return launch_pair_variant<4, true>(tmA, tmB, p, smaps, st);
             }
+            smaps.count = 1 + a.npeers;
+            return launch_pair_variant<4, true>(tmA, tmB, p, smaps, st);
         }
-        return launch_pair_variant<6, false, EPI>(tmA, tmB, p, smaps, st);
+        return launch_pair_variant<6, false>(tmA, tmB, p, smaps, st);
     }
     if constexpr (!kGated && !kGrad) {
         int rc = make_tile_map(&tmA, a.A, (uint64_t)a.M, (uint64_t)a.K, BM);
@@ -482,6 +544,7 @@ int gemm_i8(const GemmArgs& a, cudaStream_t st) {
     p.bias = static_cast<const __nv_bfloat16*>(a.bias);
     p.resid = static_cast<const __nv_bfloat16*>(a.resid);
     p.ldr = a.ldr; p.act = a.act; p.inter = a.N; p.row_top = a.row_top;
+    p.up_col = a.up_col; p.tile_n = 256;
     if (a.epilogue != kEpiPlain && (grouped || a.out_i32 || a.npeers != 0))
         return fail(DSV4_ERR_ARG, "w8a8_linear: the fused epilogues exist for the dense GEMM with bf16 output");
     {
@@ -550,32 +613,34 @@ int gemm_i8(const GemmArgs& a, cudaStream_t st) {
     }
 }
 
-// dx = dz_scaled W for digits that split_gradient wrote (see gemm_i8_grad_kernel.cuh)
-int gemm_i8_gradient(const void* digits, const unsigned* row_top, const void* W, void* dx, int M, int N, int K, int pitch,
-                     cudaStream_t st) {
-    using L = PairSmem<6, false>;
+// dx = dz_scaled W for digits that split_gradient_kernel wrote (see gemm_i8_grad_kernel.cuh)
+int gemm_i8_gradient(const GradientArgs& a, cudaStream_t st) {
+    using L = FusedPairSmem;
     static bool opted_in[64] = {};
-    if (!opt_in_shared_memory(gemm_i8_grad_kernel<6>, L::kDynamic, opted_in))
+    if (!opt_in_shared_memory(gemm_i8_grad_kernel, L::kDynamic, opted_in))
         return fail(DSV4_ERR_LAUNCH, "w8a8 backward: cannot raise the dynamic shared memory limit");
     GradParams p;
-    p.row_top = row_top;
-    p.dx = static_cast<__nv_bfloat16*>(dx);
-    p.M = M; p.N = N; p.K = K;
+    p.row_top = a.row_top;
+    p.dx = static_cast<__nv_bfloat16*>(a.dx);
+    p.M = a.M; p.K = a.K;
+    p.parts = a.parts; p.part_rows = a.part_rows; p.part_blocks = a.part_pitch / BK;
     p.wait_limit_ns = ptx::kWaitLimitNs;
+    const int pitch = a.parts * a.part_pitch;
     // groups of m-tiles whose two digits take at most 32 MB, as in gemm_i8
-    const int tiles_m = (M + 255) / 256;
+    const int tiles_m = (a.M + 255) / 256;
     int gm_max = (int)((int64_t)32 * 1024 * 1024 / ((int64_t)512 * pitch));
     if (gm_max < 1) gm_max = 1;
     const int groups = (tiles_m + gm_max - 1) / gm_max;
     p.group_m = (tiles_m + groups - 1) / groups;
     CUtensorMap tmD, tmW;
-    if (int rc = make_tile_map(&tmD, digits, (uint64_t)2 * M, (uint64_t)pitch, BM)) return rc;
-    if (int rc = make_tile_map(&tmW, W, (uint64_t)N, (uint64_t)K, 128)) return rc;
-    const int64_t tiles = (int64_t)tiles_m * ((K + 255) / 256);
+    if (int rc = make_tile_map(&tmD, a.digits, (uint64_t)2 * a.M, (uint64_t)pitch, BM)) return rc;
+    if (int rc = make_tile_map(&tmW, a.W, (uint64_t)a.parts * a.part_rows, (uint64_t)a.K, 128)) return rc;
+    const int64_t tiles = (int64_t)tiles_m * ((a.K + 255) / 256);
     int pairs = sm_count() / 2;
     if (pairs <= 0) return fail(DSV4_ERR_LAUNCH, "w8a8 backward: no CUDA device");
+    if (tiles > INT32_MAX) return fail(DSV4_ERR_ARG, "w8a8 backward: too many tiles");
     if (tiles < pairs) pairs = (int)tiles;
-    gemm_i8_grad_kernel<6><<<2 * pairs, kThreads, L::kDynamic, st>>>(tmD, tmW, p);
+    gemm_i8_grad_kernel<<<2 * pairs, kFusedThreads, L::kDynamic, st>>>(tmD, tmW, p);
     return check_launch("w8a8 backward");
 }
 

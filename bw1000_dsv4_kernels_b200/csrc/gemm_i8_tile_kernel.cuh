@@ -140,7 +140,7 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             // column scales of this tile -> this warp's shared copy
             __syncwarp();
             if constexpr (EPI == kEpiLinear) {
-                stage_columns(p, sbs, bias_s, lane, BN / 2, c.n0, c.n0 + BN / 2, p.N, p.N);
+                stage_columns(p, sbs, bias_s, lane, BN, c.n0);
             } else if (!p.out_i32) {
                 for (int j = lane; j < BN; j += 32)
                     sbs[j] = (c.n0 + j < p.N) ? __ldg(p.sb + c.n0 + j) : 0.0f;

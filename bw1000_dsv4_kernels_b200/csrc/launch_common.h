@@ -49,14 +49,21 @@ struct GemmArgs {
     int64_t ldr = 0;
     int act = 0;                   // enum Activation in activations.cuh
     unsigned* row_top = nullptr;   // gradient epilogues (3 linear, 4 gated; resid is the incoming gradient, C is fp32)
+    int up_col = 0;                // gated gradient: first column of the ups in C
     // Test hook, zero through every public entry point: the tile producers of the launch issue no
     // loads and every bounded wait gives up after test_wait_limit_ns, so the kernel's give-up path runs.
     int test_withhold_loads = 0;
     unsigned long long test_wait_limit_ns = 0;
 };
 int gemm_i8(const GemmArgs& a, cudaStream_t st);
-int gemm_i8_gradient(const void* digits, const unsigned* row_top, const void* W, void* dx, int M, int N, int K, int pitch,
-                     cudaStream_t st);
+struct GradientArgs {
+    const void* digits;         // int8 [2][M][parts * part_pitch]: hi, then lo
+    const unsigned* row_top;    // [M] float bits
+    const void* W;              // int8 [parts * part_rows, K]
+    void* dx;                   // bf16 [M, K]
+    int M, K, parts, part_rows, part_pitch;   // part_pitch: multiple of 128, zeros behind part_rows
+};
+int gemm_i8_gradient(const GradientArgs& a, cudaStream_t st);
 int scale_convert(const void* acc, const void* sa, const void* sb, void* out, int M, int N,
                   cudaStream_t st);
 
@@ -100,7 +107,7 @@ struct BackwardArgs {
     float* dbias;          // fp32 [N] or null
     int M, N, K;
 };
-int64_t w8a8_backward_workspace(int M, int N, bool recompute, bool dbias);
+int64_t w8a8_backward_workspace(int M, int N, bool gated, bool recompute, bool dbias);
 int w8a8_backward(const BackwardArgs& a, void* workspace, cudaStream_t st);
 
 int read_device_status(cudaStream_t st, int* out);

@@ -22,6 +22,7 @@
 //   * flash_mla_decode is not part of the W8A8 path and is not provided.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 
 #include <string>
@@ -60,6 +61,12 @@ int to_int(int64_t v, const char* what) {
     return static_cast<int>(v);
 }
 
+// An uninitialised dense tensor on `like`'s device.  The allocator is called directly: an operator of a few microseconds
+// notices the dispatcher's share of torch::empty (about a third of a microsecond for each output).
+Tensor fresh(const Tensor& like, at::IntArrayRef sizes, c10::ScalarType dtype) {
+    return Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt));
+}
+
 struct Rows {
     int M, N;
 };
@@ -76,10 +83,10 @@ std::vector<Tensor> per_token_quant_int8_stream(Tensor x, int64_t stream_ptr) {
     check_cuda(x, "x", torch::kBFloat16);
     c10::cuda::CUDAGuard guard(x.device());
     const Rows r = rows_of(x);
-    auto q = torch::empty_like(x, x.options().dtype(torch::kInt8));
-    auto s = torch::empty({r.M}, x.options().dtype(torch::kFloat32));
+    auto q = fresh(x, x.sizes(), torch::kInt8);
+    auto s = fresh(x, {r.M, 1}, torch::kFloat32);
     check_status(launch_ptq(x.data_ptr(), q.data_ptr(), s.data_ptr(), r.M, r.N, as_stream(stream_ptr)));
-    return {q, s.unsqueeze(-1)};
+    return {q, s};
 }
 
 // ---- per_token_group_quant_int8 (launcher dsv4_all_hip_kernels.hip:346-350) -------
@@ -255,7 +262,7 @@ Tensor w8a8_scaled_gemm_stream(Tensor A, Tensor B, Tensor sa, Tensor sb, int64_t
     const Tensor& sa_c = flat_scale(sa, g.M, "sa", A);
     const Tensor& sb_c = flat_scale(sb, g.N, "sb", A);
     c10::cuda::CUDAGuard guard(A.device());
-    auto C = torch::empty({g.M, g.N}, A.options().dtype(torch::kBFloat16));
+    auto C = fresh(A, {g.M, g.N}, torch::kBFloat16);
     check_status(launch_w8a8_gemm(A.data_ptr(), B.data_ptr(), sa_c.data_ptr(), sb_c.data_ptr(), C.data_ptr(), g.M,
                                   g.N, g.K, as_stream(stream_ptr)));
     return C;
@@ -602,8 +609,9 @@ int64_t device_status() {
 // A workspace that lives only for the launches of one call: allocated on the stream that the launches go to, so that
 // the caching allocator hands it out again only behind them on that stream, whatever torch's current stream is.
 Tensor workspace_on(dsv4_stream_t stream, int64_t bytes, const Tensor& like) {
+    if (at::cuda::getCurrentCUDAStream().stream() == reinterpret_cast<cudaStream_t>(stream)) return fresh(like, {bytes}, torch::kUInt8);
     c10::cuda::CUDAStreamGuard on(c10::cuda::getStreamFromExternal(reinterpret_cast<cudaStream_t>(stream), like.device().index()));
-    return torch::empty({bytes}, like.options().dtype(torch::kUInt8));
+    return fresh(like, {bytes}, torch::kUInt8);
 }
 
 // ---- fused linear and gated projection ------------------------------------------------
@@ -639,7 +647,7 @@ Tensor w8a8_linear_stream(Tensor A, Tensor B, Tensor sa, Tensor sb, c10::optiona
     const int act_id = activation_of(act);
     const int64_t ldr = residual.has_value() ? row_stride(*residual, "residual", g.M, g.N, A) : 0;
     c10::cuda::CUDAGuard guard(A.device());
-    auto C = torch::empty({g.M, g.N}, A.options().dtype(torch::kBFloat16));
+    auto C = fresh(A, {g.M, g.N}, torch::kBFloat16);
     check_status(launch_w8a8_linear(A.data_ptr(), B.data_ptr(), sa_c.data_ptr(), sb_c.data_ptr(), bp, act_id,
                                     residual.has_value() ? residual->data_ptr() : nullptr, ldr, C.data_ptr(), g.N, g.M, g.N,
                                     g.K, as_stream(stream_ptr)));
@@ -662,7 +670,7 @@ Tensor w8a8_gated_stream(Tensor A, Tensor W13, Tensor sa, Tensor s13, c10::optio
     const void* bp = bias_ptr(bias, g.N, A);
     const int act_id = gated_act(act);
     c10::cuda::CUDAGuard guard(A.device());
-    auto C = torch::empty({g.M, g.N / 2}, A.options().dtype(torch::kBFloat16));
+    auto C = fresh(A, {g.M, g.N / 2}, torch::kBFloat16);
     check_status(launch_w8a8_gated(A.data_ptr(), W13.data_ptr(), sa_c.data_ptr(), sb_c.data_ptr(), bp, act_id, C.data_ptr(),
                                    g.N / 2, g.M, g.N / 2, g.K, as_stream(stream_ptr)));
     return C;
@@ -679,11 +687,11 @@ std::vector<c10::optional<Tensor>> w8a8_backward_impl(bool gated, Tensor dy, Ten
     const int act_id = gated ? gated_act(act) : activation_of(act);
     const int64_t ldy = row_stride(dy, gated ? "dh" : "dy", g.M, gated ? g.N / 2 : g.N, A);
     c10::cuda::CUDAGuard guard(A.device());
-    auto dx = torch::empty({g.M, g.K}, A.options().dtype(torch::kBFloat16));
+    auto dx = fresh(A, {g.M, g.K}, torch::kBFloat16);
     c10::optional<Tensor> db;
-    if (bias.has_value()) db = torch::empty({g.N}, A.options().dtype(torch::kFloat32));
+    if (bias.has_value()) db = fresh(A, {g.N}, torch::kFloat32);
     const dsv4_stream_t st = as_stream(stream_ptr);
-    const int64_t bytes = dsv4_w8a8_backward_workspace(g.M, g.N, act_id, bias.has_value());
+    const int64_t bytes = dsv4_w8a8_backward_workspace(g.M, g.N, gated, act_id, bias.has_value());
     Tensor ws = workspace_on(st, bytes, A);
     auto launch = gated ? launch_w8a8_gated_backward : launch_w8a8_linear_backward;
     check_status(launch(dy.data_ptr(), ldy, A.data_ptr(), B.data_ptr(), sa_c.data_ptr(), sb_c.data_ptr(), bp, act_id,
@@ -727,8 +735,8 @@ NormShape check_norm(const Tensor& x, const Tensor& w, const Tensor& b, const c1
 std::vector<Tensor> layernorm_impl(c10::optional<Tensor> res, Tensor x, Tensor w, Tensor b, double eps, int64_t stream_ptr) {
     const NormShape n = check_norm(x, w, b, res);
     c10::cuda::CUDAGuard guard(x.device());
-    auto y = torch::empty_like(x);
-    auto mean = torch::empty({n.M}, x.options().dtype(torch::kFloat32)), rstd = torch::empty_like(mean);
+    auto y = fresh(x, x.sizes(), torch::kBFloat16);
+    auto mean = fresh(x, {n.M}, torch::kFloat32), rstd = fresh(x, {n.M}, torch::kFloat32);
     check_status(launch_layernorm(res.has_value() ? res->data_ptr() : nullptr, x.data_ptr(), w.data_ptr(), b.data_ptr(),
                                   y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), n.M, n.N, (float)eps, as_stream(stream_ptr)));
     return {y, mean, rstd};
@@ -744,13 +752,13 @@ std::vector<Tensor> add_layernorm_stream(Tensor res, Tensor x, Tensor w, Tensor 
 std::vector<Tensor> layernorm_quant_impl(c10::optional<Tensor> res, Tensor x, Tensor w, Tensor b, double eps, int64_t stream_ptr) {
     const NormShape n = check_norm(x, w, b, res);
     c10::cuda::CUDAGuard guard(x.device());
-    auto q = torch::empty_like(x, x.options().dtype(torch::kInt8));
-    auto s = torch::empty({n.M}, x.options().dtype(torch::kFloat32));
-    auto mean = torch::empty_like(s), rstd = torch::empty_like(s);
+    auto q = fresh(x, x.sizes(), torch::kInt8);
+    auto s = fresh(x, {n.M, 1}, torch::kFloat32);
+    auto mean = fresh(x, {n.M}, torch::kFloat32), rstd = fresh(x, {n.M}, torch::kFloat32);
     check_status(launch_layernorm_quant(res.has_value() ? res->data_ptr() : nullptr, x.data_ptr(), w.data_ptr(), b.data_ptr(),
                                         q.data_ptr(), s.data_ptr(), mean.data_ptr(), rstd.data_ptr(), n.M, n.N, (float)eps,
                                         as_stream(stream_ptr)));
-    return {q, s.unsqueeze(-1), mean, rstd};
+    return {q, s, mean, rstd};
 }
 std::vector<Tensor> layernorm_quant_stream(Tensor x, Tensor w, Tensor b, double eps, int64_t stream_ptr) {
     return layernorm_quant_impl(c10::nullopt, x, w, b, eps, stream_ptr);
@@ -769,8 +777,8 @@ std::vector<Tensor> layernorm_backward_stream(Tensor dy, Tensor x, Tensor mean, 
     const Tensor& mean_c = flat_scale(mean, n.M, "mean", x);
     const Tensor& rstd_c = flat_scale(rstd, n.M, "rstd", x);
     c10::cuda::CUDAGuard guard(x.device());
-    auto dx = torch::empty_like(x);
-    auto dw = torch::empty({n.N}, x.options().dtype(torch::kFloat32)), db = torch::empty_like(dw);
+    auto dx = fresh(x, x.sizes(), torch::kBFloat16);
+    auto dw = fresh(x, {n.N}, torch::kFloat32), db = fresh(x, {n.N}, torch::kFloat32);
     const dsv4_stream_t st = as_stream(stream_ptr);
     const int64_t bytes = dsv4_layernorm_backward_workspace(n.M, n.N);
     Tensor ws = workspace_on(st, bytes, x);

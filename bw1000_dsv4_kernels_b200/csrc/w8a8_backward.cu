@@ -67,49 +67,72 @@ __global__ void __launch_bounds__(256) row_top_kernel(const __nv_bfloat16* dy, i
     }
 }
 
-// dz [M, N] -> digits int8 [2][M][pitch] (hi, then lo; zero beyond N), and per block of rows the column sums of dz.
-// A thread owns eight columns and walks the block's rows.
-constexpr int kSplitThreads = 128;
-constexpr int kSplitCols = kSplitThreads * 8;
+// The columns of dz and of the digits: `parts` ranges (gates and ups, or one) of part_rows columns each, at multiples of
+// part_pitch (a multiple of 128, so that a K block of the gradient product never straddles two ranges).
+struct Columns {
+    int parts, part_rows, part_pitch;
+    __host__ __device__ int pitch() const { return parts * part_pitch; }
+};
+
+// dz -> digits int8 [2][M][pitch] (hi, then lo; zeros behind each range), and with SUM the column sums of every block of
+// kSplitRows rows.  A warp takes 256 columns of every eighth row of the block, all its rows' loads at once.
+constexpr int kSplitRows = 32;
+constexpr int kSplitWarps = 8;
 template <typename T, bool SUM>
-__global__ void __launch_bounds__(kSplitThreads) split_gradient_kernel(const T* dz, int64_t ld, const float* __restrict__ sb,
-                                                                       const unsigned* __restrict__ row_top, int M, int N,
-                                                                       int pitch, int rows_per_block, bool vec, int8_t* digits,
-                                                                       float* partial) {
-    const int c = blockIdx.x * kSplitCols + threadIdx.x * 8;
-    if (c >= pitch) return;
-    const int left = N - c;
-    float scale[8], sum[8] = {};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) scale[j] = j < left ? __ldg(sb + c + j) : 0.0f;
-    const int r0 = blockIdx.y * rows_per_block, r1 = min(M, r0 + rows_per_block);
+__global__ void __launch_bounds__(32 * kSplitWarps) split_gradient_kernel(const T* dz, int64_t ld, const float* __restrict__ sb,
+                                                                          const unsigned* __restrict__ row_top, int M,
+                                                                          Columns cols, bool vec, int8_t* digits,
+                                                                          float* partial) {
+    __shared__ float sums[SUM ? kSplitWarps : 1][SUM ? 264 : 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int c = blockIdx.x * 256 + lane * 8;             // column with padding
+    const int pitch = cols.pitch(), part = c >= cols.part_pitch ? 1 : 0, local = c - part * cols.part_pitch;
+    const int left = c < pitch ? cols.part_rows - local : 0, w_row = part * cols.part_rows + local;
     const int64_t plane = (int64_t)M * pitch;
-#pragma unroll 4
-    for (int r = r0; r < r1; ++r) {
-        float v[8];
-        load8(dz + (int64_t)r * ld + c, left, vec, v);
-        const float inv = digit_inverse(__uint_as_float(__ldg(row_top + r)));
+    const int r0 = blockIdx.y * kSplitRows + warp;
+    constexpr int kRows = kSplitRows / kSplitWarps;
+    float v[kRows][8], inv[kRows], scale[8], sum[8] = {};
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const int r = r0 + i * kSplitWarps;
+        const bool ok = r < M;
+        load8(dz + (int64_t)(ok ? r : 0) * ld + c, ok ? left : 0, vec, v[i]);
+        inv[i] = ok ? digit_inverse(__uint_as_float(__ldg(row_top + r))) : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) scale[j] = j < left ? __ldg(sb + w_row + j) : 0.0f;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const int r = r0 + i * kSplitWarps;
         uint32_t hi[2], lo[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             int d[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                if constexpr (SUM) sum[4 * h + j] += v[4 * h + j];
-                d[j] = digits_of(v[4 * h + j] * scale[4 * h + j], inv);
+                if constexpr (SUM) sum[4 * h + j] += v[i][4 * h + j];
+                d[j] = digits_of(v[i][4 * h + j] * scale[4 * h + j], inv[i]);
             }
             hi[h] = pack_i8x4(digit_hi(d[0]), digit_hi(d[1]), digit_hi(d[2]), digit_hi(d[3]));
             lo[h] = pack_i8x4(digit_lo(d[0]), digit_lo(d[1]), digit_lo(d[2]), digit_lo(d[3]));
         }
-        int8_t* out = digits + (int64_t)r * pitch + c;
-        *reinterpret_cast<uint2*>(out) = make_uint2(hi[0], hi[1]);
-        *reinterpret_cast<uint2*>(out + plane) = make_uint2(lo[0], lo[1]);
+        if (r < M && c < pitch) {
+            int8_t* out = digits + (int64_t)r * pitch + c;
+            *reinterpret_cast<uint2*>(out) = make_uint2(hi[0], hi[1]);
+            *reinterpret_cast<uint2*>(out + plane) = make_uint2(lo[0], lo[1]);
+        }
     }
     if constexpr (SUM) {
-        float* o = partial + (int64_t)blockIdx.y * N + c;
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (j < left) o[j] = sum[j];
+        for (int j = 0; j < 8; ++j) sums[warp][lane * 8 + j] = sum[j];
+        __syncthreads();
+        const int col = blockIdx.x * 256 + threadIdx.x, p2 = col >= cols.part_pitch ? 1 : 0, l2 = col - p2 * cols.part_pitch;
+        if (col < pitch && l2 < cols.part_rows) {
+            float t = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kSplitWarps; ++w) t += sums[w][threadIdx.x];
+            partial[(int64_t)blockIdx.y * cols.parts * cols.part_rows + p2 * cols.part_rows + l2] = t;
+        }
     }
 }
 
@@ -134,20 +157,23 @@ __global__ void __launch_bounds__(256) gradient_column_sum_kernel(const float* _
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 struct Layout {
-    int pitch, rows_per_block, row_blocks;
+    Columns cols;
+    int row_blocks;
     int64_t digits, dz, row_top, partial, total;   // offsets and size in bytes
 };
-Layout layout(int M, int N, bool recompute, bool dbias) {
+Layout layout(int M, int N, bool gated, bool recompute, bool dbias) {
     auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
     Layout l;
-    l.pitch = (int)(((int64_t)N + 15) / 16 * 16);
-    l.rows_per_block = M >= 2048 ? 32 : 16;
-    l.row_blocks = (M + l.rows_per_block - 1) / l.rows_per_block;
+    l.cols.parts = gated ? 2 : 1;
+    l.cols.part_rows = N / l.cols.parts;
+    l.cols.part_pitch = (l.cols.part_rows + 127) / 128 * 128;
+    l.row_blocks = (M + kSplitRows - 1) / kSplitRows;
+    const int64_t pitch = l.cols.pitch();
     l.digits = 0;
-    l.dz = l.digits + up((int64_t)2 * M * l.pitch);
-    l.row_top = l.dz + (recompute ? up((int64_t)4 * M * N) : 0);
-    l.partial = l.row_top + up((int64_t)4 * M);
-    l.total = l.partial + (dbias ? up((int64_t)4 * l.row_blocks * N) : 0);
+    l.dz = l.digits + up(2 * (int64_t)M * pitch);
+    l.row_top = l.dz + (recompute ? up(4 * (int64_t)M * pitch) : 0);
+    l.partial = l.row_top + up(4 * (int64_t)M);
+    l.total = l.partial + (dbias ? up(4 * (int64_t)l.row_blocks * N) : 0);
     return l;
 }
 
@@ -155,26 +181,26 @@ template <typename T>
 int split(const T* dz, int64_t ld, const BackwardArgs& a, const Layout& l, const unsigned* row_top, int8_t* digits,
           float* partial, cudaStream_t st) {
     const bool vec = (ld * sizeof(T)) % 16 == 0 && aligned16(dz);
-    const dim3 grid((l.pitch + kSplitCols - 1) / kSplitCols, l.row_blocks);
+    const dim3 grid((l.cols.pitch() + 255) / 256, l.row_blocks);
     if (a.dbias != nullptr) {
-        split_gradient_kernel<T, true><<<grid, kSplitThreads, 0, st>>>(dz, ld, a.sb, row_top, a.M, a.N, l.pitch,
-                                                                       l.rows_per_block, vec, digits, partial);
+        split_gradient_kernel<T, true><<<grid, 32 * kSplitWarps, 0, st>>>(dz, ld, a.sb, row_top, a.M, l.cols, vec, digits, partial);
         if (int rc = check_launch("w8a8 backward")) return rc;
         gradient_column_sum_kernel<<<(a.N + 31) / 32, 256, 0, st>>>(partial, l.row_blocks, a.N, a.dbias);
     } else {
-        split_gradient_kernel<T, false><<<grid, kSplitThreads, 0, st>>>(dz, ld, a.sb, row_top, a.M, a.N, l.pitch,
-                                                                        l.rows_per_block, vec, digits, partial);
+        split_gradient_kernel<T, false><<<grid, 32 * kSplitWarps, 0, st>>>(dz, ld, a.sb, row_top, a.M, l.cols, vec, digits, partial);
     }
     return check_launch("w8a8 backward");
 }
 
 }  // namespace
 
-int64_t w8a8_backward_workspace(int M, int N, bool recompute, bool dbias) { return layout(M, N, recompute, dbias).total; }
+int64_t w8a8_backward_workspace(int M, int N, bool gated, bool recompute, bool dbias) {
+    return layout(M, N, gated, recompute, dbias).total;
+}
 
 int w8a8_backward(const BackwardArgs& a, void* workspace, cudaStream_t st) {
     const bool recompute = a.act != kActNone;
-    const Layout l = layout(a.M, a.N, recompute, a.dbias != nullptr);
+    const Layout l = layout(a.M, a.N, a.gated, recompute, a.dbias != nullptr);
     char* ws = static_cast<char*>(workspace);
     int8_t* digits = reinterpret_cast<int8_t*>(ws + l.digits);
     unsigned* row_top = reinterpret_cast<unsigned*>(ws + l.row_top);
@@ -182,19 +208,26 @@ int w8a8_backward(const BackwardArgs& a, void* workspace, cudaStream_t st) {
     const __nv_bfloat16* dy = static_cast<const __nv_bfloat16*>(a.dy);
     if (recompute) {
         float* dz = reinterpret_cast<float*>(ws + l.dz);
-        if (cudaMemsetAsync(row_top, 0, (size_t)a.M * 4, st) != cudaSuccess) return check_launch("w8a8 backward");
+        if (cudaMemsetAsync(row_top, 0, (size_t)a.M * 4, st) != cudaSuccess) {
+            check_launch("w8a8 backward");
+            return DSV4_ERR_LAUNCH;
+        }
         GemmArgs g{};
         g.A = a.A; g.B = a.B; g.sa = a.sa; g.sb = a.sb; g.C = dz;
-        g.M = a.M; g.N = a.gated ? a.N / 2 : a.N; g.K = a.K; g.E = 1; g.ldc = a.N; g.sa_groups = 1;
+        g.M = a.M; g.N = l.cols.part_rows; g.K = a.K; g.E = 1; g.ldc = l.cols.pitch(); g.sa_groups = 1;
         g.epilogue = a.gated ? 4 : 3; g.bias = a.bias; g.resid = a.dy; g.ldr = a.ldy; g.act = a.act; g.row_top = row_top;
+        g.up_col = l.cols.part_pitch;
         if (int rc = gemm_i8(g, st)) return rc;
-        if (int rc = split(dz, (int64_t)a.N, a, l, row_top, digits, partial, st)) return rc;
+        if (int rc = split(dz, (int64_t)l.cols.pitch(), a, l, row_top, digits, partial, st)) return rc;
     } else {
         row_top_kernel<<<a.M, 256, 0, st>>>(dy, a.ldy, a.sb, a.N, a.ldy % 8 == 0 && aligned16(dy), row_top);
         if (int rc = check_launch("w8a8 backward")) return rc;
         if (int rc = split(dy, a.ldy, a, l, row_top, digits, partial, st)) return rc;
     }
-    return gemm_i8_gradient(digits, row_top, a.B, a.dx, a.M, a.N, a.K, l.pitch, st);
+    GradientArgs d;
+    d.digits = digits; d.row_top = row_top; d.W = a.B; d.dx = a.dx;
+    d.M = a.M; d.K = a.K; d.parts = l.cols.parts; d.part_rows = l.cols.part_rows; d.part_pitch = l.cols.part_pitch;
+    return gemm_i8_gradient(d, st);
 }
 
 }  // namespace w8a8

@@ -276,9 +276,9 @@ DSV4_API int launch_w8a8_gated(const void* A, const void* B, const void* sa, con
  * Inside, each row of dz * sb is in 16-bit fixed point relative to its largest magnitude (a row that holds an infinity or
  * a NaN therefore gives a row of NaN); dz, the sums and the scales are fp32.  With DSV4_ACT_NONE A and sa are not read
  * and may be null.  At most 131071 weight rows.  Every result depends on the inputs, sizes and device only.
- * workspace: dsv4_w8a8_backward_workspace(M, weight rows, act, dbias != null) bytes of device memory, 16-byte aligned,
- * free again once the launches have run. */
-DSV4_API int64_t dsv4_w8a8_backward_workspace(int M, int weight_rows, int act, int want_dbias);
+ * workspace: dsv4_w8a8_backward_workspace(M, weight rows, gated, act, dbias != null) bytes of device memory, 16-byte
+ * aligned, free again once the launches have run. */
+DSV4_API int64_t dsv4_w8a8_backward_workspace(int M, int weight_rows, int gated, int act, int want_dbias);
 DSV4_API int launch_w8a8_linear_backward(const void* dy, int64_t ldy, const void* A, const void* B, const void* sa,
                        const void* sb, const void* bias, int act, void* dx, void* dbias, void* workspace,
                        int64_t workspace_bytes, int M, int N, int K, dsv4_stream_t stream);

@@ -4,7 +4,8 @@ Tolerances.  dz: the recomputed z is off by 4 * 2^-24 of its size, slopes of at 
 and the fast exponential's 2^-18 make that 2^-17 of the terms' magnitude at most.  dx: every row of t = dz * sb is in
 fixed point with a step of top / 32639, off by half of it, so a sum of N terms is off by at most
 (step / 2) * sum |W[n, k]|, plus dz's own error times |W|, plus the two conversions, plus half a bf16 step of the
-result.  dbias: dz's error, and the fp32 additions of a column (rows of a block, then the blocks' slices)."""
+result.  GELU's normal distribution function comes from a published polynomial that is off by 0.75e-7 (2^-23.6) at most,
+which is CDF * |z| <= 2^-23 |z| in the activation.  dbias: dz's error, and the fp32 additions of a column (rows of a block, then the blocks' slices)."""
 import pytest
 import torch
 
@@ -79,7 +80,7 @@ def test_gated_backward(ext, m, i, k, act, bias):
     g, u, size_g, size_u = z[:, :i], z[:, i:], size[:, :i], size[:, i:]
     d = dh.double().abs()
     err_g = d * u.abs() * (DZ + 1.2 * 4 * U * size_g) + d * 1.13 * 4 * U * size_u
-    err_u = d * (DZ * (ref.act(g, act).abs() + 1e-6) + 1.13 * 4 * U * size_g)
+    err_u = d * (DZ * (ref.act(g, act).abs() + 1e-6) + 1.13 * 4 * U * size_g + 2.0 ** -23 * g.abs())
     if act == "relu":
         near = g.abs() <= 4 * U * size_g
         err_g = torch.where(near, d * u.abs() * 1.01, d * 1.13 * 4 * U * size_u + U * d * u.abs())

@@ -77,8 +77,8 @@ def test_c_abi_refuses_before_it_touches_a_device():
     assert gated(M=0) == 0
     for bad, word in ((dict(act=0), b"activation"), (dict(I=2 ** 30), b"int32"), (dict(K=8), b"multiple of 16")):
         assert gated(**bad) == 1 and word in err()
-    size = lib.dsv4_w8a8_backward_workspace(4, 8, 2, 1)
-    assert size > 2 * 4 * 16 + 4 * 4 * 8 and lib.dsv4_w8a8_backward_workspace(0, 8, 2, 1) == 0
+    size = lib.dsv4_w8a8_backward_workspace(4, 8, 0, 2, 1)
+    assert size > 2 * 4 * 16 + 4 * 4 * 8 and lib.dsv4_w8a8_backward_workspace(0, 8, 0, 2, 1) == 0
     back = lambda **k: lib.launch_w8a8_linear_backward(*[k.get(n, d) for n, d in (   # noqa: E731
         ("dy", one), ("ldy", ll(8)), ("A", one), ("B", one), ("sa", one), ("sb", one), ("bias", null), ("act", 2), ("dx", one),
         ("db", one), ("ws", one), ("bytes", ll(size)), ("M", 4), ("N", 8), ("K", 32), ("st", null))])
