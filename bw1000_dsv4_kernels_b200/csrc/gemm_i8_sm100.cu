@@ -352,20 +352,15 @@ int launch_pair_variant(const CUtensorMap& tmA, const CUtensorMap& tmB, const Pa
     return check_launch("w8a8_gemm");
 }
 
-// Width of the fused pair kernel's tiles (rows of B, multiples of `unit` up to 256) for tiles_m rows of tiles, `rows` rows of
-// B and `pairs` CTA pairs: the width with the least rounds x time of a round.
+// Width of the fused pair kernel's tiles (rows of B, a multiple of `unit`).  256 wherever that gives every pair a tile: a
+// narrower tile moves more operand bytes per MMA, and under the power cap a partly empty last round costs less than its
+// share (224 tiles at 256 on 74 pairs 203 us, 199 at 224, 208 at 160, 270 at 128).  Problems of fewer tiles take the
+// widest tile that still spreads them over the pairs (40 x 256 columns of a gated 333 x 1024 x 1040: 12.2 us at 256, 9.4
+// at 64).
 int fused_tile_n(int tiles_m, int rows, int unit, int pairs) {
-    int best = 256;
-    int64_t best_cost = INT64_MAX;
-    for (int w = 256; w >= unit; w -= unit) {
-        const int64_t tiles = (int64_t)tiles_m * ((rows + w - 1) / w);
-        const int64_t cost = (tiles + pairs - 1) / pairs * (256 + w);
-        if (cost < best_cost) {
-            best_cost = cost;
-            best = w;
-        }
-    }
-    return best;
+    int w = 256;
+    while (w > 64 && (int64_t)tiles_m * ((rows + w - unit - 1) / (w - unit)) <= pairs) w -= unit;
+    return w;
 }
 
 template <int EPI, int ACT>

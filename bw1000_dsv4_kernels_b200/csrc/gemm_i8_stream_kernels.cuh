@@ -316,8 +316,8 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
         if constexpr (EPI == kEpiPlain)
             reduce_partials_and_store<8, 4>(p, peer_base, S, cols_lo, cols_hi, n0, threadIdx.x, kThreads, sa_s, sb_s);
         else
-            reduce_partials_fused<8, EPI == kEpiGated ? 2 : 4, EPI == kEpiGated>(p, peer_base, S, cols_lo, cols_hi, n0,
-                                                                                 threadIdx.x, kThreads, sa_s, sb_s, sb_s + 128);
+            reduce_partials_fused_sized<8, EPI == kEpiGated ? 2 : 4, EPI == kEpiGated>(p, peer_base, S, cols_lo, cols_hi, n0,
+                                                                                       threadIdx.x, kThreads, sa_s);
     }
 
     // nobody leaves while a peer may still read its shared memory
@@ -525,8 +525,8 @@ gemm_i8_stream_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
         if constexpr (EPI == kEpiPlain)
             reduce_partials_and_store<4, 8>(p, peer_base, S, cols_lo, cols_hi, n0, threadIdx.x, kThreads, sa_s, sb_s);
         else
-            reduce_partials_fused<4, EPI == kEpiGated ? 4 : 8, EPI == kEpiGated>(p, peer_base, S, cols_lo, cols_hi, n0,
-                                                                                 threadIdx.x, kThreads, sa_s, sb_s, sb_s + 128);
+            reduce_partials_fused_sized<4, EPI == kEpiGated ? 4 : 8, EPI == kEpiGated>(p, peer_base, S, cols_lo, cols_hi, n0,
+                                                                                       threadIdx.x, kThreads, sa_s);
     }
 
     // nobody leaves while a peer may still read its shared memory
