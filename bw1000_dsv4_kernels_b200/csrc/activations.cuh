@@ -1,8 +1,10 @@
-// Activations of the fused linear and gated epilogues and their derivatives, fp32.  They take CUDA's fast exponential and
-// reciprocal, whose relative error (about 2^-21 at the arguments where the result still matters) is far below the bf16
-// step of every output that they reach.
+// Activations of the fused linear and gated epilogues and their derivatives, fp32, two elements at a time: products and
+// sums as packed f32x2 instructions, exponential and reciprocal as the hardware's approximations, whose relative error
+// (about 2^-21 at the arguments where the result still matters) is far below the bf16 step of every output they reach.
+// A tile's epilogue evaluates 32768 of them per SM beside the tensor cores, so their instructions count.
 #pragma once
 #include <cuda_runtime.h>
+#include "w8a8_arith.cuh"
 
 namespace w8a8 {
 
@@ -14,52 +16,86 @@ constexpr float kInvSqrt2Pi = 0.39894228f;
 constexpr float kGeluTanhC = 1.59576912f;   // 2 * sqrt(2 / pi): 0.5 * (1 + tanh(a)) = sigmoid(2 a)
 constexpr float kGeluCubic = 0.044715f;
 
-__device__ __forceinline__ float sigmoid_fast(float z) { return __fdividef(1.0f, 1.0f + __expf(-z)); }
-
-// Phi(z), the normal distribution function, and exp(-z^2 / 2), which Phi's formula needs anyway and the density is made of.
-// 0.5 * erfc(|z| / sqrt 2) by Abramowitz and Stegun, Handbook of Mathematical Functions, formula 7.1.26: a polynomial of
-// degree five in 1 / (1 + 0.3275911 x) times exp(-x^2), off by at most 0.75e-7.  erfcf is exact to the last bits but takes
-// four times the instructions and branches on its argument, which made the drain of a 7168-deep tile longer than its
-// tensor-core work.
-__device__ __forceinline__ float2 normal_cdf_exp(float z) {
-    const float x = fabsf(z) * kSqrtHalf;
-    const float t = __fdividef(1.0f, fmaf(0.3275911f, x, 1.0f));
-    const float e = __expf(-x * x);
-    float q = fmaf(t, 1.061405429f, -1.453152027f);
-    q = fmaf(t, q, 1.421413741f);
-    q = fmaf(t, q, -0.284496736f);
-    q = fmaf(t, q, 0.254829592f);
-    q = q * t * e * 0.5f;
-    return make_float2(z > 0.0f ? 1.0f - q : q, e);
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
+// 1 / (1 + exp(-a z)) for a constant a
+__device__ __forceinline__ float2 sigmoid2(float2 z, float a) {
+    const float2 t = __fmul2_rn(z, splat2(-a * kLog2e));
+    const float2 d = __fadd2_rn(make_float2(exp2_fast(t.x), exp2_fast(t.y)), splat2(1.0f));
+    return make_float2(rcp_fast(d.x), rcp_fast(d.y));
+}
+
+// Phi(z), the normal distribution function, and e = exp(-z^2 / 2), which Phi's formula needs anyway and the density is
+// made of.  1 - Phi(|z|) = 0.5 * erfc(|z| / sqrt 2) by Abramowitz and Stegun, Handbook of Mathematical Functions, formula
+// 7.1.26: a polynomial of degree five in 1 / (1 + 0.3275911 x) times exp(-x^2), off by at most 0.75e-7.  erfcf is exact
+// to the last bits but takes four times the instructions and branches on its argument, which made the drain of a
+// 7168-deep tile longer than its tensor-core work.
+__device__ __forceinline__ float2 normal_cdf2(float2 z, float2& e) {
+    const float2 a = make_float2(fabsf(z.x), fabsf(z.y));
+    const float2 d = __ffma2_rn(a, splat2(0.3275911f * kSqrtHalf), splat2(1.0f));
+    const float2 t = make_float2(rcp_fast(d.x), rcp_fast(d.y));
+    const float2 s = __fmul2_rn(__fmul2_rn(z, z), splat2(-0.5f * kLog2e));
+    e = make_float2(exp2_fast(s.x), exp2_fast(s.y));
+    float2 q = __ffma2_rn(t, splat2(0.5f * 1.061405429f), splat2(0.5f * -1.453152027f));
+    q = __ffma2_rn(t, q, splat2(0.5f * 1.421413741f));
+    q = __ffma2_rn(t, q, splat2(0.5f * -0.284496736f));
+    q = __ffma2_rn(t, q, splat2(0.5f * 0.254829592f));
+    q = __fmul2_rn(__fmul2_rn(q, t), e);
+    return make_float2(z.x > 0.0f ? 1.0f - q.x : q.x, z.y > 0.0f ? 1.0f - q.y : q.y);
+}
+
+__device__ __forceinline__ float relu(float z) { return z > 0.0f ? z : (z != z ? z : 0.0f); }   // a NaN stays one
+
 template <int ACT>
-__device__ __forceinline__ float act_value(float z) {
-    if constexpr (ACT == kActRelu) return z > 0.0f ? z : (z != z ? z : 0.0f);
-    if constexpr (ACT == kActGelu) return z * normal_cdf_exp(z).x;
-    if constexpr (ACT == kActGeluTanh) return z * sigmoid_fast(kGeluTanhC * fmaf(kGeluCubic * z * z, z, z));
-    if constexpr (ACT == kActSilu) return z * sigmoid_fast(z);
+__device__ __forceinline__ float2 act_value2(float2 z) {
+    if constexpr (ACT == kActRelu) return make_float2(relu(z.x), relu(z.y));
+    if constexpr (ACT == kActGelu) {
+        float2 e;
+        return __fmul2_rn(z, normal_cdf2(z, e));
+    }
+    if constexpr (ACT == kActGeluTanh) {
+        const float2 c = __ffma2_rn(__fmul2_rn(__fmul2_rn(z, z), splat2(kGeluCubic)), z, z);
+        return __fmul2_rn(z, sigmoid2(c, kGeluTanhC));
+    }
+    if constexpr (ACT == kActSilu) return __fmul2_rn(z, sigmoid2(z, 1.0f));
     return z;
 }
 
-// value and derivative together
+// values, and the derivatives in `slope`
 template <int ACT>
-__device__ __forceinline__ float2 act_value_slope(float z) {
-    if constexpr (ACT == kActRelu) return make_float2(act_value<kActRelu>(z), z > 0.0f ? 1.0f : 0.0f);
+__device__ __forceinline__ float2 act_value_slope2(float2 z, float2& slope) {
+    if constexpr (ACT == kActRelu) {
+        slope = make_float2(z.x > 0.0f ? 1.0f : 0.0f, z.y > 0.0f ? 1.0f : 0.0f);
+        return act_value2<kActRelu>(z);
+    }
     if constexpr (ACT == kActGelu) {
-        const float2 p = normal_cdf_exp(z);
-        return make_float2(z * p.x, fmaf(z * kInvSqrt2Pi, p.y, p.x));
+        float2 e;
+        const float2 p = normal_cdf2(z, e);
+        slope = __ffma2_rn(__fmul2_rn(z, splat2(kInvSqrt2Pi)), e, p);
+        return __fmul2_rn(z, p);
     }
-    if constexpr (ACT == kActGeluTanh) {
-        const float z2 = z * z;
-        const float p = sigmoid_fast(kGeluTanhC * fmaf(kGeluCubic * z2, z, z));
-        return make_float2(z * p, fmaf(z * p * (1.0f - p), kGeluTanhC * fmaf(3.0f * kGeluCubic, z2, 1.0f), p));
+    if constexpr (ACT == kActGeluTanh || ACT == kActSilu) {
+        // d(z sigmoid(c)) = p + z p (1 - p) c', with c' = 1 for SiLU
+        const float2 z2 = __fmul2_rn(z, z);
+        const bool tanh_form = ACT == kActGeluTanh;
+        const float2 p = tanh_form ? sigmoid2(__ffma2_rn(__fmul2_rn(z2, splat2(kGeluCubic)), z, z), kGeluTanhC) : sigmoid2(z, 1.0f);
+        const float2 v = __fmul2_rn(z, p);
+        float2 w = __ffma2_rn(p, splat2(-1.0f), splat2(1.0f));
+        if (tanh_form) w = __fmul2_rn(w, __ffma2_rn(z2, splat2(3.0f * kGeluCubic * kGeluTanhC), splat2(kGeluTanhC)));
+        slope = __ffma2_rn(v, w, p);
+        return v;
     }
-    if constexpr (ACT == kActSilu) {
-        const float p = sigmoid_fast(z);
-        return make_float2(z * p, fmaf(z * p, 1.0f - p, p));
-    }
-    return make_float2(z, 1.0f);
+    slope = splat2(1.0f);
+    return z;
 }
 
 template <int V>

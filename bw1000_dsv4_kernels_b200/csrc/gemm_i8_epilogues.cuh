@@ -37,9 +37,6 @@ __device__ __forceinline__ void load_row32(Row32& r, const __nv_bfloat16* p, int
         }
     }
 }
-__device__ __forceinline__ float row32_at(const Row32& r, int j) {
-    return (j & 1) ? bf16hi_to_f32(r.w[j >> 1]) : bf16lo_to_f32(r.w[j >> 1]);
-}
 __device__ __forceinline__ void store_row32(__nv_bfloat16* p, const Row32& r, int n_left, bool vec) {
     if (vec && n_left >= 32) {
 #pragma unroll
@@ -56,48 +53,106 @@ __device__ __forceinline__ void store_row32(__nv_bfloat16* p, const Row32& r, in
 __device__ __forceinline__ bool row_vector_ok(const void* base, int64_t ld) {
     return (ld % 8 == 0) && ((reinterpret_cast<uintptr_t>(base) & 15) == 0);
 }
+__device__ __forceinline__ bool block_vector_ok(const void* base, int64_t ld, int n) { return row_vector_ok(base, ld) && n % 8 == 0; }
 
-__device__ __forceinline__ float scaled(uint32_t acc, float sa, float sb, float bias) {
-    return __fadd_rn(__fmul_rn(__fmul_rn(__int2float_rn((int)acc), sa), sb), bias);
+// z of two columns.  A missing bias is -0, which leaves every product as it is: the bits of the plain epilogue.
+constexpr float kNoBias = -0.0f;
+__device__ __forceinline__ float2 scaled2(uint32_t acc0, uint32_t acc1, float sa, float2 sb, float2 bias) {
+    const float2 f = make_float2(__int2float_rn((int)acc0), __int2float_rn((int)acc1));
+    return __ffma2_rn(__fmul2_rn(f, splat2(sa)), sb, bias);
 }
 
-// A warp's 32 x 32 block of a bf16 array, one row per lane.  Rows that are 16-byte aligned move as four 16-byte accesses
-// per lane.  Otherwise (odd widths, odd addresses) an access per element and lane would touch 32 lines each, 32 times;
-// the block goes through the warp's shared memory instead, where lane = column makes each row one access.
-constexpr int kStagePitch = 17;                        // words per row: 16 plus one against bank conflicts
+// A warp's block of 32 rows x 64 bytes (32 bf16 or 16 fp32), one row per lane in registers.  Stored from there directly, an
+// instruction touches 32 rows, half a 32-byte sector in each; the block goes through the warp's shared memory instead,
+// and every instruction moves 64 contiguous bytes of eight rows (16-byte aligned rows) or of one row (odd widths and
+// addresses, an element per lane).  8192 x 8192 x 1024 with bias and residual: 140 us stored directly, STAGED_US staged.
+constexpr int kStagePitch = 20;                        // words per row: 16, and 4 that keep 16-byte accesses off each other's banks
 constexpr int kBlockBytes = 32 * kStagePitch * 4;
 struct RowBlock {
     int rows;     // valid rows of the block (lane r owns row r)
-    int cols;     // valid columns
-    bool vec;     // rows are 16-byte aligned
+    int cols;     // valid columns; those beyond are not touched, and read as zero
+    bool vec;     // rows are 16-byte aligned and `cols` comes in whole 16-byte pieces
 };
-__device__ __forceinline__ Row32 load_block(const __nv_bfloat16* block, int64_t ld, const RowBlock& b, uint32_t* stage, int lane) {
-    Row32 r = {};
-    if (b.vec && b.cols >= 32) {
-        if (lane < b.rows) load_row32(r, block + lane * ld, 32, true);
-        return r;
-    }
-    __syncwarp();
-    uint16_t* s16 = reinterpret_cast<uint16_t*>(stage);
-    const uint16_t* src = reinterpret_cast<const uint16_t*>(block) + lane;
-#pragma unroll 8
-    for (int i = 0; i < 32; ++i)
-        s16[i * (2 * kStagePitch) + lane] = i < b.rows && lane < b.cols ? src[i * ld] : (uint16_t)0;
+__device__ __forceinline__ void stage_row(uint32_t* stage, int lane, const uint4 (&v)[4]) {
     __syncwarp();
 #pragma unroll
-    for (int j = 0; j < 16; ++j) r.w[j] = stage[lane * kStagePitch + j];
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(stage + lane * kStagePitch + 4 * j) = v[j];
+    __syncwarp();
+}
+// 16-byte pieces: `pieces` (1..4) valid ones per row
+__device__ __forceinline__ void store_pieces(char* block, int64_t ld_bytes, const uint4 (&v)[4], int rows, int pieces,
+                                             uint32_t* stage, int lane) {
+    stage_row(stage, lane, v);
+    const int piece = lane & 3;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int row = 8 * i + (lane >> 2);
+        if (row < rows && piece < pieces)
+            *reinterpret_cast<uint4*>(block + row * ld_bytes + 16 * piece) =
+                *reinterpret_cast<const uint4*>(stage + row * kStagePitch + 4 * piece);
+    }
+}
+// Loading takes two steps, so that the requests can be out long before the block is needed: fetch_block issues them into
+// registers as the memory is laid out, arrange_block turns those into one row per lane.
+struct Fetched {
+    uint32_t w[16];
+};
+__device__ __forceinline__ Fetched fetch_block(const __nv_bfloat16* block, int64_t ld, const RowBlock& b, int lane) {
+    Fetched f = {};
+    if (b.vec) {
+        const int piece = lane & 3;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int row = 8 * i + (lane >> 2);
+            if (row < b.rows && 8 * piece < b.cols) {
+                const uint4 q = *reinterpret_cast<const uint4*>(block + row * ld + 8 * piece);
+                f.w[4 * i] = q.x; f.w[4 * i + 1] = q.y; f.w[4 * i + 2] = q.z; f.w[4 * i + 3] = q.w;
+            }
+        }
+    } else if (lane < b.cols) {
+        const uint16_t* src = reinterpret_cast<const uint16_t*>(block) + lane;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t lo = 2 * i < b.rows ? src[(2 * i) * ld] : 0u, hi = 2 * i + 1 < b.rows ? src[(2 * i + 1) * ld] : 0u;
+            f.w[i] = lo | (hi << 16);
+        }
+    }
+    return f;
+}
+__device__ __forceinline__ Row32 arrange_block(const Fetched& f, bool vec, uint32_t* stage, int lane) {
+    __syncwarp();
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint4*>(stage + (8 * i + (lane >> 2)) * kStagePitch + 4 * (lane & 3)) =
+                make_uint4(f.w[4 * i], f.w[4 * i + 1], f.w[4 * i + 2], f.w[4 * i + 3]);
+    } else {
+        uint16_t* s16 = reinterpret_cast<uint16_t*>(stage);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            s16[(2 * i) * (2 * kStagePitch) + lane] = (uint16_t)(f.w[i] & 0xffffu);
+            s16[(2 * i + 1) * (2 * kStagePitch) + lane] = (uint16_t)(f.w[i] >> 16);
+        }
+    }
+    __syncwarp();
+    Row32 r;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const uint4 q = *reinterpret_cast<const uint4*>(stage + lane * kStagePitch + 4 * j);
+        r.w[4 * j] = q.x; r.w[4 * j + 1] = q.y; r.w[4 * j + 2] = q.z; r.w[4 * j + 3] = q.w;
+    }
     return r;
 }
 __device__ __forceinline__ void store_block(__nv_bfloat16* block, int64_t ld, const Row32& r, const RowBlock& b, uint32_t* stage,
                                             int lane) {
-    if (b.vec && b.cols >= 32) {
-        if (lane < b.rows) store_row32(block + lane * ld, r, 32, true);
+    uint4 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = make_uint4(r.w[4 * j], r.w[4 * j + 1], r.w[4 * j + 2], r.w[4 * j + 3]);
+    if (b.vec) {
+        store_pieces(reinterpret_cast<char*>(block), 2 * ld, v, b.rows, (b.cols + 7) >> 3, stage, lane);
         return;
     }
-    __syncwarp();
-#pragma unroll
-    for (int j = 0; j < 16; ++j) stage[lane * kStagePitch + j] = r.w[j];
-    __syncwarp();
+    stage_row(stage, lane, v);
     const uint16_t* s16 = reinterpret_cast<const uint16_t*>(stage);
     uint16_t* dst = reinterpret_cast<uint16_t*>(block) + lane;
     if (lane < b.cols) {
@@ -117,14 +172,14 @@ struct Cols32 {
     const float* p;
     __device__ __forceinline__ float4 four(int j) const { return *reinterpret_cast<const float4*>(p + 4 * j); }
 };
-__device__ __forceinline__ float at(const float4& v, int k) { return k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w; }
+__device__ __forceinline__ float2 two(const float4& v, int k) { return k == 0 ? make_float2(v.x, v.y) : make_float2(v.z, v.w); }
 
 // Column scales and biases of a tile -> a warp's shared copy (one CTA per tile kernel)
 __device__ __forceinline__ void stage_columns(const Params& p, float* sbs, float* bias_s, int lane, int count, int first) {
     for (int j = lane; j < count; j += 32) {
         const int c = first + j;
         sbs[j] = c < p.N ? __ldg(p.sb + c) : 0.0f;
-        bias_s[j] = c < p.N && p.bias != nullptr ? __bfloat162float(p.bias[c]) : 0.0f;
+        bias_s[j] = c < p.N && p.bias != nullptr ? __bfloat162float(p.bias[c]) : kNoBias;
     }
 }
 
@@ -136,15 +191,16 @@ __device__ __forceinline__ Row32 linear_values(const uint32_t (&r)[32], float sa
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const float4 s4 = sb.four(j), b4 = bias.four(j);
-        float y[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int e = 4 * j + k;
-            y[k] = act_value<ACT>(scaled(r[e], sa, at(s4, k), at(b4, k)));
-            if (has_res) y[k] = __fadd_rn(y[k], row32_at(res, e));
+        for (int k = 0; k < 2; ++k) {
+            const int e = 4 * j + 2 * k;
+            float2 y = act_value2<ACT>(scaled2(r[e], r[e + 1], sa, two(s4, k), two(b4, k)));
+            if (has_res) {
+                const float2 add = bf16x2_to_f32x2(res.w[e >> 1]);
+                y = make_float2(__fadd_rn(y.x, add.x), __fadd_rn(y.y, add.y));
+            }
+            out.w[e >> 1] = pack_bf16x2_rn(y.x, y.y);
         }
-        out.w[2 * j] = pack_bf16x2_rn(y[0], y[1]);
-        out.w[2 * j + 1] = pack_bf16x2_rn(y[2], y[3]);
     }
     return out;
 }
@@ -183,37 +239,49 @@ __device__ __forceinline__ Row32 gated_values(const uint32_t (&g)[32], const uin
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
         const float4 sg4 = sg.four(j), bg4 = bg.four(j), su4 = su.four(j), bu4 = bu.four(j);
-        float h[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int e = 4 * j + k;
-            h[k] = act_value<ACT>(scaled(g[e], sa, at(sg4, k), at(bg4, k))) * scaled(u[e], sa, at(su4, k), at(bu4, k));
+        for (int k = 0; k < 2; ++k) {
+            const int e = 4 * j + 2 * k;
+            const float2 h = __fmul2_rn(act_value2<ACT>(scaled2(g[e], g[e + 1], sa, two(sg4, k), two(bg4, k))),
+                                        scaled2(u[e], u[e + 1], sa, two(su4, k), two(bu4, k)));
+            out.w[e >> 1] = pack_bf16x2_rn(h.x, h.y);
         }
-        out.w[2 * j] = pack_bf16x2_rn(h[0], h[1]);
-        out.w[2 * j + 1] = pack_bf16x2_rn(h[2], h[3]);
     }
     return out;
 }
 
-__device__ __forceinline__ void store4f(float* p, const float (&v)[4]) {
-    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+__device__ __forceinline__ uint4 bits4(const float2& a, const float2& b) {
+    return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
+}
+__device__ __forceinline__ unsigned top_bits2(unsigned top, const float2& v, const float2& s) {
+    const float2 t = __fmul2_rn(v, s);
+    return top_bits(top_bits(top, t.x), t.y);
 }
 
-// dz of 32 columns -> dz (16-byte aligned); returns the largest |dz * sb| as bits, together with `top`
+// dz of 32 columns -> the warp's block of dz (fp32, rows 16-byte aligned with room for whole chunks); returns the row's
+// largest |dz * sb| as bits, together with `top`
 template <int ACT>
 __device__ __forceinline__ unsigned linear_gradients(const uint32_t (&r)[32], float sa, Cols32 sb, Cols32 bias, const Row32& dy,
-                                                     float* dz, bool store, unsigned top) {
+                                                     float* block, int64_t ld, int rows, uint32_t* stage, int lane, unsigned top) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float4 s4 = sb.four(j), b4 = bias.four(j);
-        float v[4];
+    for (int half = 0; half < 2; ++half) {
+        uint4 out[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int e = 4 * j + k;
-            v[k] = row32_at(dy, e) * act_value_slope<ACT>(scaled(r[e], sa, at(s4, k), at(b4, k))).y;
-            top = top_bits(top, v[k] * at(s4, k));
+        for (int i = 0; i < 4; ++i) {
+            const int j = 4 * half + i;
+            const float4 s4 = sb.four(j), b4 = bias.four(j);
+            float2 v[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int e = 4 * j + 2 * k;
+                float2 slope;
+                act_value_slope2<ACT>(scaled2(r[e], r[e + 1], sa, two(s4, k), two(b4, k)), slope);
+                v[k] = __fmul2_rn(bf16x2_to_f32x2(dy.w[e >> 1]), slope);
+                top = top_bits2(top, v[k], two(s4, k));
+            }
+            out[i] = bits4(v[0], v[1]);
         }
-        if (store) store4f(dz + 4 * j, v);
+        store_pieces(reinterpret_cast<char*>(block + 16 * half), 4 * ld, out, rows, 4, stage, lane);
     }
     return top;
 }
@@ -221,34 +289,40 @@ __device__ __forceinline__ unsigned linear_gradients(const uint32_t (&r)[32], fl
 // dg and du of 32 outputs
 template <int ACT>
 __device__ __forceinline__ unsigned gated_gradients(const uint32_t (&g)[32], const uint32_t (&u)[32], float sa, Cols32 sg,
-                                                    Cols32 bg, Cols32 su, Cols32 bu, const Row32& dh, float* dg, float* du,
-                                                    bool store, unsigned top) {
+                                                    Cols32 bg, Cols32 su, Cols32 bu, const Row32& dh, float* block_g,
+                                                    float* block_u, int64_t ld, int rows, uint32_t* stage, int lane, unsigned top) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const float4 sg4 = sg.four(j), bg4 = bg.four(j), su4 = su.four(j), bu4 = bu.four(j);
-        float vg[4], vu[4];
+    for (int half = 0; half < 2; ++half) {
+        uint4 out_g[4], out_u[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const int e = 4 * j + k;
-            const float2 vs = act_value_slope<ACT>(scaled(g[e], sa, at(sg4, k), at(bg4, k)));
-            const float d = row32_at(dh, e);
-            vg[k] = d * scaled(u[e], sa, at(su4, k), at(bu4, k)) * vs.y;
-            vu[k] = d * vs.x;
-            top = top_bits(top_bits(top, vg[k] * at(sg4, k)), vu[k] * at(su4, k));
+        for (int i = 0; i < 4; ++i) {
+            const int j = 4 * half + i;
+            const float4 sg4 = sg.four(j), bg4 = bg.four(j), su4 = su.four(j), bu4 = bu.four(j);
+            float2 vg[2], vu[2];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const int e = 4 * j + 2 * k;
+                float2 slope;
+                const float2 value = act_value_slope2<ACT>(scaled2(g[e], g[e + 1], sa, two(sg4, k), two(bg4, k)), slope);
+                const float2 d = bf16x2_to_f32x2(dh.w[e >> 1]);
+                vg[k] = __fmul2_rn(__fmul2_rn(d, scaled2(u[e], u[e + 1], sa, two(su4, k), two(bu4, k))), slope);
+                vu[k] = __fmul2_rn(d, value);
+                top = top_bits2(top_bits2(top, vg[k], two(sg4, k)), vu[k], two(su4, k));
+            }
+            out_g[i] = bits4(vg[0], vg[1]);
+            out_u[i] = bits4(vu[0], vu[1]);
         }
-        if (store) {
-            store4f(dg + 4 * j, vg);
-            store4f(du + 4 * j, vu);
-        }
+        store_pieces(reinterpret_cast<char*>(block_g + 16 * half), 4 * ld, out_g, rows, 4, stage, lane);
+        store_pieces(reinterpret_cast<char*>(block_u + 16 * half), 4 * ld, out_u, rows, 4, stage, lane);
     }
     return top;
 }
 
 // Split-K epilogues of the weight-streaming kernels (see reduce_partials_and_store): the item's partials come through
 // distributed shared memory, its residual from HBM at the same time.
-__device__ __forceinline__ void store4(const Params& p, int row, int n, const float (&v)[4], bool vec) {
+__device__ __forceinline__ void store4(const Params& p, int row, int n, const float2& a, const float2& b, bool vec) {
     __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.C) + (int64_t)row * p.ldc + n;
-    const uint32_t lo = pack_bf16x2_rn(v[0], v[1]), hi = pack_bf16x2_rn(v[2], v[3]);
+    const uint32_t lo = pack_bf16x2_rn(a.x, a.y), hi = pack_bf16x2_rn(b.x, b.y);
     if (vec && n + 4 <= p.N) {
         *reinterpret_cast<uint2*>(out) = make_uint2(lo, hi);
     } else {
@@ -299,7 +373,7 @@ __device__ __forceinline__ void reduce_partials_fused(const Params& p, const uin
                 }
             }
         }
-        float z[U][kHalves][4];
+        float2 z[U][kHalves][2];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int it = it0 + u * nthreads;
@@ -316,8 +390,11 @@ __device__ __forceinline__ void reduce_partials_fused(const Params& p, const uin
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    z[u][h][j] = scaled((uint32_t)a[j], sa, sb_s[h * 64 + g * 4 + j], bias_s[h * 64 + g * 4 + j]);
+                for (int j = 0; j < 2; ++j) {
+                    const int col = h * 64 + g * 4 + 2 * j;
+                    z[u][h][j] = scaled2((uint32_t)a[2 * j], (uint32_t)a[2 * j + 1], sa, make_float2(sb_s[col], sb_s[col + 1]),
+                                         make_float2(bias_s[col], bias_s[col + 1]));
+                }
             }
         }
         // one choice of the activation for all items: a tile's epilogue runs once, so its instructions are fetched cold
@@ -325,9 +402,9 @@ __device__ __forceinline__ void reduce_partials_fused(const Params& p, const uin
 #pragma unroll
             for (int u = 0; u < U; ++u) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    z[u][0][j] = act_value<decltype(act)::value>(z[u][0][j]);
-                    if constexpr (GATED) z[u][0][j] *= z[u][kHalves - 1][j];
+                for (int j = 0; j < 2; ++j) {
+                    z[u][0][j] = act_value2<decltype(act)::value>(z[u][0][j]);
+                    if constexpr (GATED) z[u][0][j] = __fmul2_rn(z[u][0][j], z[u][kHalves - 1][j]);
                 }
             }
         });
@@ -338,12 +415,11 @@ __device__ __forceinline__ void reduce_partials_fused(const Params& p, const uin
             const int c = cols_lo + (it >> kShift), n = n0 + (it & (kGroups - 1)) * 4;
             if (n >= p.N) continue;
             if (!GATED && p.resid != nullptr) {
-                z[u][0][0] = __fadd_rn(z[u][0][0], bf16lo_to_f32(res[u].x));
-                z[u][0][1] = __fadd_rn(z[u][0][1], bf16hi_to_f32(res[u].x));
-                z[u][0][2] = __fadd_rn(z[u][0][2], bf16lo_to_f32(res[u].y));
-                z[u][0][3] = __fadd_rn(z[u][0][3], bf16hi_to_f32(res[u].y));
+                const float2 r0 = bf16x2_to_f32x2(res[u].x), r1 = bf16x2_to_f32x2(res[u].y);
+                z[u][0][0] = make_float2(__fadd_rn(z[u][0][0].x, r0.x), __fadd_rn(z[u][0][0].y, r0.y));
+                z[u][0][1] = make_float2(__fadd_rn(z[u][0][1].x, r1.x), __fadd_rn(z[u][0][1].y, r1.y));
             }
-            store4(p, c, n, z[u][0], vec_store);
+            store4(p, c, n, z[u][0][0], z[u][0][1], vec_store);
         }
     }
 }

@@ -211,7 +211,7 @@ gemm_i8_fused_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
         uint32_t* stage = reinterpret_cast<uint32_t*>(smem + L::kTransposeOff + (warp - 2) * kBlockBytes);
         const int chunks = out_n / 32;
         const bool has_res = p.resid != nullptr;
-        const bool in_vec = row_vector_ok(p.resid, p.ldr), out_vec = row_vector_ok(p.C, p.ldc);
+        const bool in_vec = block_vector_ok(p.resid, p.ldr, p.N), out_vec = block_vector_ok(p.C, p.ldc, p.N);
         int acc = 0;
         uint32_t acc_phase = 0;
         for (int t = pair; t < total; t += npairs) {
@@ -228,20 +228,20 @@ gemm_i8_fused_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
                 if constexpr (kGated) {
                     cols[i * 64 + lane] = ok ? __ldg(p.sb + c) : 0.0f;
                     cols[i * 64 + 32 + lane] = ok ? __ldg(p.sb + cu) : 0.0f;
-                    cols[128 + i * 64 + lane] = ok && p.bias != nullptr ? __bfloat162float(p.bias[c]) : 0.0f;
-                    cols[128 + i * 64 + 32 + lane] = ok && p.bias != nullptr ? __bfloat162float(p.bias[cu]) : 0.0f;
+                    cols[128 + i * 64 + lane] = ok && p.bias != nullptr ? __bfloat162float(p.bias[c]) : kNoBias;
+                    cols[128 + i * 64 + 32 + lane] = ok && p.bias != nullptr ? __bfloat162float(p.bias[cu]) : kNoBias;
                 } else {
                     cols[i * 32 + lane] = ok ? __ldg(p.sb + c) : 0.0f;
-                    cols[128 + i * 32 + lane] = ok && p.bias != nullptr ? __bfloat162float(p.bias[c]) : 0.0f;
+                    cols[128 + i * 32 + lane] = ok && p.bias != nullptr ? __bfloat162float(p.bias[c]) : kNoBias;
                 }
             }
             // residual or incoming gradient of the chunk at column n; zeros where there is none
             auto fetch = [&](int cc) {
                 const int n = n0 + cc * 32;
-                if (EPI == kEpiGated || (!kGrad && !has_res) || cc >= chunks || n >= p.N || rows <= 0) return Row32{};
-                return load_block(p.resid + (int64_t)row0 * p.ldr + n, p.ldr, {rows, p.N - n, in_vec}, stage, lane);
+                if (EPI == kEpiGated || (!kGrad && !has_res) || cc >= chunks || n >= p.N || rows <= 0) return Fetched{};
+                return fetch_block(p.resid + (int64_t)row0 * p.ldr + n, p.ldr, {rows, p.N - n, in_vec}, lane);
             };
-            Row32 in = fetch(turn);
+            Fetched fetched = fetch(turn);
             const float sa = row_ok ? __ldg(p.sa + row) : 0.0f;
             __syncwarp();
             if (!ptx::mbar_wait_bounded(acc_full_bar(acc), acc_phase, p.wait_limit_ns) || *abort_flag) {
@@ -261,7 +261,9 @@ gemm_i8_fused_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
                 __syncwarp();  // tcgen05.ld is warp-collective
                 ptx::tmem_ld_32x32b_x32(t_lane + cc * 32, r);
                 if constexpr (kGated) ptx::tmem_ld_32x32b_x32(t_lane + half_n + cc * 32, u);
-                const Row32 next = fetch(cc + 2);
+                Row32 in = {};
+                if (kGrad || (EPI == kEpiLinear && has_res)) in = arrange_block(fetched, in_vec, stage, lane);
+                fetched = fetch(cc + 2);
                 ptx::tmem_ld_wait();
                 if constexpr (!kGrad) {
                     Row32 out;
@@ -271,14 +273,13 @@ gemm_i8_fused_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
                                 {rows, p.N - n, out_vec}, stage, lane);
                 } else {
                     // dz has room for whole chunks; columns at or beyond N get zeros (their gradient was read as zero)
-                    float* dz = static_cast<float*>(p.C) + (int64_t)row * p.ldc + n;
+                    float* dz = static_cast<float*>(p.C) + (int64_t)row0 * p.ldc + n;
                     if constexpr (kGated)
                         top = gated_gradients<ACT>(r, u, sa, {col}, {col + 128}, {col + 32}, {col + 160}, in, dz, dz + p.up_col,
-                                                   row_ok, top);
+                                                   p.ldc, rows, stage, lane, top);
                     else
-                        top = linear_gradients<ACT>(r, sa, {col}, {col + 128}, in, dz, row_ok, top);
+                        top = linear_gradients<ACT>(r, sa, {col}, {col + 128}, in, dz, p.ldc, rows, stage, lane, top);
                 }
-                in = next;
             }
             if constexpr (kGrad) {
                 if (row_ok && top != 0) atomicMax(p.row_top + row, top);

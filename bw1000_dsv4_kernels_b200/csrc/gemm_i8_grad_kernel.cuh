@@ -157,7 +157,7 @@ gemm_i8_grad_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
         const int quarter = warp & 3, turn = (warp - 2) >> 2;
         uint32_t* stage = reinterpret_cast<uint32_t*>(smem + L::kTransposeOff + (warp - 2) * kBlockBytes);
         uint32_t acc_phase = 0;
-        const bool vec = p.K % 8 == 0 && (reinterpret_cast<uintptr_t>(p.dx) & 15) == 0;
+        const bool vec = block_vector_ok(p.dx, p.K, p.K);
         const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         for (int t = pair; t < total; t += npairs) {
             int mt, kt;

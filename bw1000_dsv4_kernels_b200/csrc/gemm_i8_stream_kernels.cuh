@@ -135,7 +135,7 @@ __device__ __forceinline__ void stage_scales(const Params& p, float* sa_s, float
             const int c = up ? p.inter + n0 + (j - 64) : n0 + j;
             const bool ok = c < (up ? 2 * p.inter : p.N);
             sb_s[j] = ok ? __ldg(p.sb + c) : 0.0f;
-            bias_s[j] = ok && p.bias != nullptr ? __bfloat162float(p.bias[c]) : 0.0f;
+            bias_s[j] = ok && p.bias != nullptr ? __bfloat162float(p.bias[c]) : kNoBias;
         }
     }
 }
