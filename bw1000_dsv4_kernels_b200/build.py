@@ -53,7 +53,7 @@ def build_cuda_lib(force: bool = False, verbose: bool = False, ptxas_info: bool 
     # -fmad=false: a multiply and an add that the sources write as two rounded steps must stay two
     # instructions (fused forms are written explicitly where they are meant)
     cmd = [nvcc, *ARCH_FLAGS, "-lineinfo", "-O3", "-fmad=false", "-std=c++17", "-shared", "-Xcompiler", "-fPIC",
-           "-Xcompiler", "-fvisibility=hidden", "--threads", "0", "--split-compile", "0", "-o", LIB_PATH, *srcs]
+           "-Xcompiler", "-fvisibility=hidden", "--threads", "4", "-o", LIB_PATH, *srcs]
     if ptxas_info:
         cmd[1:1] = ["-Xptxas", "-v"]
     _run(cmd, verbose)

@@ -13,11 +13,14 @@
 // unrounded sum).  The variance comes from the deviations, not from sum(a^2) - mean^2, which loses every digit of a row
 // with a large mean.  All statistics and sums are fp32.
 //
-// Everything here is bound by HBM.  A row belongs to a group of T threads (T a multiple of 32, chosen so that the row
-// fits the group's registers, packed as it came), is read once and stays on chip between its reductions.  Rows move in
-// accesses of eight elements where width and addresses allow, else of two, else of one; rows wider than the registers
-// hold are read again for each reduction (the *_wide kernels).  Arithmetic is on pairs (packed f32x2), without which the
-// backward pass was bound by its instructions (52 % of the issue slots, 38 % of HBM).
+// Everything here is bound by HBM.  A row belongs to a group of G threads and is read once.
+//   * Forward: a row per group, straight from HBM, several CTAs per SM.
+//   * Backward: one CTA per SM, so that every thread can keep the column sums of its columns in registers; its groups
+//     walk the rows, and the next rows are on their way into shared memory (cp.async) while two are worked on.  Rows whose
+//     width or address does not allow 16-byte accesses come in as the 16-byte granules that cover them and are taken apart
+//     in shared memory (2-byte accesses to HBM took 1270 us for 8192 x 7165, the granules 268 us).
+//   * Rows wider than 16384 are read again for each reduction (the *_wide kernels).
+// Arithmetic is on pairs (packed f32x2): the backward pass was otherwise bound by its instructions.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <cstdint>
@@ -93,39 +96,153 @@ __device__ __forceinline__ uint32_t rounded(float2 a) { return pack_bf16x2_rn(a.
 // Two slots of `red` take turns, so a group needs one barrier per reduction: a slot is written again only after the
 // barrier of the reduction in between.
 struct Group {
-    float2* red;       // [2][32] of this group
+    float2* red;       // [2][64] of this group, 16-byte aligned (not used by a group of one warp)
     int threads;       // multiple of 32
     int id;            // hardware barrier of the group: 1 + index in the CTA
     int turn = 0;
     __device__ __forceinline__ void barrier() const { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-    template <typename Op>
-    __device__ __forceinline__ float2 reduce(float2 v, Op op) {
+    template <typename T, typename Op>
+    __device__ __forceinline__ T reduce(T v, Op op) {
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-            v = op(v, make_float2(__shfl_xor_sync(kFullWarp, v.x, o), __shfl_xor_sync(kFullWarp, v.y, o)));
+        for (int o = 16; o > 0; o >>= 1) v = op(v, shuffle(v, o));
         if (threads == 32) return v;
         const int lane = threadIdx.x & 31, warp = (threadIdx.x % threads) >> 5, warps = threads >> 5;
-        float2* slot = red + 32 * turn;
+        T* slot = reinterpret_cast<T*>(red + 64 * turn);
         turn ^= 1;
         if (lane == 0) slot[warp] = v;
         barrier();
         v = slot[lane < warps ? lane : 0];
-        if (lane >= warps) v = make_float2(0.0f, 0.0f);   // neutral for sums, and for maxima of magnitudes
+        if (lane >= warps) v = T{};   // neutral for sums, and for maxima of magnitudes
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-            v = op(v, make_float2(__shfl_xor_sync(kFullWarp, v.x, o), __shfl_xor_sync(kFullWarp, v.y, o)));
+        for (int o = 16; o > 0; o >>= 1) v = op(v, shuffle(v, o));
         return v;
     }
+    static __device__ __forceinline__ float shuffle(float v, int o) { return __shfl_xor_sync(kFullWarp, v, o); }
+    static __device__ __forceinline__ float2 shuffle(float2 v, int o) { return make_float2(shuffle(v.x, o), shuffle(v.y, o)); }
     __device__ __forceinline__ float2 sum2(float2 v) {
         return reduce(v, [](float2 a, float2 b) { return make_float2(a.x + b.x, a.y + b.y); });
     }
     __device__ __forceinline__ float sum(float v) {
-        return reduce(make_float2(v, 0.0f), [](float2 a, float2 b) { return make_float2(a.x + b.x, 0.0f); }).x;
+        return reduce(v, [](float a, float b) { return a + b; });
     }
     __device__ __forceinline__ float max(float v) {
-        return reduce(make_float2(v, 0.0f), [](float2 a, float2 b) { return make_float2(fmaxf(a.x, b.x), 0.0f); }).x;
+        return reduce(v, [](float a, float b) { return fmaxf(a, b); });
+    }
+    // Four sums at once: halves of the warp keep two of the values each, quarters one, so that thirteen shuffles do what
+    // forty would.  Entries of warps that the group does not have must be zero (clear4).
+    __device__ __forceinline__ void clear4() {
+        const int i = threadIdx.x % threads;
+        if (threads > 32) {
+            for (int k = i; k < 256; k += threads) reinterpret_cast<float*>(red)[k] = 0.0f;
+            barrier();
+        }
+    }
+    __device__ __forceinline__ float4 sum4(float4 v) {
+        const int lane = threadIdx.x & 31;
+        const bool up16 = lane & 16, up8 = lane & 8;
+        float a = up16 ? v.z : v.x, b = up16 ? v.w : v.y;
+        a += shuffle(up16 ? v.x : v.z, 16);
+        b += shuffle(up16 ? v.y : v.w, 16);
+        float k = up8 ? b : a;
+        k += shuffle(up8 ? a : b, 8);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) k += shuffle(k, o);
+        if (threads > 32) {
+            // value (lane / 8) of warp w at [lane / 8][w]; the two turns use 128 floats each
+            float* slot = reinterpret_cast<float*>(red) + 128 * turn;
+            turn ^= 1;
+            if ((lane & 7) == 0) slot[(lane >> 3) * 32 + ((threadIdx.x % threads) >> 5)] = k;
+            barrier();
+            const float4 q = *reinterpret_cast<const float4*>(slot + (lane >> 3) * 32 + (lane & 7) * 4);
+            k = (q.x + q.y) + (q.z + q.w);
+#pragma unroll
+            for (int o = 4; o > 0; o >>= 1) k += shuffle(k, o);
+        }
+        return make_float4(__shfl_sync(kFullWarp, k, 0), __shfl_sync(kFullWarp, k, 8), __shfl_sync(kFullWarp, k, 16),
+                           __shfl_sync(kFullWarp, k, 24));
+    }
+    // everything that the group's threads wrote to shared memory is visible to all of them
+    __device__ __forceinline__ void sync() const {
+        if (threads == 32) __syncwarp();
+        else barrier();
     }
 };
+
+// ---- rows on their way through shared memory -------------------------------------------------------------------------
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(reinterpret_cast<uint64_t>(src)) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// One array's rows, `depth` of them in shared memory.  W = 8: thread t owns accesses t, t + G, ... of a row and copies
+// exactly those, so what it waits for is its own.  W < 8: the group copies the 16-byte granules that cover the row
+// (element by element where a granule leaves the array) to the same offset modulo 16, and meets before it reads them.  Results go straight to HBM, an access of W per lane.
+template <int W, int V>
+struct RowStage {
+    char* base;          // this array's slots in the group's shared memory
+    const char* array;   // [M, K] bf16
+    int64_t bytes;       // of the array
+    int slot_bytes;
+    int K, G, t;
+    __device__ __forceinline__ const char* row_ptr(int64_t row) const { return array + row * K * 2; }
+    __device__ __forceinline__ void issue(int slot, int64_t row) const {
+        char* s = base + slot * slot_bytes;
+        const char* src = row_ptr(row);
+        if constexpr (W == 8) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int a = t + j * G;
+                if (a * 8 < K) cp_async16(ptx::smem_u32(s + a * 16), src + a * 16);
+            }
+        } else {
+            const int skew = (int)(reinterpret_cast<uintptr_t>(src) & 15);
+            const char* first = src - skew;
+            const int granules = (skew + 2 * K + 15) >> 4;
+#pragma unroll 1
+            for (int i = t; i < granules; i += G) {
+                const char* g = first + 16 * i;
+                if (g >= array && g + 16 <= array + bytes) {
+                    cp_async16(ptx::smem_u32(s + 16 * i), g);
+                } else {
+#pragma unroll 1
+                    for (int b = 0; b < 16; b += 2)
+                        if (g + b >= src && g + b < src + 2 * K)
+                            *reinterpret_cast<uint16_t*>(s + 16 * i + b) = *reinterpret_cast<const uint16_t*>(g + b);
+                }
+            }
+        }
+    }
+    // where this thread's accesses of a row that has arrived begin, and access j of them
+    __device__ __forceinline__ const char* row(int slot, int64_t r) const {
+        const char* s = base + slot * slot_bytes + t * W * 2;
+        if constexpr (W != 8) s += reinterpret_cast<uintptr_t>(row_ptr(r)) & 15;
+        return s;
+    }
+    __device__ __forceinline__ Pack<W> at(const char* row, int j) const {
+        return load_pack<W>(reinterpret_cast<const __nv_bfloat16*>(row + j * G * W * 2));
+    }
+};
+
+// int8 codes of W values
+template <int W, int N, typename T>
+__device__ __forceinline__ void store_codes(int8_t* q, const T (&y)[N], float inv) {
+    if constexpr (W == 8) {
+        uint32_t o[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            o[2 * i] = quant_rn_lowbyte(y[i].x, inv);
+            o[2 * i + 1] = quant_rn_lowbyte(y[i].y, inv);
+        }
+        *reinterpret_cast<uint2*>(q) = make_uint2(pack_lowbytes(o[0], o[1], o[2], o[3]), pack_lowbytes(o[4], o[5], o[6], o[7]));
+    } else if constexpr (W == 2) {
+        const uint32_t lo = quant_rn_lowbyte(y[0].x, inv) & 0xffu, hi = quant_rn_lowbyte(y[0].y, inv) & 0xffu;
+        *reinterpret_cast<uint16_t*>(q) = (uint16_t)(lo | (hi << 8));
+    } else {
+        *q = (int8_t)(quant_rn_lowbyte(y[0], inv) & 0xffu);
+    }
+}
 
 __device__ __forceinline__ float rstd_of(float sumsq, int K, float eps) {
     return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sumsq, (float)K), eps)));
@@ -141,25 +258,29 @@ struct NormArgs {
     float* s;
     float* mean;
     float* rstd;
-    int M, K, T;
+    int M, K, T;               // T: threads of a group
     float eps;
 };
 
-// ---- forward: blockDim = R groups of T threads, one row per group, V accesses of W elements per thread -------------
-// The row stays packed (four registers per eight elements) and is widened again for each pass: with 62 registers a
-// thread for a widened row, 28 warps an SM did not cover the loads' latency (53 % of HBM).
+// ---- forward: blockDim = R groups of G threads, one row per group, V accesses of W elements per thread ---------------
+// The row stays packed (four registers per eight elements) and is widened again for each pass; the row's pointers are
+// formed once (inside the access loops every access had a 64-bit product of its own, and spilled).  8192 x 7168 with the
+// residual: 98 us with spills, 76-82 us without, 72 us at the measured copy rate.
 template <int W, int V, int THREADS, int CTAS, bool ADD, bool QUANT>
 __global__ void __launch_bounds__(THREADS, CTAS) layernorm_kernel(const NormArgs p) {
     using T = typename Vals<W>::T;
     constexpr int N = Vals<W>::kN;
-    __shared__ float2 red_all[8 * 64];   // a CTA holds at most eight groups
+    __shared__ __align__(16) float2 red_all[8 * 128];   // a CTA holds at most eight groups
     ptx::grid_launch_dependents();  // a GEMM launched to overlap this kernel may start its set-up and weight loads
     const int G = p.T, g = threadIdx.x / G, t = threadIdx.x - g * G;
     const int64_t row = (int64_t)blockIdx.x * (blockDim.x / G) + g;
     if (row >= p.M) return;  // whole groups: nobody is left waiting at the group's barrier
-    Group grp{red_all + 64 * g, G, 1 + g};
+    Group grp{red_all + 128 * g, G, 1 + g};
     const int K = p.K;
     const __nv_bfloat16* x = p.x + row * K;
+    __nv_bfloat16* res_row = p.res + row * K;
+    __nv_bfloat16* y_row = p.y + row * K;
+    int8_t* q_row = p.q + row * K;
     Pack<W> a[V];
     Pack<W> w1, b1;                      // a thread with one access has its weight and bias requested with the row
 #pragma unroll
@@ -179,7 +300,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) layernorm_kernel(const NormArgs
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c = (t + j * G) * W;
-            if (c < K) r[j] = load_pack<W>(p.res + row * K + c);
+            if (c < K) r[j] = load_pack<W>(res_row + c);
         }
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -187,7 +308,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) layernorm_kernel(const NormArgs
             if (c < K) {
 #pragma unroll
                 for (int i = 0; i < N; ++i) a[j].w[i] = rounded(add(value<W>(r[j], i), value<W>(a[j], i)));
-                store_pack<W>(p.res + row * K + c, a[j]);
+                store_pack<W>(res_row + c, a[j]);
             }
         }
     }
@@ -232,7 +353,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) layernorm_kernel(const NormArgs
                 Pack<W> o;
 #pragma unroll
                 for (int i = 0; i < N; ++i) o.w[i] = rounded(y[i]);
-                store_pack<W>(p.y + row * K + c, o);
+                store_pack<W>(y_row + c, o);
             }
         }
     } else {
@@ -256,21 +377,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) layernorm_kernel(const NormArgs
             if (c < K) {
                 T y[N];
                 y_of(j, c, y);
-                int8_t* q = p.q + row * K + c;
-                if constexpr (W == 8) {
-                    uint32_t o[8];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        o[2 * i] = quant_rn_lowbyte(y[i].x, inv);
-                        o[2 * i + 1] = quant_rn_lowbyte(y[i].y, inv);
-                    }
-                    *reinterpret_cast<uint2*>(q) = make_uint2(pack_lowbytes(o[0], o[1], o[2], o[3]), pack_lowbytes(o[4], o[5], o[6], o[7]));
-                } else if constexpr (W == 2) {
-                    const uint32_t lo = quant_rn_lowbyte(y[0].x, inv) & 0xffu, hi = quant_rn_lowbyte(y[0].y, inv) & 0xffu;
-                    *reinterpret_cast<uint16_t*>(q) = (uint16_t)(lo | (hi << 8));
-                } else {
-                    *q = (int8_t)(quant_rn_lowbyte(y[0], inv) & 0xffu);
-                }
+                store_codes<W>(q_row + c, y, inv);
             }
         }
     }
@@ -279,7 +386,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) layernorm_kernel(const NormArgs
 // rows wider than the registers hold: one CTA per row, every reduction reads the row again (it stays in L1 / L2)
 template <bool ADD, bool QUANT>
 __global__ void __launch_bounds__(kMaxGroupThreads) layernorm_wide_kernel(const NormArgs p) {
-    __shared__ float2 red_all[64];
+    __shared__ __align__(16) float2 red_all[128];
     ptx::grid_launch_dependents();
     const int64_t row = blockIdx.x;
     Group grp{red_all, (int)blockDim.x, 1};
@@ -327,91 +434,141 @@ struct NormBwdArgs {
     __nv_bfloat16* dx;
     float* partial;              // [gridDim.x][2][K]: this CTA's share of dw and db
     int M, K, T;
+    int slot_bytes;
 };
 
-// ---- backward: one CTA per SM, its groups walk rows; every thread keeps the sums of its own columns in registers ----
-// AHEAD: the next row's loads are issued before the current row's reduction, so HBM stays busy across the group's
-// barrier; only where both rows fit the registers that THREADS threads leave each (72 for 896, 64 for 1024).
-template <int W, int V, int THREADS, bool RES, bool AHEAD>
+// ---- backward: every thread keeps the sums of its own columns in registers over all the rows that its group walks ----
+// B rows (1 or 2) at a time: one barrier for both, and two rows' work to hide each other's latencies.  One row at a time
+// stood at its barriers (8192 x 7168: 172 us with eight columns per thread and one group of 896 threads, 138 us with 16 and
+// two groups, which spilled).  Two rows, 16 columns per thread and 448 threads with 128 registers each: 79 us, of which 4.5
+// are the sum of the CTAs' shares; 72 us at the measured copy rate.  Eight columns and 896 threads take 85 to 111 us, with
+// the compiler's luck; rows in pieces of two or one elements are better off with them (7165: 191 against 219 us).
+template <int W, int V, int B, int DEPTH, int THREADS, bool RES>
 __global__ void __launch_bounds__(THREADS, 1) layernorm_backward_kernel(const NormBwdArgs p) {
     using T = typename Vals<W>::T;
-    constexpr int N = Vals<W>::kN;
-    __shared__ float2 red_all[32 * 64];
-    extern __shared__ float cols[];   // [R][2][K]: the groups' column sums, when there is more than one group
-    const int G = p.T, R = blockDim.x / G, g = threadIdx.x / G, t = threadIdx.x - g * G;
-    Group grp{red_all + 64 * g, G, 1 + g};
-    const int K = p.K;
+    constexpr int N = Vals<W>::kN, kArrays = RES ? 3 : 2;
+    __shared__ __align__(16) float2 red_all[15 * 128];
+    extern __shared__ __align__(16) char rows_smem[];   // the groups' row slots; at the end their column sums
+    const int G = p.T, R = blockDim.x / G, g = threadIdx.x / G, t = threadIdx.x - g * G, K = p.K;
+    Group grp{red_all + (G == 32 ? 0 : 128 * g), G, 1 + g};
+    char* mine = rows_smem + (size_t)g * DEPTH * B * kArrays * p.slot_bytes;
+    const int64_t bytes = (int64_t)p.M * K * 2;
+    const RowStage<W, V> xs{mine, reinterpret_cast<const char*>(p.x), bytes, p.slot_bytes, K, G, t};
+    const RowStage<W, V> ys{mine + DEPTH * B * p.slot_bytes, reinterpret_cast<const char*>(p.dy), bytes, p.slot_bytes, K, G, t};
+    const RowStage<W, V> rs{mine + 2 * DEPTH * B * p.slot_bytes, reinterpret_cast<const char*>(p.dres), bytes, p.slot_bytes, K, G, t};
     const float inv_k = __fdiv_rn(1.0f, (float)K);
+    if constexpr (B == 2) grp.clear4();
     T dw[V][N], db[V][N];
-    Pack<W> w[V], nx[V], ny[V], nr[V];
+    Pack<W> w[V];
 #pragma unroll
     for (int j = 0; j < V; ++j) {
 #pragma unroll
         for (int i = 0; i < N; ++i) dw[j][i] = db[j][i] = all<T>(0.0f);
         if ((t + j * G) * W < K) w[j] = load_pack<W>(p.w + (t + j * G) * W);
     }
-    float nmean = 0.0f, nrstd = 0.0f;
-    const int64_t step = (int64_t)gridDim.x * R;
-    auto fetch = [&](int64_t row) {
-        if (row < p.M) {
+    const int64_t step = (int64_t)gridDim.x * R * B;
+    auto issue = [&](int stage, int64_t first) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const int c = (t + j * G) * W;
-                if (c < K) {
-                    nx[j] = load_pack<W>(p.x + row * K + c);
-                    ny[j] = load_pack<W>(p.dy + row * K + c);
-                    if constexpr (RES) nr[j] = load_pack<W>(p.dres + row * K + c);
-                }
+        for (int b = 0; b < B; ++b) {
+            if (first + b < p.M) {
+                xs.issue(stage * B + b, first + b);
+                ys.issue(stage * B + b, first + b);
+                if constexpr (RES) rs.issue(stage * B + b, first + b);
             }
-            nmean = __ldg(p.mean + row);
-            nrstd = __ldg(p.rstd + row);
+        }
+        cp_async_commit();   // empty past the last row: the count of groups stays in step
+    };
+    float mean[B], rstd[B], next_mean[B], next_rstd[B];
+    auto statistics = [&](int64_t first) {
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            next_mean[b] = first + b < p.M ? __ldg(p.mean + first + b) : 0.0f;
+            next_rstd[b] = first + b < p.M ? __ldg(p.rstd + first + b) : 0.0f;
         }
     };
-    int64_t row = (int64_t)blockIdx.x * R + g;
-    fetch(row);
+    int64_t row = ((int64_t)blockIdx.x * R + g) * B;
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d) issue(d, row + d * step);
+    statistics(row);
+    int stage = 0;
     for (; row < p.M; row += step) {
-        T xh[V][N], tv[V][N];
-        Pack<W> r[V];
-        const float rstd = nrstd;
-        const T rs = all<T>(nrstd), shift = all<T>(-nmean);
-        T c0 = all<T>(0.0f), c1 = all<T>(0.0f);   // sums of t = dy * w and of t * xhat
+        cp_async_wait<DEPTH - 2>();
+        if constexpr (W != 8) grp.sync();
+        // the stage of the rows before: its last readers are behind the barrier above, or are this thread (W = 8)
+        issue(stage == 0 ? DEPTH - 1 : stage - 1, row + (DEPTH - 1) * step);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            if ((t + j * G) * W < K) {
+        for (int b = 0; b < B; ++b) {
+            mean[b] = next_mean[b];
+            rstd[b] = next_rstd[b];
+        }
+        statistics(row + step);
+        float c[B][2];   // sums of t = dy * w and of t * xhat
 #pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const T y = value<W>(ny[j], i);
-                    xh[j][i] = mul(add(value<W>(nx[j], i), shift), rs);
-                    tv[j][i] = mul(y, value<W>(w[j], i));
-                    dw[j][i] = fma(y, xh[j][i], dw[j][i]);
-                    db[j][i] = add(db[j][i], y);
-                    c0 = add(c0, tv[j][i]);
-                    c1 = fma(tv[j][i], xh[j][i], c1);
+        for (int b = 0; b < B; ++b) {
+            T c0 = all<T>(0.0f), c1 = all<T>(0.0f);
+            if (row + b < p.M) {
+                const char* xp = xs.row(stage * B + b, row + b);
+                const char* yp = ys.row(stage * B + b, row + b);
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    if ((t + j * G) * W < K) {
+                        const Pack<W> px = xs.at(xp, j), py = ys.at(yp, j);
+#pragma unroll
+                        for (int i = 0; i < N; ++i) {
+                            const T y = value<W>(py, i), u = mul(y, value<W>(w[j], i));
+                            const T h = mul(add(value<W>(px, i), all<T>(-mean[b])), all<T>(rstd[b]));
+                            dw[j][i] = fma(y, h, dw[j][i]);
+                            db[j][i] = add(db[j][i], y);
+                            c0 = add(c0, u);
+                            c1 = fma(u, h, c1);
+                        }
+                    }
                 }
-                if constexpr (RES) r[j] = nr[j];
+            }
+            c[b][0] = total(c0);
+            c[b][1] = total(c1);
+        }
+        if constexpr (B == 2) {
+            const float4 q = grp.sum4(make_float4(c[0][0], c[0][1], c[B - 1][0], c[B - 1][1]));
+            c[0][0] = q.x; c[0][1] = q.y; c[B - 1][0] = q.z; c[B - 1][1] = q.w;
+        } else {
+            const float2 q = grp.sum2(make_float2(c[0][0], c[0][1]));
+            c[0][0] = q.x; c[0][1] = q.y;
+        }
+#pragma unroll
+        for (int b = 0; b < B; ++b) {
+            if (row + b >= p.M) break;
+            const float m0 = -c[b][0] * inv_k, m1 = -c[b][1] * inv_k;
+            __nv_bfloat16* dst = p.dx + (row + b) * K;   // outside the access loop, as the pointers below: no spills
+            const char* xp = xs.row(stage * B + b, row + b);
+            const char* yp = ys.row(stage * B + b, row + b);
+            const char* rp = RES ? rs.row(stage * B + b, row + b) : nullptr;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const int col = (t + j * G) * W;
+                if (col < K) {
+                    // read again: cheaper than xhat and t in registers
+                    const Pack<W> px = xs.at(xp, j), py = ys.at(yp, j);
+                    Pack<W> o, r;
+                    if constexpr (RES) r = rs.at(rp, j);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const T h = mul(add(value<W>(px, i), all<T>(-mean[b])), all<T>(rstd[b]));
+                        const T d = fma(h, all<T>(m1), fma(value<W>(py, i), value<W>(w[j], i), all<T>(m0)));
+                        if constexpr (RES) o.w[i] = rounded(fma(d, all<T>(rstd[b]), value<W>(r, i)));
+                        else o.w[i] = rounded(mul(d, all<T>(rstd[b])));
+                    }
+                    store_pack<W>(dst + col, o);
+                }
             }
         }
-        if constexpr (AHEAD) fetch(row + step);
-        const float2 c = grp.sum2(make_float2(total(c0), total(c1)));
-        const T m0 = all<T>(-c.x * inv_k), m1 = all<T>(-c.y * inv_k), out_scale = all<T>(rstd);
-#pragma unroll
-        for (int j = 0; j < V; ++j) {
-            const int col = (t + j * G) * W;
-            if (col < K) {
-                Pack<W> o;
-#pragma unroll
-                for (int i = 0; i < N; ++i) {
-                    const T d = fma(xh[j][i], m1, add(tv[j][i], m0));
-                    if constexpr (RES) o.w[i] = rounded(fma(d, out_scale, value<W>(r[j], i)));
-                    else o.w[i] = rounded(mul(d, out_scale));
-                }
-                store_pack<W>(p.dx + row * K + col, o);
-            }
-        }
-        if constexpr (!AHEAD) fetch(row + step);
+        if (++stage == DEPTH) stage = 0;
     }
+    cp_async_wait<0>();
     // column sums of the CTA's groups, added in the groups' order
     float* out = p.partial + (int64_t)blockIdx.x * 2 * K;
+    float* cols = reinterpret_cast<float*>(rows_smem);   // [R][2][K]
+    if (R > 1) __syncthreads();
     float* to = R == 1 ? out : cols + (size_t)g * 2 * K;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -442,7 +599,7 @@ __global__ void __launch_bounds__(THREADS, 1) layernorm_backward_kernel(const No
 // rows wider than the registers hold: dx by one CTA per row, then the column sums by a second read
 template <bool RES>
 __global__ void __launch_bounds__(kMaxGroupThreads) layernorm_backward_wide_kernel(const NormBwdArgs p) {
-    __shared__ float2 red_all[64];
+    __shared__ __align__(16) float2 red_all[128];
     const int64_t row = blockIdx.x;
     Group grp{red_all, (int)blockDim.x, 1};
     const int K = p.K, T = blockDim.x;
@@ -529,8 +686,39 @@ int launch_norm(NormArgs p, cudaStream_t st) {
     return check_launch("layernorm");
 }
 
-// Accesses per thread: few rows (fewer than fill the device twice) take one wide access per thread, for latency (8 x 7168:
-// 7.3 us with four, FEW_US with one); many rows two to eight, for fewer barriers and reductions per byte.
+// Groups per CTA and shared memory of the kernel that walks rows
+struct RowsShape {
+    int G, R, slot_bytes, smem;
+};
+constexpr int kRowsSmem = 200 * 1024;
+template <int W, int V, int DEPTH>
+RowsShape rows_shape(int K, int arrays, int threads, int column_floats) {
+    RowsShape s;
+    s.G = group_threads((K + W - 1) / W, V);
+    // W = 8: whole accesses; otherwise the granules that cover a row at any offset
+    s.slot_bytes = W == 8 ? K * 2 : (2 * K + 30 + 15) / 16 * 16;
+    s.R = s.G == 32 ? threads / 32 : min(15, threads / s.G);   // hardware barriers 1..15; a one-warp group needs none
+    const int per_group = max(DEPTH * arrays * s.slot_bytes, column_floats * 4);
+    s.R = max(1, min(s.R, kRowsSmem / per_group));
+    s.smem = s.R * per_group;
+    return s;
+}
+template <typename Kernel>
+int opt_in(Kernel kernel, bool (&done)[64], const char* what) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && done[dev]) return 0;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem) != cudaSuccess) {
+        cudaGetLastError();
+        return fail(DSV4_ERR_LAUNCH, what);
+    }
+    if (dev >= 0 && dev < 64) done[dev] = true;
+    return 0;
+}
+
+// Few rows (no more than two per SM) take one wide access per thread, for latency (8 x 7168 with the quantiser: 7.3 us with
+// four accesses, 4 us with one); more rows take four (8192 x 7168 with the residual: 121 us with one, 83-99 with two,
+// 76-82 with four).
 template <bool ADD, bool QUANT>
 int dispatch_norm(const NormArgs& p, cudaStream_t st) {
     int w = access_width(p.K, p.x, p.w, p.b, (const __nv_bfloat16*)p.res, (const __nv_bfloat16*)p.y);
@@ -538,14 +726,13 @@ int dispatch_norm(const NormArgs& p, cudaStream_t st) {
     if (QUANT && w == 2 && (reinterpret_cast<uintptr_t>(p.q) & 1)) w = 1;
     if (w == 8) {
         if (p.K <= 8192 && p.M <= 2 * sm_count()) return launch_norm<8, 1, 1024, 1, ADD, QUANT>(p, st);
-        if (p.K <= 4096) return launch_norm<8, 2, 256, 6, ADD, QUANT>(p, st);
-        if (p.K <= 8192) return launch_norm<8, 4, 256, 5, ADD, QUANT>(p, st);
-        if (p.K <= 16384) return launch_norm<8, 8, 256, 3, ADD, QUANT>(p, st);
+        if (p.K <= 16384) return launch_norm<8, 4, 512, 2, ADD, QUANT>(p, st);
     } else if (w == 2) {
-        if (p.K <= 4096) return launch_norm<2, 4, 512, 2, ADD, QUANT>(p, st);
+        if (p.K <= 8192) return launch_norm<2, 4, 1024, 1, ADD, QUANT>(p, st);
         if (p.K <= 16384) return launch_norm<2, 8, 1024, 1, ADD, QUANT>(p, st);
     } else {
         if (p.K <= 4096) return launch_norm<1, 4, 1024, 1, ADD, QUANT>(p, st);
+        if (p.K <= 8192) return launch_norm<1, 8, 1024, 1, ADD, QUANT>(p, st);
         if (p.K <= 16384) return launch_norm<1, 16, 1024, 1, ADD, QUANT>(p, st);
     }
     layernorm_wide_kernel<ADD, QUANT><<<p.M, kMaxGroupThreads, 0, st>>>(p);
@@ -556,23 +743,22 @@ constexpr int kWideParts = 64;
 // Most CTAs whose column sums the workspace has room for; a launch uses one per SM (148 on a B200).
 constexpr int kMaxParts = 160;
 
-template <int W, int V, int THREADS, bool RES, bool AHEAD>
+template <int W, int V, int B, int DEPTH, int THREADS, bool RES>
 int launch_norm_backward(NormBwdArgs p, float* dw, float* db, int parts, cudaStream_t st) {
-    p.T = group_threads((p.K + W - 1) / W, V);
-    int R = THREADS / p.T;
-    if (p.T != 32 && R > 15) R = 15;   // hardware barriers 1..15; a one-warp group needs none
-    const int smem = R > 1 ? R * 2 * p.K * 4 : 0;
     static bool opted_in[64] = {};
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (smem > 32 * 1024 && !(dev >= 0 && dev < 64 && opted_in[dev])) {
-        if (cudaFuncSetAttribute(layernorm_backward_kernel<W, V, THREADS, RES, AHEAD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 THREADS * W * V * 8) != cudaSuccess)
-            return fail(DSV4_ERR_LAUNCH, "layernorm_backward: cannot raise the dynamic shared memory limit");
-        if (dev >= 0 && dev < 64) opted_in[dev] = true;
+    if (int rc = opt_in(layernorm_backward_kernel<W, V, B, DEPTH, THREADS, RES>, opted_in, "layernorm_backward: cannot raise the dynamic shared memory limit"))
+        return rc;
+    RowsShape s = rows_shape<W, V, DEPTH * B>(p.K, RES ? 3 : 2, THREADS, 2 * p.K);
+    p.T = s.G;
+    p.slot_bytes = s.slot_bytes;
+    // few rows: rather one group on every SM than several on some
+    const int want = (int)max((int64_t)1, ((int64_t)p.M + (int64_t)parts * B - 1) / ((int64_t)parts * B));
+    if (s.R > want) {
+        s.smem = s.smem / s.R * want;
+        s.R = want;
     }
-    const int grid = (int)min((int64_t)parts, ((int64_t)p.M + R - 1) / R);
-    layernorm_backward_kernel<W, V, THREADS, RES, AHEAD><<<grid, R * p.T, smem, st>>>(p);
+    const int grid = (int)min((int64_t)parts, ((int64_t)p.M + s.R * B - 1) / (s.R * B));
+    layernorm_backward_kernel<W, V, B, DEPTH, THREADS, RES><<<grid, s.R * s.G, s.smem, st>>>(p);
     if (int rc = check_launch("layernorm_backward")) return rc;
     layernorm_column_sum_kernel<<<(2 * p.K + 31) / 32, 256, 0, st>>>(p.partial, grid, p.K, dw, db);
     return check_launch("layernorm_backward");
@@ -582,16 +768,16 @@ template <bool RES>
 int dispatch_norm_backward(const NormBwdArgs& p, float* dw, float* db, int parts, cudaStream_t st) {
     const int w = access_width(p.K, p.x, p.dy, p.w, (const __nv_bfloat16*)p.dx, p.dres);
     if (w == 8) {
-        if (p.K <= 7168) return launch_norm_backward<8, 1, 896, RES, true>(p, dw, db, parts, st);
-        if (p.K <= 8192) return launch_norm_backward<8, 1, 1024, RES, true>(p, dw, db, parts, st);
-        if (p.K <= 16384) return launch_norm_backward<8, 4, 512, RES, true>(p, dw, db, parts, st);
+        if (p.K <= 8192) return launch_norm_backward<8, 2, 2, 2, 512, RES>(p, dw, db, parts, st);
+        if (p.K <= 16384) return launch_norm_backward<8, 4, 1, 2, 512, RES>(p, dw, db, parts, st);
     } else if (w == 2) {
-        if (p.K <= 7168) return launch_norm_backward<2, 4, 896, RES, true>(p, dw, db, parts, st);
-        if (p.K <= 16384) return launch_norm_backward<2, 16, 512, RES, false>(p, dw, db, parts, st);
+        if (p.K <= 7168) return launch_norm_backward<2, 4, 2, 2, 896, RES>(p, dw, db, parts, st);
+        if (p.K <= 8192) return launch_norm_backward<2, 4, 2, 2, 1024, RES>(p, dw, db, parts, st);
+        if (p.K <= 16384) return launch_norm_backward<2, 16, 1, 2, 512, RES>(p, dw, db, parts, st);
     } else {
-        if (p.K <= 3584) return launch_norm_backward<1, 4, 896, RES, true>(p, dw, db, parts, st);
-        if (p.K <= 8192) return launch_norm_backward<1, 16, 512, RES, true>(p, dw, db, parts, st);
-        if (p.K <= 16384) return launch_norm_backward<1, 32, 512, RES, false>(p, dw, db, parts, st);
+        if (p.K <= 7168) return launch_norm_backward<1, 8, 2, 2, 896, RES>(p, dw, db, parts, st);
+        if (p.K <= 8192) return launch_norm_backward<1, 8, 2, 2, 1024, RES>(p, dw, db, parts, st);
+        if (p.K <= 16384) return launch_norm_backward<1, 32, 1, 2, 512, RES>(p, dw, db, parts, st);
     }
     layernorm_backward_wide_kernel<RES><<<p.M, kMaxGroupThreads, 0, st>>>(p);
     if (int rc = check_launch("layernorm_backward")) return rc;
@@ -636,7 +822,7 @@ int layernorm_backward(const void* dy, const void* x, const void* mean, const vo
     p.dres = static_cast<const __nv_bfloat16*>(dres);
     p.dx = static_cast<__nv_bfloat16*>(dx);
     p.partial = static_cast<float*>(workspace);
-    p.M = M; p.K = K; p.T = 0;
+    p.M = M; p.K = K; p.T = 0; p.slot_bytes = 0;
     float *dwf = static_cast<float*>(dw), *dbf = static_cast<float*>(db);
     return dres != nullptr ? dispatch_norm_backward<true>(p, dwf, dbf, parts, st)
                            : dispatch_norm_backward<false>(p, dwf, dbf, parts, st);
