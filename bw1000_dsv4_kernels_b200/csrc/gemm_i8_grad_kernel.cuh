@@ -34,8 +34,28 @@ struct GradParams {
     // columns that are multiples of part_blocks * 128, with zeros behind each
     int parts, part_rows, part_blocks;
     int group_m;
+    // bias gradient: column sums of blocks of rows, added up by the drain warps while the first tile is multiplied
+    const float* partial;      // [row_blocks][columns], or null
+    int row_blocks;
+    float* dbias;
     unsigned long long wait_limit_ns;
 };
+
+// 32 columns per warp, a lane per column; the blocks' sums are added in four interleaved chains, in an order that only the
+// number of blocks fixes
+__device__ __forceinline__ void sum_columns(const GradParams& p, int warp, int warps) {
+    const int columns = p.parts * p.part_rows, lane = threadIdx.x & 31;
+    for (int c = warp * 32 + lane; c < columns; c += warps * 32) {
+        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        int b = 0;
+        for (; b + 4 <= p.row_blocks; b += 4) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) s[j] += __ldcg(p.partial + (int64_t)(b + j) * columns + c);
+        }
+        for (; b < p.row_blocks; ++b) s[0] += __ldcg(p.partial + (int64_t)b * columns + c);
+        p.dbias[c] = (s[0] + s[1]) + (s[2] + s[3]);
+    }
+}
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kFusedThreads, 1)
 gemm_i8_grad_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmW, const GradParams p) {
@@ -86,6 +106,7 @@ gemm_i8_grad_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     if (warp == 0) {
         // ---------------- TMA producer (both CTAs) ----------------
         if (ptx::elect_one()) {
+            ptx::grid_dependency_wait();   // the digits come from the kernel before
             int stage = 0;
             uint32_t phase = 0;
             bool ok = true;
@@ -154,6 +175,8 @@ gemm_i8_grad_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
         }
     } else {
         // ---------------- drain warps (both CTAs) ----------------
+        ptx::grid_dependency_wait();
+        if (p.partial != nullptr) sum_columns(p, blockIdx.x * kFusedDrainWarps + warp - 2, gridDim.x * kFusedDrainWarps);
         const int quarter = warp & 3, turn = (warp - 2) >> 2;
         uint32_t* stage = reinterpret_cast<uint32_t*>(smem + L::kTransposeOff + (warp - 2) * kBlockBytes);
         uint32_t acc_phase = 0;
@@ -163,7 +186,7 @@ gemm_i8_grad_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
             int mt, kt;
             order.at(t, mt, kt);
             const int row0 = mt * 256 + (int)rank * 128 + quarter * 32, rows = min(32, p.M - row0);
-            const float s = lane < rows ? digit_scale(__uint_as_float(__ldg(p.row_top + row0 + lane))) : 0.0f;
+            const float s = lane < rows ? digit_scale(__uint_as_float(__ldcg(p.row_top + row0 + lane))) : 0.0f;
             __syncwarp();
             if (!ptx::mbar_wait_bounded(acc_full_bar, acc_phase, p.wait_limit_ns) || *abort_flag) {
                 report_wait_failure(kWaitAccFull);

@@ -390,7 +390,7 @@ int launch_fused_pair(const GemmArgs& a, Params p, cudaStream_t st) {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = overlap_previous_kernel() ? 1 : 0;
+    cfg.numAttrs = overlap_previous_kernel() || a.follows ? 1 : 0;
     const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_fused_pair_kernel<EPI, ACT>, tmA, tmB, p);
     if (err != cudaSuccess) {
         cudaGetLastError();  // clear the sticky launch error
@@ -635,8 +635,10 @@ int gemm_i8_gradient(const GradientArgs& a, cudaStream_t st) {
     if (pairs <= 0) return fail(DSV4_ERR_LAUNCH, "w8a8 backward: no CUDA device");
     if (tiles > INT32_MAX) return fail(DSV4_ERR_ARG, "w8a8 backward: too many tiles");
     if (tiles < pairs) pairs = (int)tiles;
-    gemm_i8_grad_kernel<<<2 * pairs, kFusedThreads, L::kDynamic, st>>>(tmD, tmW, p);
-    return check_launch("w8a8 backward");
+    p.partial = a.partial;
+    p.row_blocks = a.row_blocks;
+    p.dbias = a.dbias;
+    return launch_after(gemm_i8_grad_kernel, dim3(2 * pairs), dim3(kFusedThreads), L::kDynamic, st, "w8a8 backward", tmD, tmW, p);
 }
 
 // ------------------------------------------------------------------------------------

@@ -12,6 +12,30 @@ int fail(int code, const char* msg);
 // cudaGetLastError() after a launch; records "<what>: <cuda error string>" on failure.
 int check_launch(const char* what);
 
+#ifdef __CUDACC__
+// Launches a kernel that may start while the one before it on the stream still runs (programmatic dependent launch); it
+// has to wait (griddepcontrol.wait) before it touches anything that kernel, or one before it, reads or writes.
+template <typename... P, typename... A>
+int launch_after(void (*kernel)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, const char* what, const A&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+    if (err != cudaSuccess) {
+        cudaGetLastError();  // clear the sticky launch error
+        return fail(DSV4_ERR_LAUNCH, what);
+    }
+    return check_launch(what);
+}
+#endif
+
 // ---- launchers implemented in rowwise_quant.cu -----------------------------------
 int ptq(const void* x, void* q, void* s, int M, int K, int64_t ldx, cudaStream_t st);
 int ptgq(const void* x, void* q, void* s, int M, int K, int gs, cudaStream_t st);
@@ -50,6 +74,7 @@ struct GemmArgs {
     int act = 0;                   // enum Activation in activations.cuh
     unsigned* row_top = nullptr;   // gradient epilogues (3 linear, 4 gated; resid is the incoming gradient, C is fp32)
     int up_col = 0;                // gated gradient: first column of the ups in C
+    bool follows = false;          // launched to overlap the kernel before it, whatever the thread's option says
     // Test hook, zero through every public entry point: the tile producers of the launch issue no
     // loads and every bounded wait gives up after test_wait_limit_ns, so the kernel's give-up path runs.
     int test_withhold_loads = 0;
@@ -62,6 +87,9 @@ struct GradientArgs {
     const void* W;              // int8 [parts * part_rows, K]
     void* dx;                   // bf16 [M, K]
     int M, K, parts, part_rows, part_pitch;   // part_pitch: multiple of 128, zeros behind part_rows
+    const float* partial;       // null, or [row_blocks][parts * part_rows]: column sums of blocks of rows
+    int row_blocks;
+    float* dbias;               // their sums
 };
 int gemm_i8_gradient(const GradientArgs& a, cudaStream_t st);
 int scale_convert(const void* acc, const void* sa, const void* sb, void* out, int M, int N,

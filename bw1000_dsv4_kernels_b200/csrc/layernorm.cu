@@ -449,6 +449,7 @@ __global__ void __launch_bounds__(THREADS, 1) layernorm_backward_kernel(const No
     constexpr int N = Vals<W>::kN, kArrays = RES ? 3 : 2;
     __shared__ __align__(16) float2 red_all[15 * 128];
     extern __shared__ __align__(16) char rows_smem[];   // the groups' row slots; at the end their column sums
+    ptx::grid_launch_dependents();   // the column sums' kernel
     const int G = p.T, R = blockDim.x / G, g = threadIdx.x / G, t = threadIdx.x - g * G, K = p.K;
     Group grp{red_all + (G == 32 ? 0 : 128 * g), G, 1 + g};
     char* mine = rows_smem + (size_t)g * DEPTH * B * kArrays * p.slot_bytes;
@@ -638,11 +639,12 @@ __global__ void __launch_bounds__(256) layernorm_wide_columns_kernel(const NormB
 __global__ void __launch_bounds__(256) layernorm_column_sum_kernel(const float* __restrict__ partial, int parts, int K,
                                                                    float* __restrict__ dw, float* __restrict__ db) {
     __shared__ float sh[8][33];
+    ptx::grid_dependency_wait();   // may have started while the CTAs still write their shares
     const int col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
     float v = 0.0f;
     if (col < 2 * K) {
 #pragma unroll 8
-        for (int i = slice; i < parts; i += 8) v += partial[(int64_t)i * 2 * K + col];
+        for (int i = slice; i < parts; i += 8) v += __ldcg(partial + (int64_t)i * 2 * K + col);
     }
     sh[slice][threadIdx.x & 31] = v;
     __syncthreads();
@@ -760,8 +762,8 @@ int launch_norm_backward(NormBwdArgs p, float* dw, float* db, int parts, cudaStr
     const int grid = (int)min((int64_t)parts, ((int64_t)p.M + s.R * B - 1) / (s.R * B));
     layernorm_backward_kernel<W, V, B, DEPTH, THREADS, RES><<<grid, s.R * s.G, s.smem, st>>>(p);
     if (int rc = check_launch("layernorm_backward")) return rc;
-    layernorm_column_sum_kernel<<<(2 * p.K + 31) / 32, 256, 0, st>>>(p.partial, grid, p.K, dw, db);
-    return check_launch("layernorm_backward");
+    return launch_after(layernorm_column_sum_kernel, dim3((2 * p.K + 31) / 32), dim3(256), 0, st, "layernorm_backward", p.partial, grid,
+                        p.K, dw, db);
 }
 
 template <bool RES>

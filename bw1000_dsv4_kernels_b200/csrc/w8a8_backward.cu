@@ -6,7 +6,8 @@
 //
 // Three steps: the forward's GEMM with a gradient epilogue writes dz in fp32 and each row's largest |dz * sb|
 // (gemm_i8_epilogues.cuh); split_gradient_kernel puts dz * sb into two int8 digits per element and sums the columns;
-// gemm_i8_grad_kernel multiplies the digits with W.  The codes and scales of the forward are all that has to be kept for
+// gemm_i8_grad_kernel multiplies the digits with W and adds the column sums up.  Each kernel is launched to start while the
+// one before it drains (333 x 1001 x 1040 with bias: 41 us as five launches in a row).  The codes and scales of the forward are all that has to be kept for
 // it.  Without an activation dz is dy itself: the first step is a pass over dy for the rows' largest magnitudes.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
@@ -15,6 +16,7 @@
 #include "activations.cuh"
 #include "gradient_digits.cuh"
 #include "launch_common.h"
+#include "sm100_ptx.cuh"
 #include "w8a8_arith.cuh"
 
 namespace w8a8 {
@@ -22,14 +24,15 @@ namespace {
 
 __device__ __forceinline__ unsigned top_bits(unsigned top, float v) { return max(top, __float_as_uint(v) & 0x7fffffffu); }
 
-// eight consecutive gradients of one row as fp32; those at or beyond `left` are zero
+// eight consecutive gradients of one row as fp32; those at or beyond `left` are zero.  What the kernel before wrote is read
+// past L1: this kernel may have started before that one ended.
 __device__ __forceinline__ void load8(const float* p, int left, bool vec, float (&v)[8]) {
     if (vec && left >= 8) {
-        const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+        const float4 a = __ldcg(reinterpret_cast<const float4*>(p)), b = __ldcg(reinterpret_cast<const float4*>(p + 4));
         v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < left ? p[j] : 0.0f;
+        for (int j = 0; j < 8; ++j) v[j] = j < left ? __ldcg(p + j) : 0.0f;
     }
 }
 __device__ __forceinline__ void load8(const __nv_bfloat16* p, int left, bool vec, float (&v)[8]) {
@@ -43,10 +46,17 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, int left, bool vec
     }
 }
 
+__global__ void __launch_bounds__(256) clear_row_top_kernel(unsigned* row_top, int M) {
+    ptx::grid_launch_dependents();
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < M) row_top[i] = 0u;
+}
+
 // row_top[row] = largest |dy * sb| of the row, as float bits: one CTA per row
 __global__ void __launch_bounds__(256) row_top_kernel(const __nv_bfloat16* dy, int64_t ldy, const float* __restrict__ sb, int N,
                                                       bool vec, unsigned* row_top) {
     __shared__ unsigned part[8];
+    ptx::grid_launch_dependents();
     const __nv_bfloat16* row = dy + (int64_t)blockIdx.x * ldy;
     unsigned top = 0;
     for (int c = threadIdx.x * 8; c < N; c += 256 * 8) {
@@ -84,6 +94,8 @@ __global__ void __launch_bounds__(32 * kSplitWarps) split_gradient_kernel(const 
                                                                           Columns cols, bool vec, int8_t* digits,
                                                                           float* partial) {
     __shared__ float sums[SUM ? kSplitWarps : 1][SUM ? 264 : 1];
+    ptx::grid_launch_dependents();
+    ptx::grid_dependency_wait();   // dz and the rows' tops come from the kernel before
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const int c = blockIdx.x * 256 + lane * 8;             // column with padding
     const int pitch = cols.pitch(), part = c >= cols.part_pitch ? 1 : 0, local = c - part * cols.part_pitch;
@@ -97,7 +109,7 @@ __global__ void __launch_bounds__(32 * kSplitWarps) split_gradient_kernel(const 
         const int r = r0 + i * kSplitWarps;
         const bool ok = r < M;
         load8(dz + (int64_t)(ok ? r : 0) * ld + c, ok ? left : 0, vec, v[i]);
-        inv[i] = ok ? digit_inverse(__uint_as_float(__ldg(row_top + r))) : 0.0f;
+        inv[i] = ok ? digit_inverse(__uint_as_float(__ldcg(row_top + r))) : 0.0f;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) scale[j] = j < left ? __ldg(sb + w_row + j) : 0.0f;
@@ -136,24 +148,6 @@ __global__ void __launch_bounds__(32 * kSplitWarps) split_gradient_kernel(const 
     }
 }
 
-// column sums over the row blocks, eight slices of them, each in order: 32 columns per CTA
-__global__ void __launch_bounds__(256) gradient_column_sum_kernel(const float* __restrict__ partial, int parts, int N,
-                                                                  float* __restrict__ out) {
-    __shared__ float sh[8][33];
-    const int col = blockIdx.x * 32 + (threadIdx.x & 31), slice = threadIdx.x >> 5;
-    float v = 0.0f;
-    if (col < N)
-        for (int i = slice; i < parts; i += 8) v += partial[(int64_t)i * N + col];
-    sh[slice][threadIdx.x & 31] = v;
-    __syncthreads();
-    if (slice == 0 && col < N) {
-        float s = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) s += sh[k][threadIdx.x & 31];
-        out[col] = s;
-    }
-}
-
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 struct Layout {
@@ -182,14 +176,11 @@ int split(const T* dz, int64_t ld, const BackwardArgs& a, const Layout& l, const
           float* partial, cudaStream_t st) {
     const bool vec = (ld * sizeof(T)) % 16 == 0 && aligned16(dz);
     const dim3 grid((l.cols.pitch() + 255) / 256, l.row_blocks);
-    if (a.dbias != nullptr) {
-        split_gradient_kernel<T, true><<<grid, 32 * kSplitWarps, 0, st>>>(dz, ld, a.sb, row_top, a.M, l.cols, vec, digits, partial);
-        if (int rc = check_launch("w8a8 backward")) return rc;
-        gradient_column_sum_kernel<<<(a.N + 31) / 32, 256, 0, st>>>(partial, l.row_blocks, a.N, a.dbias);
-    } else {
-        split_gradient_kernel<T, false><<<grid, 32 * kSplitWarps, 0, st>>>(dz, ld, a.sb, row_top, a.M, l.cols, vec, digits, partial);
-    }
-    return check_launch("w8a8 backward");
+    return a.dbias != nullptr
+               ? launch_after(split_gradient_kernel<T, true>, grid, dim3(32 * kSplitWarps), 0, st, "w8a8 backward", dz, ld, a.sb,
+                              row_top, a.M, l.cols, vec, digits, partial)
+               : launch_after(split_gradient_kernel<T, false>, grid, dim3(32 * kSplitWarps), 0, st, "w8a8 backward", dz, ld, a.sb,
+                              row_top, a.M, l.cols, vec, digits, partial);
 }
 
 }  // namespace
@@ -208,15 +199,14 @@ int w8a8_backward(const BackwardArgs& a, void* workspace, cudaStream_t st) {
     const __nv_bfloat16* dy = static_cast<const __nv_bfloat16*>(a.dy);
     if (recompute) {
         float* dz = reinterpret_cast<float*>(ws + l.dz);
-        if (cudaMemsetAsync(row_top, 0, (size_t)a.M * 4, st) != cudaSuccess) {
-            check_launch("w8a8 backward");
-            return DSV4_ERR_LAUNCH;
-        }
+        clear_row_top_kernel<<<(a.M + 255) / 256, 256, 0, st>>>(row_top, a.M);
+        if (int rc = check_launch("w8a8 backward")) return rc;
         GemmArgs g{};
         g.A = a.A; g.B = a.B; g.sa = a.sa; g.sb = a.sb; g.C = dz;
         g.M = a.M; g.N = l.cols.part_rows; g.K = a.K; g.E = 1; g.ldc = l.cols.pitch(); g.sa_groups = 1;
         g.epilogue = a.gated ? 4 : 3; g.bias = a.bias; g.resid = a.dy; g.ldr = a.ldy; g.act = a.act; g.row_top = row_top;
         g.up_col = l.cols.part_pitch;
+        g.follows = true;
         if (int rc = gemm_i8(g, st)) return rc;
         if (int rc = split(dz, (int64_t)l.cols.pitch(), a, l, row_top, digits, partial, st)) return rc;
     } else {
@@ -227,6 +217,7 @@ int w8a8_backward(const BackwardArgs& a, void* workspace, cudaStream_t st) {
     GradientArgs d;
     d.digits = digits; d.row_top = row_top; d.W = a.B; d.dx = a.dx;
     d.M = a.M; d.K = a.K; d.parts = l.cols.parts; d.part_rows = l.cols.part_rows; d.part_pitch = l.cols.part_pitch;
+    d.partial = a.dbias != nullptr ? partial : nullptr; d.row_blocks = l.row_blocks; d.dbias = a.dbias;
     return gemm_i8_gradient(d, st);
 }
 
