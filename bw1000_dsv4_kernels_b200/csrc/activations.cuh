@@ -85,7 +85,8 @@ __device__ __forceinline__ float2 act_value_slope2(float2 z, float2& slope) {
     }
     if constexpr (ACT == kActGeluTanh || ACT == kActSilu) {
         // d(z sigmoid(c)) = p + z p (1 - p) c', with c' = 1 for SiLU
-        const float2 z2 = __fmul2_rn(z, z);
+        float2 z2 = __fmul2_rn(z, z);
+        z2 = make_float2(fminf(z2.x, 1e30f), fminf(z2.y, 1e30f));   // finite: 1 - p is zero long before
         const bool tanh_form = ACT == kActGeluTanh;
         const float2 p = tanh_form ? sigmoid2(__ffma2_rn(__fmul2_rn(z2, splat2(kGeluCubic)), z, z), kGeluTanhC) : sigmoid2(z, 1.0f);
         const float2 v = __fmul2_rn(z, p);

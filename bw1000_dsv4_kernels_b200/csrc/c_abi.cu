@@ -343,7 +343,7 @@ static int backward_entry(const char* op, bool gated, const void* dy, int64_t ld
     if (act != DSV4_ACT_NONE && (A == nullptr || sa == nullptr)) return bad("null pointer A or sa");
     if ((reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(B) & 15)) return bad("A and B must be 16-byte aligned");
     if (ldy < (gated ? N / 2 : N)) return bad("gradient row stride smaller than its row");
-    if ((int64_t)2 * M > INT32_MAX) return bad("too many rows");
+    if (M > (1 << 29)) return bad("too many rows");
     if (workspace_bytes < w8a8_backward_workspace(M, N, gated, act != DSV4_ACT_NONE, dbias != nullptr) ||
         (reinterpret_cast<uintptr_t>(workspace) & 15))
         return bad("the workspace is smaller than dsv4_w8a8_backward_workspace or not 16-byte aligned");

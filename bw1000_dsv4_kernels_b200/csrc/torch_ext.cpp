@@ -18,7 +18,8 @@
 //   * silu ops accept row-strided 2-D views, so the halves of a packed gate_up work;
 //   * new names: w8a8_gemm (alias), w8a8_gemm_i32, scale_convert,
 //     per_token_group_quant_int8, silu_mul_masked_quant, grouped_gemm, moe_segments,
-//     gather_rows, device_status;
+//     gather_rows, device_status; w8a8_linear, w8a8_gated, layernorm (and the add_ / _quant forms) with their
+//     _backward operators;
 //   * flash_mla_decode is not part of the W8A8 path and is not provided.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>

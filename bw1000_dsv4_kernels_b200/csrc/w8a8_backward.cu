@@ -6,9 +6,10 @@
 //
 // Three steps: the forward's GEMM with a gradient epilogue writes dz in fp32 and each row's largest |dz * sb|
 // (gemm_i8_epilogues.cuh); split_gradient_kernel puts dz * sb into two int8 digits per element and sums the columns;
-// gemm_i8_grad_kernel multiplies the digits with W and adds the column sums up.  Each kernel is launched to start while the
-// one before it drains (333 x 1001 x 1040 with bias: 41 us as five launches in a row).  The codes and scales of the forward are all that has to be kept for
-// it.  Without an activation dz is dy itself: the first step is a pass over dy for the rows' largest magnitudes.
+// gemm_i8_grad_kernel multiplies the digits with W and adds the column sums up.  The codes and scales of the forward are
+// all that has to be kept for it.  Each kernel is launched to start while the one before it drains: 333 x 1001 x 1040 with
+// bias takes 34 us, 41 us as five launches in a row.  Without an activation dz is dy itself: the first step is a pass over
+// dy for the rows' largest magnitudes.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <cstdint>
@@ -97,11 +98,14 @@ __global__ void __launch_bounds__(32 * kSplitWarps) split_gradient_kernel(const 
     ptx::grid_launch_dependents();
     ptx::grid_dependency_wait();   // dz and the rows' tops come from the kernel before
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int c = blockIdx.x * 256 + lane * 8;             // column with padding
-    const int pitch = cols.pitch(), part = c >= cols.part_pitch ? 1 : 0, local = c - part * cols.part_pitch;
+    // one grid dimension for blocks of rows and of columns: there can be more than 65535 of the first
+    const int pitch = cols.pitch(), col_blocks = (pitch + 255) / 256;
+    const int row_block = blockIdx.x / col_blocks, col_block = blockIdx.x - row_block * col_blocks;
+    const int c = col_block * 256 + lane * 8;              // column with padding
+    const int part = c >= cols.part_pitch ? 1 : 0, local = c - part * cols.part_pitch;
     const int left = c < pitch ? cols.part_rows - local : 0, w_row = part * cols.part_rows + local;
     const int64_t plane = (int64_t)M * pitch;
-    const int r0 = blockIdx.y * kSplitRows + warp;
+    const int r0 = row_block * kSplitRows + warp;
     constexpr int kRows = kSplitRows / kSplitWarps;
     float v[kRows][8], inv[kRows], scale[8], sum[8] = {};
 #pragma unroll
@@ -138,12 +142,12 @@ __global__ void __launch_bounds__(32 * kSplitWarps) split_gradient_kernel(const 
 #pragma unroll
         for (int j = 0; j < 8; ++j) sums[warp][lane * 8 + j] = sum[j];
         __syncthreads();
-        const int col = blockIdx.x * 256 + threadIdx.x, p2 = col >= cols.part_pitch ? 1 : 0, l2 = col - p2 * cols.part_pitch;
+        const int col = col_block * 256 + threadIdx.x, p2 = col >= cols.part_pitch ? 1 : 0, l2 = col - p2 * cols.part_pitch;
         if (col < pitch && l2 < cols.part_rows) {
             float t = 0.0f;
 #pragma unroll
             for (int w = 0; w < kSplitWarps; ++w) t += sums[w][threadIdx.x];
-            partial[(int64_t)blockIdx.y * cols.parts * cols.part_rows + p2 * cols.part_rows + l2] = t;
+            partial[(int64_t)row_block * cols.parts * cols.part_rows + p2 * cols.part_rows + l2] = t;
         }
     }
 }
@@ -175,7 +179,9 @@ template <typename T>
 int split(const T* dz, int64_t ld, const BackwardArgs& a, const Layout& l, const unsigned* row_top, int8_t* digits,
           float* partial, cudaStream_t st) {
     const bool vec = (ld * sizeof(T)) % 16 == 0 && aligned16(dz);
-    const dim3 grid((l.cols.pitch() + 255) / 256, l.row_blocks);
+    const int64_t blocks = (int64_t)((l.cols.pitch() + 255) / 256) * l.row_blocks;
+    if (blocks > INT32_MAX) return fail(DSV4_ERR_ARG, "w8a8 backward: too many rows");
+    const dim3 grid((unsigned)blocks);
     return a.dbias != nullptr
                ? launch_after(split_gradient_kernel<T, true>, grid, dim3(32 * kSplitWarps), 0, st, "w8a8 backward", dz, ld, a.sb,
                               row_top, a.M, l.cols, vec, digits, partial)

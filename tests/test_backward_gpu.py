@@ -165,6 +165,24 @@ def test_empty_batches_and_refusals(ext):
         ext.w8a8_gated_backward(dy[:, :16], a, w, sa, sw, None, "none")
 
 
+def test_more_rows_than_a_grid_dimension_of_row_blocks(ext):
+    """2.1 million rows: 65536 blocks of 32"""
+    m, n, k = 65536 * 32 + 5, 16, 16
+    (w, sw) = ref.weight(n, k, 2)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    a = torch.randint(-127, 128, (m, k), generator=g, device="cuda", dtype=torch.int8)
+    sa = torch.rand((m, 1), generator=g, device="cuda") * 0.02
+    dy = torch.randn((m, n), generator=g, device="cuda").to(torch.bfloat16)
+    b = ref.bf16((n,), 3)
+    dx, db = ext.w8a8_linear_backward(dy, a, *(t.cuda() for t in (w,)), sa, sw.cuda(), b.cuda(), "silu")
+    pick = torch.tensor([0, 1, 31, 32, 65535 * 32 - 1, 65535 * 32, 65536 * 32 - 1, 65536 * 32, m - 1])
+    want = ref.linear_backward(dy.cpu()[pick], a.cpu()[pick], sa.cpu()[pick], w, sw, b, "silu")[0]
+    assert ((dx.cpu()[pick].double() - want).norm(dim=1) <= 4e-3 * want.norm(dim=1)).all()
+    dz = (dy.double() * ref.dact((a.double() @ w.cuda().double().T) * sa.double() * sw.cuda().double() + b.cuda().double(), "silu"))
+    # 65537 block sums in four chains of 16384 additions, 32 rows each
+    assert ((db.double() - dz.sum(0)).abs() <= U * (16384 + 60) * dz.abs().sum(0)).all()
+
+
 def test_two_runs_other_streams_and_captured_replays(ext):
     m, i, k = 200, 136, 272
     (a, sa), (w, sw) = ref.tokens(m, k, 1), ref.weight(2 * i, k, 2)
