@@ -77,8 +77,18 @@ __device__ __forceinline__ float fma(float a, float b, float c) { return __fmaf_
 __device__ __forceinline__ float2 fma(float2 a, float2 b, float2 c) { return __ffma2_rn(a, b, c); }
 __device__ __forceinline__ float total(float a) { return a; }
 __device__ __forceinline__ float total(float2 a) { return __fadd_rn(a.x, a.y); }
-__device__ __forceinline__ float top_of(float t, float a) { return fmaxf(t, fabsf(a)); }
-__device__ __forceinline__ float top_of(float t, float2 a) { return max3_abs(t, a.x, a.y); }
+// larger magnitude; a NaN stays one and becomes the row's scale (codes alone would turn it into a number)
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float top_of(float t, float a) { return max_nan(t, fabsf(a)); }
+__device__ __forceinline__ float top_of(float t, float2 a) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(t), "f"(fabsf(a.x)), "f"(fabsf(a.y)));
+    return d;
+}
 template <typename T>
 __device__ __forceinline__ T all(float v) {
     if constexpr (sizeof(T) == 8) return splat2(v);
@@ -126,7 +136,7 @@ struct Group {
         return reduce(v, [](float a, float b) { return a + b; });
     }
     __device__ __forceinline__ float max(float v) {
-        return reduce(v, [](float a, float b) { return fmaxf(a, b); });
+        return reduce(v, [](float a, float b) { return max_nan(a, b); });
     }
     // Four sums at once: halves of the warp keep two of the values each, quarters one, so that thirteen shuffles do what
     // forty would.  Entries of warps that the group does not have must be zero (clear4).
@@ -242,6 +252,11 @@ __device__ __forceinline__ void store_codes(int8_t* q, const T (&y)[N], float in
     } else {
         *q = (int8_t)(quant_rn_lowbyte(y[0], inv) & 0xffu);
     }
+}
+
+__device__ __forceinline__ void scale_of(float top, float& scale, float& inv) {
+    scale_from_amax(top, scale, inv);
+    if (isnan(top)) scale = top;
 }
 
 __device__ __forceinline__ float rstd_of(float sumsq, int K, float eps) {
@@ -369,7 +384,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) layernorm_kernel(const NormArgs
             }
         }
         float scale, inv;
-        scale_from_amax(grp.max(top), scale, inv);
+        scale_of(grp.max(top), scale, inv);
         if (t == 0) p.s[row] = scale;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
@@ -417,8 +432,8 @@ __global__ void __launch_bounds__(kMaxGroupThreads) layernorm_wide_kernel(const 
         for (int c = threadIdx.x; c < K; c += T) p.y[row * K + c] = __float2bfloat16_rn(norm(c));
     } else {
         float top = 0.0f, scale, inv;
-        for (int c = threadIdx.x; c < K; c += T) top = fmaxf(top, fabsf(norm(c)));
-        scale_from_amax(grp.max(top), scale, inv);
+        for (int c = threadIdx.x; c < K; c += T) top = top_of(top, norm(c));
+        scale_of(grp.max(top), scale, inv);
         if (threadIdx.x == 0) p.s[row] = scale;
         for (int c = threadIdx.x; c < K; c += T) p.q[row * K + c] = (int8_t)quant_rn(norm(c), inv);
     }
@@ -684,7 +699,7 @@ int launch_norm(NormArgs p, cudaStream_t st) {
     p.T = group_threads((p.K + W - 1) / W, V);
     // narrow rows share a CTA of up to 256 threads: one row each, at most 8 rows
     const int R = p.T >= 256 ? 1 : 256 / p.T;
-    layernorm_kernel<W, V, THREADS, CTAS, ADD, QUANT><<<(p.M + R - 1) / R, R * p.T, 0, st>>>(p);
+    layernorm_kernel<W, V, THREADS, CTAS, ADD, QUANT><<<(unsigned)(((int64_t)p.M + R - 1) / R), R * p.T, 0, st>>>(p);
     return check_launch("layernorm");
 }
 

@@ -291,7 +291,7 @@ DSV4_API int launch_w8a8_gated_backward(const void* dh, int64_t ldh, const void*
  * mean, rstd fp32 [M] of a's rows (rstd = 1/sqrt(var + eps), population variance); y = (a - mean)*rstd*w + b.
  * w, b bf16 [N].  Statistics are those of the row as it is stored in bf16, which is what the backward pass reads.
  * launch_layernorm stores y as bf16; launch_layernorm_quant stores the codes and scales of launch_ptq on the
- * unrounded y.  N must be positive. */
+ * unrounded y (a row of y with a NaN gets a NaN as its scale).  N must be positive. */
 DSV4_API int launch_layernorm(void* res, const void* x, const void* w, const void* b, void* y, void* mean, void* rstd,
                        int M, int N, float eps, dsv4_stream_t stream);
 DSV4_API int launch_layernorm_quant(void* res, const void* x, const void* w, const void* b, void* q, void* s, void* mean,

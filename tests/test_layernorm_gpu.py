@@ -210,3 +210,21 @@ def test_other_stream_and_captured_replay(ext):
         want = ext.layernorm_backward(dy, x, eager[1], eager[2], w)
         torch.cuda.synchronize()
         assert torch.equal(y, eager[0]) and all(torch.equal(p, q) for p, q in zip(want, grads))
+
+
+@pytest.mark.parametrize("m,k", [(12, 1), (12, 33), (12, 64), (600, 2048), (12, 4104), (3, 16392)])
+def test_a_row_with_nan_or_infinity_keeps_it(ext, m, k):
+    """statistics, bf16 rows and scales of such rows are not finite, and no other row notices"""
+    x, (w, b) = rows(m, k, 1), weights(k, 2)
+    clean = x.clone()
+    x[1, k // 2], x[2, 0] = float("nan"), float("inf")
+    y, mean, rstd = ext.layernorm(*(t.cuda() for t in (x, w, b)), EPS)
+    q, s, _, _ = ext.layernorm_quant(*(t.cuda() for t in (x, w, b)), EPS)
+    y0 = ext.layernorm(*(t.cuda() for t in (clean, w, b)), EPS)[0]
+    q0, s0, _, _ = ext.layernorm_quant(*(t.cuda() for t in (clean, w, b)), EPS)
+    fine = [r for r in range(m) if r not in (1, 2)]
+    for t in (y[1:3], rstd[1:3], s[1:3]):
+        assert t.isnan().all()
+    assert torch.equal(y[fine], y0[fine]) and torch.equal(q[fine], q0[fine]) and torch.equal(s[fine], s0[fine])
+    b[k - 1] = float("nan")
+    assert ext.layernorm_quant(*(t.cuda() for t in (clean, w, b)), EPS)[1].isnan().all()
