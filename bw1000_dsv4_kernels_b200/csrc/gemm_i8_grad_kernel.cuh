@@ -41,19 +41,26 @@ struct GradParams {
     unsigned long long wait_limit_ns;
 };
 
-// 32 columns per warp, a lane per column; the blocks' sums are added in four interleaved chains, in an order that only the
-// number of blocks fixes
+// 32 columns per warp, a lane per column; the blocks' sums are added in sixteen interleaved chains (so that as many loads are
+// under way), in an order that only the number of blocks fixes
 __device__ __forceinline__ void sum_columns(const GradParams& p, int warp, int warps) {
     const int columns = p.parts * p.part_rows, lane = threadIdx.x & 31;
     for (int c = warp * 32 + lane; c < columns; c += warps * 32) {
-        float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        int b = 0;
-        for (; b + 4 <= p.row_blocks; b += 4) {
+        float s[16] = {};
+#pragma unroll 1
+        for (int b = 0; b < p.row_blocks; b += 16) {
+            float v[16];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) s[j] += __ldcg(p.partial + (int64_t)(b + j) * columns + c);
+            for (int j = 0; j < 16; ++j) v[j] = b + j < p.row_blocks ? __ldcg(p.partial + (int64_t)(b + j) * columns + c) : 0.0f;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) s[j] += v[j];
         }
-        for (; b < p.row_blocks; ++b) s[0] += __ldcg(p.partial + (int64_t)b * columns + c);
-        p.dbias[c] = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+        for (int h = 8; h > 0; h >>= 1) {
+#pragma unroll
+            for (int j = 0; j < h; ++j) s[j] += s[j + h];
+        }
+        p.dbias[c] = s[0];
     }
 }
 
