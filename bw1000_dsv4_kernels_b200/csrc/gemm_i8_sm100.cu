@@ -222,7 +222,9 @@ int launch_stream_variant(const CUtensorMap& tmW, const CUtensorMap& tmX, const 
 }
 
 // How many clusters of 2*splits CTAs of the pair streaming kernel the device can run at once (one
-// CTA per SM, a cluster inside one GPC); asked once per device and cluster size.
+// CTA per SM, a cluster inside one GPC); asked once per device and cluster size, of a kernel that has its shared memory
+// opted in (the answer is none otherwise).
+template <int EPI>
 int stream_pair_active_clusters(int splits) {
     static int cached[64][5] = {};
     int dev = 0;
@@ -240,7 +242,7 @@ int stream_pair_active_clusters(int splits) {
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_stream_pair_kernel<>, &cfg) != cudaSuccess) {
+        if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_stream_pair_kernel<EPI>, &cfg) != cudaSuccess) {
             cudaGetLastError();
             n = -1;
         }
@@ -258,7 +260,7 @@ int launch_stream_pair(const CUtensorMap& tmW, const CUtensorMap& tmX, const Par
     if (!opt_in_shared_memory(gemm_i8_stream_pair_kernel<EPI>, L::kDynamic, opted_in))
         return fail(DSV4_ERR_LAUNCH, "w8a8_gemm: cannot raise the dynamic shared memory limit");
     // a cluster must fit into one GPC: take the widest K split whose clusters all run in one wave
-    while (splits > 1 && stream_pair_active_clusters(splits) < n_tiles) --splits;
+    while (splits > 1 && stream_pair_active_clusters<EPI>(splits) < n_tiles) --splits;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(n_tiles * 2 * splits), 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
