@@ -292,6 +292,7 @@ int launch_w8a8_gemm_ld(const void* A, const void* B, const void* sa, const void
 int launch_w8a8_linear(const void* A, const void* B, const void* sa, const void* sb, const void* bias, int act,
                        const void* residual, int64_t ldr, void* C, int64_t ldc, int M, int N, int K, dsv4_stream_t stream) {
     if (act < DSV4_ACT_NONE || act > DSV4_ACT_SILU) return fail(DSV4_ERR_ARG, "w8a8_linear: unknown activation");
+    if (M > (1 << 30)) return fail(DSV4_ERR_ARG, "w8a8_linear: too many rows");
     if (residual != nullptr && ldr < N) return fail(DSV4_ERR_ARG, "w8a8_linear: residual row stride smaller than N");
     GemmArgs a{};
     a.A = A; a.B = B; a.sa = static_cast<const float*>(sa); a.sb = static_cast<const float*>(sb); a.C = C;
@@ -303,6 +304,7 @@ int launch_w8a8_linear(const void* A, const void* B, const void* sa, const void*
 int launch_w8a8_gated(const void* A, const void* B, const void* sa, const void* sb, const void* bias, int act, void* C,
                       int64_t ldc, int M, int I, int K, dsv4_stream_t stream) {
     if (act <= DSV4_ACT_NONE || act > DSV4_ACT_SILU) return fail(DSV4_ERR_ARG, "w8a8_gated: unknown activation");
+    if (M > (1 << 30)) return fail(DSV4_ERR_ARG, "w8a8_gated: too many rows");
     if (I > INT32_MAX / 2) return fail(DSV4_ERR_ARG, "w8a8_gated: 2 * I does not fit in int32");
     GemmArgs a{};
     a.A = A; a.B = B; a.sa = static_cast<const float*>(sa); a.sb = static_cast<const float*>(sb); a.C = C;

@@ -81,6 +81,8 @@ struct Params {
     int up_col;
     // fused CTA-pair kernel: rows of B per tile, gates and ups together (a multiple of 32, of 64 when gated)
     int tile_n;
+    // weight-streaming kernels with fused epilogues: tokens of a block (a multiple of 32 for CTA pairs, at most 256)
+    int block_m;
 };
 
 template <int BN, int STAGES>
@@ -91,8 +93,7 @@ struct Smem {
     static constexpr int kTilesBytes = STAGES * kStageBytes;
     // after the tiles: one copy of the tile's column scales per drain warp, barriers, tmem slot
     static constexpr int kSbOff = kTilesBytes;
-    static constexpr int kBiasOff = kSbOff + 4 * BN * 4;   // the same for the biases of the fused epilogue
-    static constexpr int kBarOff = kBiasOff + 4 * BN * 4;  // 8-byte aligned below
+    static constexpr int kBarOff = kSbOff + 4 * BN * 4;  // 8-byte aligned below
     static constexpr int kNumBars = 2 * STAGES + 8;  // stage full/empty + up to 4 accumulator full/empty pairs
     static constexpr int kTmemSlotOff = ((kBarOff + 7) & ~7) + kNumBars * 8;
     static constexpr int kAbortOff = kTmemSlotOff + 4;

@@ -21,39 +21,10 @@ namespace {
 struct Row32 {
     uint32_t w[16];
 };
-__device__ __forceinline__ void load_row32(Row32& r, const __nv_bfloat16* p, int n_left, bool vec) {
-    if (vec && n_left >= 32) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint4 q = *reinterpret_cast<const uint4*>(p + 8 * j);
-            r.w[4 * j] = q.x; r.w[4 * j + 1] = q.y; r.w[4 * j + 2] = q.z; r.w[4 * j + 3] = q.w;
-        }
-    } else {
-        const uint16_t* s = reinterpret_cast<const uint16_t*>(p);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const uint32_t lo = 2 * j < n_left ? s[2 * j] : 0u, hi = 2 * j + 1 < n_left ? s[2 * j + 1] : 0u;
-            r.w[j] = lo | (hi << 16);
-        }
-    }
+// rows of `n` elements come in whole 16-byte pieces at 16-byte aligned addresses
+__device__ __forceinline__ bool block_vector_ok(const void* base, int64_t ld, int n) {
+    return ld % 8 == 0 && (reinterpret_cast<uintptr_t>(base) & 15) == 0 && n % 8 == 0;
 }
-__device__ __forceinline__ void store_row32(__nv_bfloat16* p, const Row32& r, int n_left, bool vec) {
-    if (vec && n_left >= 32) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-            *reinterpret_cast<uint4*>(p + 8 * j) = make_uint4(r.w[4 * j], r.w[4 * j + 1], r.w[4 * j + 2], r.w[4 * j + 3]);
-    } else {
-        uint16_t* s = reinterpret_cast<uint16_t*>(p);
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (j < n_left) s[j] = (uint16_t)((j & 1) ? r.w[j >> 1] >> 16 : r.w[j >> 1] & 0xffffu);
-    }
-}
-
-__device__ __forceinline__ bool row_vector_ok(const void* base, int64_t ld) {
-    return (ld % 8 == 0) && ((reinterpret_cast<uintptr_t>(base) & 15) == 0);
-}
-__device__ __forceinline__ bool block_vector_ok(const void* base, int64_t ld, int n) { return row_vector_ok(base, ld) && n % 8 == 0; }
 
 // z of two columns.  A missing bias is -0, which leaves every product as it is: the bits of the plain epilogue.
 constexpr float kNoBias = -0.0f;
@@ -175,15 +146,6 @@ struct Cols32 {
 };
 __device__ __forceinline__ float2 two(const float4& v, int k) { return k == 0 ? make_float2(v.x, v.y) : make_float2(v.z, v.w); }
 
-// Column scales and biases of a tile -> a warp's shared copy (one CTA per tile kernel)
-__device__ __forceinline__ void stage_columns(const Params& p, float* sbs, float* bias_s, int lane, int count, int first) {
-    for (int j = lane; j < count; j += 32) {
-        const int c = first + j;
-        sbs[j] = c < p.N ? __ldg(p.sb + c) : 0.0f;
-        bias_s[j] = c < p.N && p.bias != nullptr ? __bfloat162float(p.bias[c]) : kNoBias;
-    }
-}
-
 // y of 32 columns from the accumulators of one row
 template <int ACT>
 __device__ __forceinline__ Row32 linear_values(const uint32_t (&r)[32], float sa, Cols32 sb, Cols32 bias, bool has_res,
@@ -204,32 +166,6 @@ __device__ __forceinline__ Row32 linear_values(const uint32_t (&r)[32], float sa
         }
     }
     return out;
-}
-
-// One finished accumulator of NCOLS columns (one CTA per tile kernel): this thread owns tile row `row`.
-template <int NCOLS>
-__device__ __forceinline__ void drain_linear(const Params& p, uint32_t t_lane, const float* sbs, const float* bias_s, int row,
-                                             bool row_ok, int n0, bool vec_ok) {
-    const float sa = row_ok ? __ldg(p.sa + row) : 0.0f;
-    const bool has_res = p.resid != nullptr && row_ok;
-    const bool res_vec = row_vector_ok(p.resid, p.ldr);
-#pragma unroll 1
-    for (int cc = 0; cc < NCOLS / 32; ++cc) {
-        const int n = n0 + cc * 32;
-        Row32 res = {};
-        if (has_res && n < p.N) load_row32(res, p.resid + (int64_t)row * p.ldr + n, p.N - n, res_vec);
-        uint32_t r[32];
-        __syncwarp();  // tcgen05.ld is warp-collective: reconverge after the stores
-        ptx::tmem_ld_32x32b_x32(t_lane + cc * 32, r);
-        ptx::tmem_ld_wait();
-        if (row_ok && n < p.N) {
-            Row32 out;
-            with_act(p.act, [&](auto a) {
-                out = linear_values<decltype(a)::value>(r, sa, {sbs + cc * 32}, {bias_s + cc * 32}, has_res, res);
-            });
-            store_row32(static_cast<__nv_bfloat16*>(p.C) + (int64_t)row * p.ldc + n, out, p.N - n, vec_ok);
-        }
-    }
 }
 
 // h of 32 outputs from the accumulators of their gates and ups
@@ -334,17 +270,20 @@ __device__ __forceinline__ void store4(const Params& p, int row, int n, const fl
     }
 }
 
-// GATED: rows [0, 64) of the weight tile are gates, [64, 128) the ups of the same outputs; 16 groups of four outputs
-// per token instead of 32.
-template <int MAXS, int U, bool GATED>
-__device__ __forceinline__ void reduce_partials_fused(const Params& p, const uint32_t (&peer_base)[MAXS], int S, int cols_lo,
+// Gated: rows [0, 64) of the weight tile are gates, [64, 128) the ups of the same outputs; 16 groups of four outputs
+// per token instead of 32.  Tokens count from m0, the first of the CTA's block of tokens.
+template <int MAXS, int U, int EPI>
+__device__ __forceinline__ void reduce_partials_fused(const Params& p, const uint32_t (&peer_base)[MAXS], int S, int m0, int cols_lo,
                                                       int cols_hi, int n0, int tid, int nthreads, const float* sa_s,
                                                       const float* sb_s, const float* bias_s) {
-    constexpr int kGroups = GATED ? 16 : 32, kShift = GATED ? 4 : 5, kHalves = GATED ? 2 : 1;
+    constexpr bool kGated = is_gated(EPI), kGrad = EPI == kEpiLinearGrad || EPI == kEpiGatedGrad;
+    constexpr bool kReads = EPI != kEpiGated;   // a residual, or the incoming gradient
+    constexpr int kGroups = kGated ? 16 : 32, kShift = kGated ? 4 : 5, kHalves = kGated ? 2 : 1;
     const bool vec_store = (p.ldc % 4 == 0) && ((reinterpret_cast<uintptr_t>(p.C) & 7) == 0);
     const bool res_vec = (p.ldr % 4 == 0) && ((reinterpret_cast<uintptr_t>(p.resid) & 7) == 0);
     const int items = (cols_hi - cols_lo) * kGroups;
-    for (int it0 = tid; it0 < items; it0 += nthreads * U) {
+    // a warp's lanes stay together: the gradients' largest magnitudes are exchanged between them
+    for (int it0 = tid; (it0 & ~31) < items; it0 += nthreads * U) {
         uint4 v[U][kHalves][MAXS];
         uint2 res[U];
 #pragma unroll
@@ -353,9 +292,9 @@ __device__ __forceinline__ void reduce_partials_fused(const Params& p, const uin
             res[u] = make_uint2(0u, 0u);
             if (it < items) {
                 const int c = cols_lo + (it >> kShift), g = it & (kGroups - 1);
-                if (!GATED && p.resid != nullptr) {
+                if (kReads && p.resid != nullptr) {
                     const int n = n0 + g * 4;
-                    const __nv_bfloat16* rp = p.resid + (int64_t)c * p.ldr + n;
+                    const __nv_bfloat16* rp = p.resid + (int64_t)(m0 + c) * p.ldr + n;
                     if (res_vec && n + 4 <= p.N) {
                         res[u] = *reinterpret_cast<const uint2*>(rp);
                     } else {
@@ -404,36 +343,68 @@ __device__ __forceinline__ void reduce_partials_fused(const Params& p, const uin
             for (int u = 0; u < U; ++u) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    z[u][0][j] = act_value2<decltype(act)::value>(z[u][0][j]);
-                    if constexpr (GATED) z[u][0][j] = __fmul2_rn(z[u][0][j], z[u][kHalves - 1][j]);
+                    if constexpr (kGrad) {
+                        const float2 d = bf16x2_to_f32x2(j == 0 ? res[u].x : res[u].y);
+                        float2 slope;
+                        const float2 value = act_value_slope2<decltype(act)::value>(z[u][0][j], slope);
+                        if constexpr (kGated) {
+                            z[u][0][j] = __fmul2_rn(__fmul2_rn(d, z[u][kHalves - 1][j]), slope);
+                            z[u][kHalves - 1][j] = __fmul2_rn(d, value);
+                        } else {
+                            z[u][0][j] = __fmul2_rn(d, slope);
+                        }
+                    } else {
+                        z[u][0][j] = act_value2<decltype(act)::value>(z[u][0][j]);
+                        if constexpr (kGated) z[u][0][j] = __fmul2_rn(z[u][0][j], z[u][kHalves - 1][j]);
+                    }
                 }
             }
         });
 #pragma unroll
         for (int u = 0; u < U; ++u) {
             const int it = it0 + u * nthreads;
-            if (it >= items) break;
-            const int c = cols_lo + (it >> kShift), n = n0 + (it & (kGroups - 1)) * 4;
-            if (n >= p.N) continue;
-            if (!GATED && p.resid != nullptr) {
-                const float2 r0 = bf16x2_to_f32x2(res[u].x), r1 = bf16x2_to_f32x2(res[u].y);
-                z[u][0][0] = make_float2(__fadd_rn(z[u][0][0].x, r0.x), __fadd_rn(z[u][0][0].y, r0.y));
-                z[u][0][1] = make_float2(__fadd_rn(z[u][0][1].x, r1.x), __fadd_rn(z[u][0][1].y, r1.y));
+            const int c = cols_lo + (it >> kShift), g = it & (kGroups - 1), n = n0 + g * 4;
+            const bool ok = it < items && n < p.N;
+            if constexpr (kGrad) {
+                // dz rows have room for whole tiles: four columns are stored, those at or beyond N with zeros
+                unsigned top = 0;
+                if (ok) {
+                    float* dz = static_cast<float*>(p.C) + (int64_t)(m0 + c) * p.ldc + n;
+#pragma unroll
+                    for (int h = 0; h < kHalves; ++h) {
+                        *reinterpret_cast<uint4*>(dz + h * p.up_col) = bits4(z[u][h][0], z[u][h][1]);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const int col = h * 64 + g * 4 + 2 * j;
+                            top = top_bits2(top, z[u][h][j], make_float2(sb_s[col], sb_s[col + 1]));
+                        }
+                    }
+                }
+#pragma unroll
+                for (int o = kGroups >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                if (g == 0 && top != 0) atomicMax(p.row_top + m0 + c, top);
+            } else if (ok) {
+                if (kReads && p.resid != nullptr) {
+                    const float2 r0 = bf16x2_to_f32x2(res[u].x), r1 = bf16x2_to_f32x2(res[u].y);
+                    z[u][0][0] = make_float2(__fadd_rn(z[u][0][0].x, r0.x), __fadd_rn(z[u][0][0].y, r0.y));
+                    z[u][0][1] = make_float2(__fadd_rn(z[u][0][1].x, r1.x), __fadd_rn(z[u][0][1].y, r1.y));
+                }
+                store4(p, m0 + c, n, z[u][0][0], z[u][0][1], vec_store);
             }
-            store4(p, c, n, z[u][0][0], z[u][0][1], vec_store);
         }
     }
 }
 
 // With no more items than threads (few tokens) one item per thread: the loop body for U of them would be fetched, cold, to
 // do nothing, which cost 1.4 us of a 9 us kernel.
-template <int MAXS, int U, bool GATED>
-__device__ __forceinline__ void reduce_partials_fused_sized(const Params& p, const uint32_t (&peer_base)[MAXS], int S, int cols_lo,
-                                                            int cols_hi, int n0, int tid, int nthreads, const float* scales) {
-    if ((cols_hi - cols_lo) * (GATED ? 16 : 32) <= nthreads)
-        reduce_partials_fused<MAXS, 1, GATED>(p, peer_base, S, cols_lo, cols_hi, n0, tid, nthreads, scales, scales + 256, scales + 384);
+template <int MAXS, int U, int EPI>
+__device__ __forceinline__ void reduce_partials_fused_sized(const Params& p, const uint32_t (&peer_base)[MAXS], int S, int m0,
+                                                            int cols_lo, int cols_hi, int n0, int tid, int nthreads,
+                                                            const float* scales) {
+    if ((cols_hi - cols_lo) * (is_gated(EPI) ? 16 : 32) <= nthreads)
+        reduce_partials_fused<MAXS, 1, EPI>(p, peer_base, S, m0, cols_lo, cols_hi, n0, tid, nthreads, scales, scales + 256, scales + 384);
     else
-        reduce_partials_fused<MAXS, U, GATED>(p, peer_base, S, cols_lo, cols_hi, n0, tid, nthreads, scales, scales + 256, scales + 384);
+        reduce_partials_fused<MAXS, U, EPI>(p, peer_base, S, m0, cols_lo, cols_hi, n0, tid, nthreads, scales, scales + 256, scales + 384);
 }
 
 }  // namespace

@@ -234,6 +234,251 @@ gemm_i8_grad_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
     }
 }
 
+// ------------------------------------------------------------------------------------
+// The same product for few rows: operands swapped, as in gemm_i8_stream_kernel.  128 columns of W sit on the MMA's M axis
+// (W is then the A operand, MN-major as above), ROWS rows of both digits side by side on its N axis, so W is read once
+// for both digits and no tensor-core rows are spent on padding.  A cluster of S CTAs shares one tile and splits W's rows
+// between its CTAs; the int32 partials [2 ROWS][128] meet in shared memory and are summed exactly.  More rows than ROWS
+// are further blocks of clusters, which read W again.
+// ------------------------------------------------------------------------------------
+template <int ROWS>
+struct GradStreamSmem {
+    static constexpr int kWBytes = 128 * BK;
+    static constexpr int kDigitBytes = ROWS * BK;   // one digit's rows
+    static constexpr int kStageBytes = kWBytes + 2 * kDigitBytes;
+    static constexpr int kRingBytes = 196 * 1024;
+    static constexpr int kStages = kRingBytes / kStageBytes < 10 ? kRingBytes / kStageBytes : 10;
+    static constexpr int kTilesBytes = kStages * kStageBytes;
+    static constexpr int kPartialBytes = 2 * ROWS * 128 * 4;
+    static_assert(kPartialBytes <= kTilesBytes, "the partial tile reuses the stage ring");
+    static constexpr int kScaleOff = kTilesBytes;   // the rows' digit scales
+    static constexpr int kBarOff = kScaleOff + ROWS * 4;
+    static constexpr int kNumBars = 2 * kStages + 1;
+    static constexpr int kTmemSlotOff = kBarOff + kNumBars * 8;
+    static constexpr int kAbortOff = kTmemSlotOff + 4;
+    static constexpr int kTotal = kAbortOff + 4;
+    static constexpr int kDynamic = kTotal + 1024;
+};
+
+// dx of the rows [lo, hi) of the block: item = (row, four columns), consecutive threads on consecutive columns
+template <int ROWS, int U>
+__device__ __forceinline__ void reduce_gradient(const GradParams& p, const uint32_t (&peer_base)[8], int S, int m0, int lo, int hi,
+                                                int k0, const float* scale_s) {
+    const int items = (hi - lo) * 32;
+    const bool vec = (reinterpret_cast<uintptr_t>(p.dx) & 7) == 0;   // K is a multiple of 16
+    for (int it0 = threadIdx.x; it0 < items; it0 += kThreads * U) {
+        uint4 v[U][2][8];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int it = it0 + u * kThreads;
+            if (it < items) {
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    const uint32_t off = (uint32_t)((d * ROWS + lo + (it >> 5)) * 128 + (it & 31) * 4) * 4u;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                        if (r < S) v[u][d][r] = ptx::ld_shared_cluster_v4(peer_base[r] + off);
+                }
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int it = it0 + u * kThreads;
+            if (it >= items) break;
+            const int c = lo + (it >> 5), k = k0 + (it & 31) * 4;
+            if (k >= p.K) continue;
+            int a[2][4] = {};
+#pragma unroll
+            for (int d = 0; d < 2; ++d) {
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    if (r < S) {
+                        a[d][0] += (int)v[u][d][r].x; a[d][1] += (int)v[u][d][r].y;
+                        a[d][2] += (int)v[u][d][r].z; a[d][3] += (int)v[u][d][r].w;
+                    }
+                }
+            }
+            const float s = scale_s[c];
+            float y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[j] = digit_value(a[0][j], a[1][j], s);
+            const uint32_t out_lo = pack_bf16x2_rn(y[0], y[1]), out_hi = pack_bf16x2_rn(y[2], y[3]);
+            __nv_bfloat16* out = p.dx + (int64_t)(m0 + c) * p.K + k;
+            if (vec) {
+                *reinterpret_cast<uint2*>(out) = make_uint2(out_lo, out_hi);
+            } else {
+                uint16_t* o = reinterpret_cast<uint16_t*>(out);
+                o[0] = (uint16_t)(out_lo & 0xffffu); o[1] = (uint16_t)(out_lo >> 16);
+                o[2] = (uint16_t)(out_hi & 0xffffu); o[3] = (uint16_t)(out_hi >> 16);
+            }
+        }
+    }
+}
+
+template <int ROWS>
+__global__ void __launch_bounds__(kThreads, 1)
+gemm_i8_grad_stream_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_constant__ CUtensorMap tmW, const GradParams p) {
+    using L = GradStreamSmem<ROWS>;
+    constexpr int STAGES = L::kStages, NCOL = 2 * ROWS;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::kBarOff);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kTmemSlotOff);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kAbortOff);
+    int* partial = reinterpret_cast<int*>(smem);  // [NCOL][128] once the ring has drained
+    float* scale_s = reinterpret_cast<float*>(smem + L::kScaleOff);
+    const uint32_t tiles_base = ptx::smem_u32(smem);
+    const uint32_t bar_base = ptx::smem_u32(bars);
+    auto full_bar = [&](int s) { return bar_base + 8u * s; };
+    auto empty_bar = [&](int s) { return bar_base + 8u * (STAGES + s); };
+    const uint32_t acc_full_bar = bar_base + 8u * (2 * STAGES);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int S = (int)ptx::cluster_nctarank(), split = (int)ptx::cluster_ctarank();
+    const int tiles_k = (p.K + 127) / 128, cluster = blockIdx.x / S, m_block = cluster / tiles_k;
+    const int k0 = (cluster - m_block * tiles_k) * 128, m0 = m_block * ROWS;
+
+    const int blocks = p.parts * p.part_blocks;
+    const int nb0 = (int)((int64_t)blocks * split / S), nb1 = (int)((int64_t)blocks * (split + 1) / S);
+    const int prologue = (nb1 - nb0) < STAGES ? (nb1 - nb0) : STAGES;
+    auto load_weight = [&](uint32_t dst, int nb, uint32_t bar) {
+        const int part = nb >= p.part_blocks ? 1 : 0;
+        ptx::tma_load_2d(dst, &tmW, k0, part * p.part_rows + (nb - part * p.part_blocks) * BK, bar);
+    };
+    auto load_digits = [&](uint32_t dst, int nb, uint32_t bar) {   // rows past the block or the digit belong to no output
+        ptx::tma_load_2d(dst, &tmD, nb * BK, m0, bar);
+        ptx::tma_load_2d(dst + L::kDigitBytes, &tmD, nb * BK, p.M + m0, bar);
+    };
+    bool ok = true;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            ptx::mbar_init(full_bar(s), 1);
+            ptx::mbar_init(empty_bar(s), 1);
+        }
+        ptx::mbar_init(acc_full_bar, 1);
+        *abort_flag = 0;
+        ptx::fence_barrier_init();
+        ptx::fence_proxy_async_smem();
+        // the weight does not depend on the kernel before this one, the digits do
+        for (int i = 0; i < prologue; ++i) {
+            ptx::mbar_arrive_expect_tx(full_bar(i), L::kStageBytes);
+            load_weight(tiles_base + i * L::kStageBytes, nb0 + i, full_bar(i));
+        }
+        ptx::grid_dependency_wait();
+        for (int i = 0; i < prologue; ++i) load_digits(tiles_base + i * L::kStageBytes + L::kWBytes, nb0 + i, full_bar(i));
+    }
+    if (warp == 1) {
+        ptx::tmem_alloc(ptx::smem_u32(tmem_slot), NCOL);
+        ptx::tmem_relinquish();
+    }
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::tc_fence_after_sync();
+    const uint32_t tmem_base = *tmem_slot;
+
+    if (warp == 0) {
+        if (ptx::elect_one()) {
+            int stage = prologue == STAGES ? 0 : prologue;
+            uint32_t phase = prologue == STAGES ? 1u : 0u;
+            for (int nb = nb0 + prologue; nb < nb1; ++nb) {
+                if (!ptx::mbar_wait_bounded(empty_bar(stage), phase ^ 1u, p.wait_limit_ns) || *abort_flag) {
+                    report_wait_failure(kWaitEmptyStage);
+                    *abort_flag = 1;
+                    break;
+                }
+                const uint32_t dst = tiles_base + stage * L::kStageBytes;
+                ptx::mbar_arrive_expect_tx(full_bar(stage), L::kStageBytes);
+                load_weight(dst, nb, full_bar(stage));
+                load_digits(dst + L::kWBytes, nb, full_bar(stage));
+                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+            }
+        }
+    } else if (warp == 1) {
+        if (ptx::elect_one()) {
+            constexpr uint32_t idesc = ptx::idesc_i8_a_mn(128, NCOL);
+            int stage = 0;
+            uint32_t phase = 0;
+            bool issued_all = true;
+            for (int nb = nb0; nb < nb1; ++nb) {
+                if (!ptx::mbar_wait_bounded(full_bar(stage), phase, p.wait_limit_ns) || *abort_flag) {
+                    report_wait_failure(kWaitFullStage);
+                    *abort_flag = 1;
+                    issued_all = false;
+                    break;
+                }
+                ptx::tc_fence_after_sync();
+                const uint32_t src = tiles_base + stage * L::kStageBytes;
+                const uint64_t adesc = ptx::smem_desc_mn_sw128(src);
+                const uint64_t bdesc = ptx::smem_desc_k_sw128(src + L::kWBytes);
+#pragma unroll
+                for (int k = 0; k < BK / UMMA_K; ++k)
+                    ptx::mma_i8_ss(tmem_base, adesc + (4096u >> 4) * k, bdesc + 2u * k, idesc, (nb > nb0 || k != 0) ? 1u : 0u);
+                ptx::tc_commit(empty_bar(stage));
+                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+            }
+            if (issued_all) ptx::tc_commit(acc_full_bar);
+        }
+    } else {
+        // drain warps: scales and column sums first, then accumulator -> shared partial
+        ptx::grid_dependency_wait();
+        for (int i = threadIdx.x - 64; i < ROWS; i += kDrainThreads)
+            scale_s[i] = m0 + i < p.M ? digit_scale(__uint_as_float(__ldcg(p.row_top + m0 + i))) : 0.0f;
+        if (p.partial != nullptr) sum_columns(p, blockIdx.x * 4 + warp - 2, gridDim.x * 4);
+        const int quarter = warp & 3, wcol = quarter * 32 + lane;  // column of W inside the tile = TMEM lane
+        __syncwarp();
+        if (nb1 > nb0) {
+            if (!ptx::mbar_wait_bounded(acc_full_bar, 0, p.wait_limit_ns) || *abort_flag) {
+                report_wait_failure(kWaitAccFull);
+                *abort_flag = 1;
+                ok = false;
+            }
+        }
+        ptx::tc_fence_after_sync();
+        __syncwarp();
+        if (ok) {
+            const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+#pragma unroll 1
+            for (int cc = 0; cc < NCOL / 32; ++cc) {
+                uint32_t r[32];
+                if (nb1 > nb0) {
+                    ptx::tmem_ld_32x32b_x32(t_lane + cc * 32, r);
+                    ptx::tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) r[j] = 0;  // a CTA without blocks contributes zero
+                }
+#pragma unroll
+                for (int j = 0; j < 32; ++j) partial[(cc * 32 + j) * 128 + wcol] = (int)r[j];
+            }
+        }
+    }
+
+    // every CTA's partial is complete and visible to the cluster
+    ptx::tc_fence_before_sync();
+    __syncthreads();
+    ptx::cluster_sync();
+    ptx::grid_dependency_wait();
+
+    {
+        const int rows = min(ROWS, p.M - m0);
+        const int lo = (int)((int64_t)rows * split / S), hi = (int)((int64_t)rows * (split + 1) / S);
+        const uint32_t my_partial = ptx::smem_u32(partial);
+        uint32_t peer_base[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) peer_base[r] = ptx::map_to_cta(my_partial, r < S ? r : 0);
+        if ((hi - lo) * 32 <= kThreads) reduce_gradient<ROWS, 1>(p, peer_base, S, m0, lo, hi, k0, scale_s);
+        else reduce_gradient<ROWS, 2>(p, peer_base, S, m0, lo, hi, k0, scale_s);
+    }
+
+    // nobody leaves while a peer may still read its shared memory
+    __syncthreads();
+    ptx::cluster_sync();
+    if (warp == 1) {
+        ptx::tc_fence_after_sync();
+        ptx::tmem_dealloc(tmem_base, NCOL);
+    }
+}
+
 }  // namespace
 }  // namespace w8a8
 

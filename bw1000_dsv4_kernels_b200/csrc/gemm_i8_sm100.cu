@@ -173,25 +173,25 @@ int sm_count() {
     return cached;
 }
 
-template <int BN, int STAGES, int EPI>
+template <int BN, int STAGES>
 int launch_variant(const CUtensorMap& tmA, const CUtensorMap& tmB, const Params& p, int max_tiles,
                    cudaStream_t st) {
     using L = Smem<BN, STAGES>;
     static_assert(L::kDynamic <= 227 * 1024, "shared memory limit");
     static bool opted_in[64] = {};
-    if (!opt_in_shared_memory(gemm_i8_kernel<BN, STAGES, EPI>, L::kDynamic, opted_in))
+    if (!opt_in_shared_memory(gemm_i8_kernel<BN, STAGES>, L::kDynamic, opted_in))
         return fail(DSV4_ERR_LAUNCH, "w8a8_gemm: cannot raise the dynamic shared memory limit");
     int grid = sm_count();
     if (grid <= 0) return fail(DSV4_ERR_LAUNCH, "w8a8_gemm: no CUDA device");
     if (max_tiles < grid) grid = max_tiles;
     if (grid < 1) grid = 1;
-    gemm_i8_kernel<BN, STAGES, EPI><<<grid, kThreads, L::kDynamic, st>>>(tmA, tmB, p);
+    gemm_i8_kernel<BN, STAGES><<<grid, kThreads, L::kDynamic, st>>>(tmA, tmB, p);
     return check_launch("w8a8_gemm");
 }
 
 template <int NTOK, int EPI>
 int launch_stream_variant(const CUtensorMap& tmW, const CUtensorMap& tmX, const Params& p, int n_tiles, int splits,
-                          cudaStream_t st) {
+                          bool follows, cudaStream_t st) {
     using L = StreamSmem<NTOK>;
     static_assert(L::kDynamic <= 227 * 1024, "shared memory limit");
     static bool opted_in[64] = {};
@@ -210,7 +210,7 @@ int launch_stream_variant(const CUtensorMap& tmW, const CUtensorMap& tmX, const 
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = overlap_previous_kernel() ? 2 : 1;
+    cfg.numAttrs = overlap_previous_kernel() || follows ? 2 : 1;
     const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_stream_kernel<NTOK, EPI>, tmW, tmX, p);
     if (err != cudaSuccess) {
         cudaGetLastError();  // clear the sticky launch error
@@ -221,39 +221,44 @@ int launch_stream_variant(const CUtensorMap& tmW, const CUtensorMap& tmX, const 
     return check_launch("w8a8_gemm (weight streaming)");
 }
 
-// How many clusters of 2*splits CTAs of the pair streaming kernel the device can run at once (one
-// CTA per SM, a cluster inside one GPC); asked once per device and cluster size, of a kernel that has its shared memory
-// opted in (the answer is none otherwise).
-template <int EPI>
-int stream_pair_active_clusters(int splits) {
-    static int cached[64][5] = {};
+// How many clusters of `size` (at most eight) CTAs of a kernel the device can run at once (one CTA per SM, a cluster inside one
+// GPC); asked once per kernel, device and cluster size, of a kernel that has its shared memory opted in (the answer is
+// none otherwise).
+using ClusterCounts = int[64][9];
+template <typename Kernel>
+int active_clusters(Kernel kernel, int size, int smem, ClusterCounts& cached) {
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || splits < 1 || splits > 4) return 0;
-    if (cached[dev][splits] == 0) {
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64 || size < 1 || size > 8) return 0;
+    if (cached[dev][size] == 0) {
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)(2 * splits * 64), 1, 1);
+        cfg.gridDim = dim3((unsigned)(size * 64), 1, 1);
         cfg.blockDim = dim3(kThreads, 1, 1);
-        cfg.dynamicSmemBytes = StreamPairSmem::kDynamic;
+        cfg.dynamicSmemBytes = smem;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = (unsigned)(2 * splits);
+        attr[0].val.clusterDim.x = (unsigned)size;
         attr[0].val.clusterDim.y = 1;
         attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         int n = 0;
-        if (cudaOccupancyMaxActiveClusters(&n, gemm_i8_stream_pair_kernel<EPI>, &cfg) != cudaSuccess) {
+        if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
             cudaGetLastError();
             n = -1;
         }
-        cached[dev][splits] = n > 0 ? n : -1;
+        cached[dev][size] = n > 0 ? n : -1;
     }
-    return cached[dev][splits] > 0 ? cached[dev][splits] : 0;
+    return cached[dev][size] > 0 ? cached[dev][size] : 0;
+}
+template <int EPI>
+int stream_pair_active_clusters(int splits) {
+    static ClusterCounts cached = {};
+    return active_clusters(gemm_i8_stream_pair_kernel<EPI>, 2 * splits, StreamPairSmem::kDynamic, cached);
 }
 
 template <int EPI>
 int launch_stream_pair(const CUtensorMap& tmW, const CUtensorMap& tmX, const Params& p, int n_tiles, int splits,
-                       cudaStream_t st) {
+                       bool follows, cudaStream_t st) {
     using L = StreamPairSmem;
     static_assert(L::kDynamic <= 227 * 1024, "shared memory limit");
     static bool opted_in[64] = {};
@@ -274,7 +279,7 @@ int launch_stream_pair(const CUtensorMap& tmW, const CUtensorMap& tmX, const Par
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = overlap_previous_kernel() ? 2 : 1;
+    cfg.numAttrs = overlap_previous_kernel() || follows ? 2 : 1;
     const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_stream_pair_kernel<EPI>, tmW, tmX, p);
     if (err != cudaSuccess) {
         cudaGetLastError();  // clear the sticky launch error
@@ -403,51 +408,92 @@ int launch_fused_pair(const GemmArgs& a, Params p, cudaStream_t st) {
     return check_launch("w8a8_linear");
 }
 
+// The CTA-pair streaming kernel over `blocks` blocks of tokens of about the same length
+int stream_block_tokens(int M, int blocks) { return ((M + blocks - 1) / blocks + 31) / 32 * 32; }
+template <int EPI>
+int launch_stream_blocks(const GemmArgs& a, Params p, int blocks, int pair_tiles, int splits, cudaStream_t st) {
+    const int w_rows = is_gated(EPI) ? 2 * a.N : a.N;
+    p.block_m = EPI == kEpiPlain ? 256 : stream_block_tokens(a.M, blocks);
+    CUtensorMap tmW, tmX;
+    if (int rc = make_tile_map(&tmW, a.B, (uint64_t)w_rows, (uint64_t)a.K, is_gated(EPI) ? 64 : 128)) return rc;
+    if (int rc = make_tile_map(&tmX, a.A, (uint64_t)a.M, (uint64_t)a.K, (uint32_t)(p.block_m / 2))) return rc;  // a CTA's half of the tokens
+    return launch_stream_pair<EPI>(tmW, tmX, p, pair_tiles * blocks, splits, a.follows, st);
+}
+
+// Whether a K split over `splits` CTAs or pairs pays for a block of so many tokens: a K block costs 0.3 us, the split saves
+// (1 - 1 / splits) of them, and the sum of the partials through shared memory, with its epilogue, costs 6 to 9 us more for 256
+// tokens than the tile kernel's drain.
+bool split_pays(int tokens, int splits, int k_blocks) { return k_blocks * (splits - 1) >= tokens / 8 * splits; }
+
+// Whether few tokens with a fused epilogue go to the weight-streaming kernel rather than the tiles of 256 tokens.  Up to
+// 64 tokens always.  Measured (tiles / streaming, with bias, GELU, residual): 128 x 4096 x 1024 5.6 / 9.0 us, x 7168 14.7 /
+// 14.8; 128 x 18432 x 4096 28.2 / 29.2; 65 x 18432 x 4096 27.2 / 24.0; 65 x 4096 x 1024 6.2 / 7.6; 33 x 18432 x 1024 14.4 / 9.7;
+// 200 x 200 x 7168 15.3 (pairs) / 12.4.
+bool fused_few(int M, int w_rows, int splits, int k_blocks) {
+    if (M <= 64) return true;
+    if (M > 128 && w_rows >= 256) return false;
+    return splits == 1 ? M <= 96 : split_pays(M, splits, k_blocks);
+}
+
+// K split of more tokens over the streaming kernel's pairs, or 0 where the tile kernel is faster.  Measured (tiles / this
+// one): 600 x 1000 x 8192 with bias, GELU, residual 24.3 / 16.8 us, x 2048 10.3 / 13.4; gated 300 x 2048 x 7168 20.4 / 17.5,
+// 400 x 500 x 4096 12.0 / 12.4; 200 x 2000 x 2048 9.0 / 12.8.
+template <int EPI>
+int stream_blocks_splits(int M, int pair_tiles, int blocks, int k_blocks) {
+    const int64_t clusters = (int64_t)pair_tiles * blocks;
+    static bool opted_in[64] = {};
+    if (clusters > 37 || !opt_in_shared_memory(gemm_i8_stream_pair_kernel<EPI>, StreamPairSmem::kDynamic, opted_in)) return 0;
+    for (int s = k_blocks < 4 ? k_blocks : 4; s > 1; --s)
+        if (stream_pair_active_clusters<EPI>(s) >= clusters) return split_pays(stream_block_tokens(M, blocks), s, k_blocks) ? s : 0;
+    return 0;
+}
+
 // Dense problems: the kernel by the number of tokens and tiles.  A gated weight [2 N, K] gives N outputs, and each weight
 // tile takes half its rows from the gates and half from the ups, so its N counts twice.
 template <int EPI>
 int gemm_i8_dense(const GemmArgs& a, const Params& p, int bn, cudaStream_t st) {
     constexpr bool kGated = is_gated(EPI);
-    constexpr bool kGrad = EPI == kEpiLinearGrad || EPI == kEpiGatedGrad;
     const int sms = sm_count();
     const int w_rows = kGated ? 2 * a.N : a.N;
     CUtensorMap tmA, tmB;
+    const int k_blocks = (a.K + BK - 1) / BK;
     // Few tokens: stream the weight once, tokens on the MMA's N axis, K split over a cluster
-    if constexpr (!kGrad) if (a.M <= 256 && a.npeers == 0) {
-        const int k_blocks = (a.K + BK - 1) / BK;
-        if (a.M > 128 && w_rows >= 256) {
+    if (a.M <= 256 && a.npeers == 0) {
+        if (EPI == kEpiPlain && a.M > 128 && a.N >= 256) {
             // 129..256 tokens: CTA pairs halve the token traffic per SM
-            const int pair_tiles = kGated ? (a.N + 127) / 128 : (a.N + 255) / 256;
+            const int pair_tiles = (a.N + 255) / 256;
             int psplits = sms / (2 * pair_tiles);
             if (psplits > 4) psplits = 4;
             if (psplits > k_blocks) psplits = k_blocks;
             if (psplits < 1) psplits = 1;
-            int rc5 = make_tile_map(&tmA, a.B, (uint64_t)w_rows, (uint64_t)a.K, kGated ? 64 : 128);   // weights
-            if (rc5) return rc5;
-            rc5 = make_tile_map(&tmB, a.A, (uint64_t)a.M, (uint64_t)a.K, 128);  // this CTA's half of the tokens
-            if (rc5) return rc5;
-            return launch_stream_pair<EPI>(tmA, tmB, p, pair_tiles, psplits, st);
+            return launch_stream_blocks<EPI>(a, p, 1, pair_tiles, psplits, st);
         }
         const int n_tiles = kGated ? (a.N + 63) / 64 : (a.N + 127) / 128;
         int splits = sms / n_tiles;
         if (splits > 8) splits = 8;
         if (splits > k_blocks) splits = k_blocks;
         if (splits < 1) splits = 1;
-        const int ntok = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : a.M <= 128 ? 128 : 256;
-        int rc4 = make_tile_map(&tmA, a.B, (uint64_t)w_rows, (uint64_t)a.K, kGated ? 64 : 128);   // weights
-        if (rc4) return rc4;
-        rc4 = make_tile_map(&tmB, a.A, (uint64_t)a.M, (uint64_t)a.K, (uint32_t)ntok);  // tokens
-        if (rc4) return rc4;
-        switch (ntok) {
-            case 16: return launch_stream_variant<16, EPI>(tmA, tmB, p, n_tiles, splits, st);
-            case 32: return launch_stream_variant<32, EPI>(tmA, tmB, p, n_tiles, splits, st);
-            case 64: return launch_stream_variant<64, EPI>(tmA, tmB, p, n_tiles, splits, st);
-            case 128: return launch_stream_variant<128, EPI>(tmA, tmB, p, n_tiles, splits, st);
-            default: return launch_stream_variant<256, EPI>(tmA, tmB, p, n_tiles, splits, st);
+        if (EPI == kEpiPlain || fused_few(a.M, w_rows, splits, k_blocks)) {
+            const int ntok = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : a.M <= 128 ? 128 : 256;
+            int rc4 = make_tile_map(&tmA, a.B, (uint64_t)w_rows, (uint64_t)a.K, kGated ? 64 : 128);   // weights
+            if (rc4) return rc4;
+            rc4 = make_tile_map(&tmB, a.A, (uint64_t)a.M, (uint64_t)a.K, (uint32_t)ntok);  // tokens
+            if (rc4) return rc4;
+            switch (ntok) {
+                case 16: return launch_stream_variant<16, EPI>(tmA, tmB, p, n_tiles, splits, a.follows, st);
+                case 32: return launch_stream_variant<32, EPI>(tmA, tmB, p, n_tiles, splits, a.follows, st);
+                case 64: return launch_stream_variant<64, EPI>(tmA, tmB, p, n_tiles, splits, a.follows, st);
+                case 128: return launch_stream_variant<128, EPI>(tmA, tmB, p, n_tiles, splits, a.follows, st);
+                default: return launch_stream_variant<256, EPI>(tmA, tmB, p, n_tiles, splits, a.follows, st);
+            }
         }
     }
-    // Dense problems with more than one 128-row tile go to the CTA-pair kernel, gated ones and gradients always
-    if constexpr (EPI != kEpiPlain) if (kGated || kGrad || (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256) >= sms / 4)
+    if constexpr (EPI != kEpiPlain) {
+        // More tokens, few tiles, long K: CTA pairs over blocks of tokens; otherwise tiles of 256 tokens
+        const int pair_tiles = kGated ? (a.N + 127) / 128 : (a.N + 255) / 256;
+        const int blocks = (a.M + 255) / 256;
+        const int splits = stream_blocks_splits<EPI>(a.M, pair_tiles, blocks, k_blocks);
+        if (splits > 0) return launch_stream_blocks<EPI>(a, p, blocks, pair_tiles, splits, st);
         switch (a.act) {
             case kActRelu: return launch_fused_pair<EPI, kActRelu>(a, p, st);
             case kActGelu: return launch_fused_pair<EPI, kActGelu>(a, p, st);
@@ -457,7 +503,9 @@ int gemm_i8_dense(const GemmArgs& a, const Params& p, int bn, cudaStream_t st) {
                 if constexpr (EPI == kEpiLinear) return launch_fused_pair<EPI, kActNone>(a, p, st);
                 return fail(DSV4_ERR_ARG, "w8a8_linear: unknown activation");
         }
-    if constexpr (EPI == kEpiPlain) if ((a.M > 128 && (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256) >= sms / 4)) {
+    }
+    // Dense problems with more than one 128-row tile go to the CTA-pair kernel
+    if (a.M > 128 && (int64_t)((a.M + 255) / 256) * ((a.N + 255) / 256) >= sms / 4) {
         int rc2 = make_tile_map(&tmA, a.A, (uint64_t)a.M, (uint64_t)a.K, BM);
         if (rc2) return rc2;
         rc2 = make_tile_map(&tmB, a.B, (uint64_t)w_rows, (uint64_t)a.K, 128);
@@ -477,20 +525,17 @@ int gemm_i8_dense(const GemmArgs& a, const Params& p, int bn, cudaStream_t st) {
         }
         return launch_pair_variant<6, false>(tmA, tmB, p, smaps, st);
     }
-    if constexpr (!kGated && !kGrad) {
-        int rc = make_tile_map(&tmA, a.A, (uint64_t)a.M, (uint64_t)a.K, BM);
-        if (rc) return rc;
-        rc = make_tile_map(&tmB, a.B, (uint64_t)w_rows, (uint64_t)a.K, (uint32_t)bn);
-        if (rc) return rc;
-        const int max_tiles = ((a.M + BM - 1) / BM) * ((a.N + bn - 1) / bn);
-        switch (bn) {
-            case 256: return launch_variant<256, 4, EPI>(tmA, tmB, p, max_tiles, st);
-            case 128: return launch_variant<128, 6, EPI>(tmA, tmB, p, max_tiles, st);
-            case 64: return launch_variant<64, 8, EPI>(tmA, tmB, p, max_tiles, st);
-            default: return launch_variant<32, 10, EPI>(tmA, tmB, p, max_tiles, st);
-        }
+    int rc = make_tile_map(&tmA, a.A, (uint64_t)a.M, (uint64_t)a.K, BM);
+    if (rc) return rc;
+    rc = make_tile_map(&tmB, a.B, (uint64_t)w_rows, (uint64_t)a.K, (uint32_t)bn);
+    if (rc) return rc;
+    const int max_tiles = ((a.M + BM - 1) / BM) * ((a.N + bn - 1) / bn);
+    switch (bn) {
+        case 256: return launch_variant<256, 4>(tmA, tmB, p, max_tiles, st);
+        case 128: return launch_variant<128, 6>(tmA, tmB, p, max_tiles, st);
+        case 64: return launch_variant<64, 8>(tmA, tmB, p, max_tiles, st);
+        default: return launch_variant<32, 10>(tmA, tmB, p, max_tiles, st);
     }
-    return 0;
 }
 
 }  // namespace
@@ -610,13 +655,64 @@ int gemm_i8(const GemmArgs& a, cudaStream_t st) {
     }
 }
 
+namespace {
+
+// The gradient product of few rows.  The sum is split over as many CTAs (at most eight) as still let all clusters run at
+// once.
+//
+// Returns without a launch where the kernel for many rows is faster (`launched` says so): clusters that do not run at once,
+// or a sum so short that the rows' share of it is not worth joining the partials.  A block of 128 rows of W costs a pair of
+// CTAs 0.75 us there (two digits), a CTA here up to 0.55 us, shared by S of them.  Measured (there / here, whole backward
+// pass): gated 16 x 2048 x 7168 34.7 / 19.6 us, 64 x 9000 x 5008 69 / 38, 200 x 4096 x 7168 49 / 47, 600 x 8192 x 512 73 / 47,
+// gated 700 x 300 x 1024 21.3 / 22.0.
+template <int ROWS>
+int launch_grad_stream(const GradientArgs& a, const GradParams& p, cudaStream_t st, bool& launched) {
+    using L = GradStreamSmem<ROWS>;
+    launched = false;
+    static_assert(L::kDynamic <= 227 * 1024, "shared memory limit");
+    static bool opted_in[64] = {};
+    static ClusterCounts cached = {};
+    if (!opt_in_shared_memory(gemm_i8_grad_stream_kernel<ROWS>, L::kDynamic, opted_in))
+        return fail(DSV4_ERR_LAUNCH, "w8a8 backward: cannot raise the dynamic shared memory limit");
+    const int64_t clusters = (int64_t)((a.K + 127) / 128) * ((a.M + ROWS - 1) / ROWS);
+    const int blocks = a.parts * p.part_blocks;
+    int splits = blocks < 8 ? blocks : 8;
+    while (splits > 0 && active_clusters(gemm_i8_grad_stream_kernel<ROWS>, splits, L::kDynamic, cached) < clusters) --splits;
+    if (blocks * (3 * splits - 2) < 20 * splits || splits == 0) return 0;
+    launched = true;
+    CUtensorMap tmD, tmW;
+    if (int rc = make_tile_map(&tmD, a.digits, (uint64_t)2 * a.M, (uint64_t)a.parts * a.part_pitch, ROWS)) return rc;
+    if (int rc = make_tile_map(&tmW, a.W, (uint64_t)a.parts * a.part_rows, (uint64_t)a.K, 128)) return rc;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(clusters * splits), 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = L::kDynamic;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    if (cudaLaunchKernelEx(&cfg, gemm_i8_grad_stream_kernel<ROWS>, tmD, tmW, p) != cudaSuccess) {
+        cudaGetLastError();  // clear the sticky launch error
+        return fail(DSV4_ERR_LAUNCH, "w8a8 backward: launch of the gradient product");
+    }
+    return check_launch("w8a8 backward");
+}
+
+}  // namespace
+
 // dx = dz_scaled W for digits that split_gradient_kernel wrote (see gemm_i8_grad_kernel.cuh)
 int gemm_i8_gradient(const GradientArgs& a, cudaStream_t st) {
     using L = FusedPairSmem;
     static bool opted_in[64] = {};
     if (!opt_in_shared_memory(gemm_i8_grad_kernel, L::kDynamic, opted_in))
         return fail(DSV4_ERR_LAUNCH, "w8a8 backward: cannot raise the dynamic shared memory limit");
-    GradParams p;
+    GradParams p = {};
     p.row_top = a.row_top;
     p.dx = static_cast<__nv_bfloat16*>(a.dx);
     p.M = a.M; p.K = a.K;
@@ -629,6 +725,15 @@ int gemm_i8_gradient(const GradientArgs& a, cudaStream_t st) {
     if (gm_max < 1) gm_max = 1;
     const int groups = (tiles_m + gm_max - 1) / gm_max;
     p.group_m = (tiles_m + groups - 1) / groups;
+    p.partial = a.partial;
+    p.row_blocks = a.row_blocks;
+    p.dbias = a.dbias;
+    bool launched;
+    const int rc = a.M <= 16   ? launch_grad_stream<16>(a, p, st, launched)
+                   : a.M <= 32 ? launch_grad_stream<32>(a, p, st, launched)
+                   : a.M <= 64 ? launch_grad_stream<64>(a, p, st, launched)
+                               : launch_grad_stream<128>(a, p, st, launched);
+    if (rc != 0 || launched) return rc;
     CUtensorMap tmD, tmW;
     if (int rc = make_tile_map(&tmD, a.digits, (uint64_t)2 * a.M, (uint64_t)pitch, BM)) return rc;
     if (int rc = make_tile_map(&tmW, a.W, (uint64_t)a.parts * a.part_rows, (uint64_t)a.K, 128)) return rc;
@@ -637,9 +742,6 @@ int gemm_i8_gradient(const GradientArgs& a, cudaStream_t st) {
     if (pairs <= 0) return fail(DSV4_ERR_LAUNCH, "w8a8 backward: no CUDA device");
     if (tiles > INT32_MAX) return fail(DSV4_ERR_ARG, "w8a8 backward: too many tiles");
     if (tiles < pairs) pairs = (int)tiles;
-    p.partial = a.partial;
-    p.row_blocks = a.row_blocks;
-    p.dbias = a.dbias;
     return launch_after(gemm_i8_grad_kernel, dim3(2 * pairs), dim3(kFusedThreads), L::kDynamic, st, "w8a8 backward", tmD, tmW, p);
 }
 

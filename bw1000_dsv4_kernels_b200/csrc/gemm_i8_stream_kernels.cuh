@@ -117,21 +117,37 @@ struct StreamSmem {
     static constexpr int kDynamic = kTotal + 1024;
 };
 
+// The outputs and tokens of a cluster: all weight tiles of the first block of tokens, then those of the next.  The plain
+// GEMM has one block (block_m 0).
+struct TileOf {
+    int n0, m0;
+    __device__ __forceinline__ TileOf(const Params& p, int cluster, int tile_outputs, int block_m) {
+        if (block_m == 0) {
+            n0 = cluster * tile_outputs;
+            m0 = 0;
+        } else {
+            const int tiles = (p.N + tile_outputs - 1) / tile_outputs, block = cluster / tiles;
+            n0 = (cluster - block * tiles) * tile_outputs;
+            m0 = block * block_m;
+        }
+    }
+};
+
 // The drain warps (threads 64..191) have nothing to do while the weight streams: they fetch the scales the
 // epilogue needs.  Activation scales may come from the kernel before this one, hence the dependency wait.
 template <int EPI>
-__device__ __forceinline__ void stage_scales(const Params& p, float* sa_s, float* sb_s, int ntok, int n0) {
+__device__ __forceinline__ void stage_scales(const Params& p, float* sa_s, float* sb_s, int ntok, int n0, int m0) {
     ptx::grid_dependency_wait();
     if (p.out_i32) return;
     const int t = threadIdx.x - 64;
-    for (int i = t; i < ntok; i += kDrainThreads) sa_s[i] = i < p.M ? __ldg(p.sa + i) : 0.0f;
+    for (int i = t; i < ntok; i += kDrainThreads) sa_s[i] = m0 + i < p.M ? __ldg(p.sa + m0 + i) : 0.0f;
     if constexpr (EPI == kEpiPlain) {
         for (int j = t; j < 128; j += kDrainThreads) sb_s[j] = n0 + j < p.N ? __ldg(p.sb + n0 + j) : 0.0f;
     } else {
         // a gated tile is 64 gate rows, then the 64 up rows of the same outputs
         float* bias_s = sb_s + 128;
         for (int j = t; j < 128; j += kDrainThreads) {
-            const bool up = EPI == kEpiGated && j >= 64;
+            const bool up = is_gated(EPI) && j >= 64;
             const int c = up ? p.inter + n0 + (j - 64) : n0 + j;
             const bool ok = c < (up ? 2 * p.inter : p.N);
             sb_s[j] = ok ? __ldg(p.sb + c) : 0.0f;
@@ -145,7 +161,7 @@ __device__ __forceinline__ void stage_scales(const Params& p, float* sa_s, float
 template <int EPI>
 __device__ __forceinline__ void load_weight_tile(uint32_t dst, const CUtensorMap* tmW, int k, int n0, int inter, uint32_t bar) {
     ptx::tma_load_2d(dst, tmW, k, n0, bar);
-    if constexpr (EPI == kEpiGated) ptx::tma_load_2d(dst + 64 * BK, tmW, k, inter + n0, bar);
+    if constexpr (is_gated(EPI)) ptx::tma_load_2d(dst + 64 * BK, tmW, k, inter + n0, bar);
 }
 
 template <int NTOK, int EPI = kEpiPlain>
@@ -173,8 +189,8 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int S = (int)ptx::cluster_nctarank();
     const int split = (int)ptx::cluster_ctarank();
-    const int nt = blockIdx.x / S;
-    const int n0 = nt * (EPI == kEpiGated ? 64 : 128);
+    const TileOf tile(p, blockIdx.x / S, is_gated(EPI) ? 64 : 128, EPI == kEpiPlain ? 0 : NTOK);
+    const int n0 = tile.n0, m0 = tile.m0;
     constexpr uint32_t kTmemCols = NTOK < 32 ? 32 : NTOK;
 
     // this CTA's share of the K blocks
@@ -203,7 +219,7 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
         }
         ptx::grid_dependency_wait();
         for (int i = 0; i < prologue; ++i)
-            ptx::tma_load_2d(tiles_base + i * L::kStageBytes + L::kWBytes, &tmX, (kb0 + i) * BK, 0, full_bar(i));
+            ptx::tma_load_2d(tiles_base + i * L::kStageBytes + L::kWBytes, &tmX, (kb0 + i) * BK, m0, full_bar(i));
     }
     if (warp == 1) {
         ptx::tmem_alloc(ptx::smem_u32(tmem_slot), kTmemCols);
@@ -227,7 +243,7 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
                 const uint32_t w_dst = tiles_base + stage * L::kStageBytes;
                 ptx::mbar_arrive_expect_tx(full_bar(stage), L::kStageBytes);
                 load_weight_tile<EPI>(w_dst, &tmW, kb * BK, n0, p.inter, full_bar(stage));
-                ptx::tma_load_2d(w_dst + L::kWBytes, &tmX, kb * BK, 0, full_bar(stage));
+                ptx::tma_load_2d(w_dst + L::kWBytes, &tmX, kb * BK, m0, full_bar(stage));
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
         }
@@ -258,7 +274,7 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
         }
     } else {
         // drain warps: the epilogue's scales first, then accumulator -> shared partial
-        stage_scales<EPI>(p, sa_s, sb_s, NTOK, n0);
+        stage_scales<EPI>(p, sa_s, sb_s, NTOK, n0, m0);
         const int quarter = warp & 3;
         const int wrow = quarter * 32 + lane;  // weight row inside the tile = TMEM lane
         if (kb1 > kb0) {
@@ -306,9 +322,11 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
 
     {
         // all six warps take part: the producer and MMA threads are done by now
-        const int cols_lo = (int)((int64_t)NTOK * split / S);
-        int cols_hi = (int)((int64_t)NTOK * (split + 1) / S);
-        if (cols_hi > p.M) cols_hi = p.M;
+        // (the fused epilogues, which take longer, share out the tokens that there are)
+        const int cols = EPI == kEpiPlain ? NTOK : min(NTOK, p.M - m0);
+        const int cols_lo = (int)((int64_t)cols * split / S);
+        int cols_hi = (int)((int64_t)cols * (split + 1) / S);
+        if (EPI == kEpiPlain && cols_hi > p.M) cols_hi = p.M;
         const uint32_t my_partial = ptx::smem_u32(partial);
         uint32_t peer_base[8];
 #pragma unroll
@@ -316,8 +334,8 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
         if constexpr (EPI == kEpiPlain)
             reduce_partials_and_store<8, 4>(p, peer_base, S, cols_lo, cols_hi, n0, threadIdx.x, kThreads, sa_s, sb_s);
         else
-            reduce_partials_fused_sized<8, EPI == kEpiGated ? 2 : 4, EPI == kEpiGated>(p, peer_base, S, cols_lo, cols_hi, n0,
-                                                                                       threadIdx.x, kThreads, sa_s);
+            reduce_partials_fused_sized<8, is_gated(EPI) ? 2 : 4, EPI>(p, peer_base, S, m0, cols_lo, cols_hi, n0, threadIdx.x,
+                                                                       kThreads, sa_s);
     }
 
     // nobody leaves while a peer may still read its shared memory
@@ -342,7 +360,7 @@ gemm_i8_stream_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_cons
 // ------------------------------------------------------------------------------------
 struct StreamPairSmem {
     static constexpr int kWBytes = 128 * BK;
-    static constexpr int kXBytes = 128 * BK;   // this CTA's half of the 256 token rows
+    static constexpr int kXBytes = 128 * BK;   // this CTA's half of at most 256 token rows
     static constexpr int kStageBytes = kWBytes + kXBytes;
     static constexpr int kStages = 6;
     static constexpr int kTilesBytes = kStages * kStageBytes;
@@ -385,12 +403,15 @@ gemm_i8_stream_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
     const int S = csize >> 1, split = crank >> 1, half = crank & 1;
     const uint32_t leader = (uint32_t)(crank & ~1);
     const uint16_t pair_mask = (uint16_t)(0x3u << leader);
-    const int nt = blockIdx.x / csize;
+    // the block's tokens, half of them loaded by each CTA of the pair
+    const int ntok = EPI == kEpiPlain ? NTOK : p.block_m;
+    const TileOf tile(p, blockIdx.x / csize, is_gated(EPI) ? 128 : 256, EPI == kEpiPlain ? 0 : ntok);
     // this CTA's outputs: 128 weight rows, or the 64 gates and 64 ups of 64 gated outputs
-    const int n0 = EPI == kEpiGated ? nt * 128 + half * 64 : nt * 256 + half * 128;
+    const int n0 = tile.n0 + half * (is_gated(EPI) ? 64 : 128), m0 = tile.m0;
+    const uint32_t pair_stage_bytes = 2u * (uint32_t)(L::kWBytes + (ntok >> 1) * BK);
     auto load_weights = [&](uint32_t dst, int k, uint32_t bar) {
         ptx::tma_load_2d_pair(dst, &tmW, k, n0, bar);
-        if constexpr (EPI == kEpiGated) ptx::tma_load_2d_pair(dst + 64 * BK, &tmW, k, p.inter + n0, bar);
+        if constexpr (is_gated(EPI)) ptx::tma_load_2d_pair(dst + 64 * BK, &tmW, k, p.inter + n0, bar);
     };
     constexpr uint32_t kTmemCols = NTOK;
 
@@ -427,12 +448,12 @@ gemm_i8_stream_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
             const int prologue = (kb1 - kb0) < STAGES ? (kb1 - kb0) : STAGES;
             for (int i = 0; i < prologue; ++i) {
                 const uint32_t leader_full = ptx::map_to_cta(full_bar(i), leader);
-                if (half == 0) ptx::mbar_arrive_expect_tx(full_bar(i), 2 * L::kStageBytes);
+                if (half == 0) ptx::mbar_arrive_expect_tx(full_bar(i), pair_stage_bytes);
                 load_weights(tiles_base + i * L::kStageBytes, (kb0 + i) * BK, leader_full);
             }
             ptx::grid_dependency_wait();
             for (int i = 0; i < prologue; ++i)
-                ptx::tma_load_2d_pair(tiles_base + i * L::kStageBytes + L::kWBytes, &tmX, (kb0 + i) * BK, half * 128,
+                ptx::tma_load_2d_pair(tiles_base + i * L::kStageBytes + L::kWBytes, &tmX, (kb0 + i) * BK, m0 + half * (ntok >> 1),
                                       ptx::map_to_cta(full_bar(i), leader));
             int stage = prologue == STAGES ? 0 : prologue;
             uint32_t phase = prologue == STAGES ? 1u : 0u;
@@ -444,15 +465,15 @@ gemm_i8_stream_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
                 }
                 const uint32_t w_dst = tiles_base + stage * L::kStageBytes;
                 const uint32_t leader_full = ptx::map_to_cta(full_bar(stage), leader);
-                if (half == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), 2 * L::kStageBytes);
+                if (half == 0) ptx::mbar_arrive_expect_tx(full_bar(stage), pair_stage_bytes);
                 load_weights(w_dst, kb * BK, leader_full);
-                ptx::tma_load_2d_pair(w_dst + L::kWBytes, &tmX, kb * BK, half * 128, leader_full);
+                ptx::tma_load_2d_pair(w_dst + L::kWBytes, &tmX, kb * BK, m0 + half * (ntok >> 1), leader_full);
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
         }
     } else if (warp == 1) {
         if (half == 0 && ptx::elect_one()) {
-            constexpr uint32_t idesc = ptx::idesc_i8(256, NTOK);
+            const uint32_t idesc = ptx::idesc_i8(256, ntok);
             int stage = 0;
             uint32_t phase = 0;
             bool issued_all = true;
@@ -478,7 +499,7 @@ gemm_i8_stream_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
     } else {
         // drain warps of both CTAs: the epilogue's scales first, then the accumulator of this CTA's 128 weight
         // rows -> shared partial
-        stage_scales<EPI>(p, sa_s, sb_s, NTOK, n0);
+        stage_scales<EPI>(p, sa_s, sb_s, ntok, n0, m0);
         const int quarter = warp & 3;
         const int wrow = quarter * 32 + lane;
         if (kb1 > kb0) {
@@ -493,7 +514,7 @@ gemm_i8_stream_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
         if (ok) {
             const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
 #pragma unroll 1
-            for (int cc = 0; cc < NTOK / 32; ++cc) {
+            for (int cc = 0; cc < ntok / 32; ++cc) {
                 uint32_t r[32];
                 if (kb1 > kb0) {
                     ptx::tmem_ld_32x32b_x32(t_lane + cc * 32, r);
@@ -515,9 +536,11 @@ gemm_i8_stream_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
     ptx::grid_dependency_wait();     // before this thread reads activation scales or writes C
 
     {
-        const int cols_lo = (int)((int64_t)NTOK * split / S);
-        int cols_hi = (int)((int64_t)NTOK * (split + 1) / S);
-        if (cols_hi > p.M) cols_hi = p.M;
+        // (the fused epilogues, which take longer, share out the tokens that there are)
+        const int cols = EPI == kEpiPlain ? NTOK : min(ntok, p.M - m0);
+        const int cols_lo = (int)((int64_t)cols * split / S);
+        int cols_hi = (int)((int64_t)cols * (split + 1) / S);
+        if (EPI == kEpiPlain && cols_hi > p.M) cols_hi = p.M;
         const uint32_t my_partial = ptx::smem_u32(partial);
         uint32_t peer_base[4];
 #pragma unroll
@@ -525,8 +548,8 @@ gemm_i8_stream_pair_kernel(const __grid_constant__ CUtensorMap tmW, const __grid
         if constexpr (EPI == kEpiPlain)
             reduce_partials_and_store<4, 8>(p, peer_base, S, cols_lo, cols_hi, n0, threadIdx.x, kThreads, sa_s, sb_s);
         else
-            reduce_partials_fused_sized<4, EPI == kEpiGated ? 4 : 8, EPI == kEpiGated>(p, peer_base, S, cols_lo, cols_hi, n0,
-                                                                                       threadIdx.x, kThreads, sa_s);
+            reduce_partials_fused_sized<4, is_gated(EPI) ? 4 : 8, EPI>(p, peer_base, S, m0, cols_lo, cols_hi, n0, threadIdx.x,
+                                                                       kThreads, sa_s);
     }
 
     // nobody leaves while a peer may still read its shared memory

@@ -4,7 +4,6 @@
 #define W8A8_GEMM_I8_TILE_KERNEL_CUH
 
 #include "gemm_i8_common.cuh"
-#include "gemm_i8_epilogues.cuh"
 
 namespace w8a8 {
 namespace {
@@ -12,7 +11,7 @@ namespace {
 // ------------------------------------------------------------------------------------
 // Per-token-scaled (or raw int32) kernel: whole K accumulates in tensor memory.
 // ------------------------------------------------------------------------------------
-template <int BN, int STAGES, int EPI = kEpiPlain>
+template <int BN, int STAGES>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_i8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                const Params p) {
@@ -131,7 +130,6 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
         // ---------------- drain warps (2..5) ----------------
         const int quarter = warp & 3;  // TMEM lanes a warp may touch: 32*(warp%4)..+31
         float* sbs = sb_tile + (warp - 2) * BN;  // private to this warp: no block-level barrier
-        float* bias_s = reinterpret_cast<float*>(smem + L::kBiasOff) + (warp - 2) * BN;
         int acc = 0;
         uint32_t acc_phase = 0;
         const bool vec_ok = c_vector_stores_ok(p);
@@ -139,9 +137,7 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             const TileCoord c = sched.at(t, BN);
             // column scales of this tile -> this warp's shared copy
             __syncwarp();
-            if constexpr (EPI == kEpiLinear) {
-                stage_columns(p, sbs, bias_s, lane, BN, c.n0);
-            } else if (!p.out_i32) {
+            if (!p.out_i32) {
                 for (int j = lane; j < BN; j += 32)
                     sbs[j] = (c.n0 + j < p.N) ? __ldg(p.sb + c.n0 + j) : 0.0f;
             }
@@ -156,10 +152,8 @@ gemm_i8_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ 
             const int row = c.a_row0 + quarter * 32 + lane;
             const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * BN;
             // a warp whose 32 rows all lie past the last row has nothing to load or store
-            if (c.a_row0 + quarter * 32 < c.row_end) {
-                if constexpr (EPI == kEpiLinear) drain_linear<BN>(p, t_lane, sbs, bias_s, row, row < c.row_end, c.n0, vec_ok);
-                else drain_accumulator<BN>(p, t_lane, sbs, row, row < c.row_end, c.n0, vec_ok);
-            }
+            if (c.a_row0 + quarter * 32 < c.row_end)
+                drain_accumulator<BN>(p, t_lane, sbs, row, row < c.row_end, c.n0, vec_ok);
             ptx::tc_fence_before_sync();
             __syncwarp();
             if (lane == 0) ptx::mbar_arrive(acc_empty_bar(acc));

@@ -343,6 +343,8 @@ __host__ __device__ constexpr uint32_t idesc_i8(int m, int n) {
 }
 // B is MN-major (bit 16 set)
 __host__ __device__ constexpr uint32_t idesc_i8_b_mn(int m, int n) { return idesc_i8(m, n) | (1u << 16); }
+// A is MN-major (bit 15 set)
+__host__ __device__ constexpr uint32_t idesc_i8_a_mn(int m, int n) { return idesc_i8(m, n) | (1u << 15); }
 
 }  // namespace ptx
 }  // namespace w8a8
