@@ -65,11 +65,17 @@ __device__ __forceinline__ void store_pieces(char* block, int64_t ld_bytes, cons
     }
 }
 // Loading takes two steps, so that the requests can be out long before the block is needed: fetch_block issues them into
-// registers as the memory is laid out, arrange_block turns those into one row per lane.
+// registers as the memory is laid out, arrange_block turns those into one row per lane.  Rows that are not 16-byte
+// aligned come as the 16-byte granules that cover them, at most five for 64 bytes, and each lane shifts its row into place;
+// element by element, 2048 x 7167 x 1024 with bias, GELU and residual took 113 us instead of 61 (50 at 7168).  Only the
+// first and the last granule of the array can reach out of it; what they hold of it is fetched by elements.
 struct Fetched {
-    uint32_t w[16];
+    uint32_t w[20];
+    int skew;     // bytes from the first granule to this lane's row
 };
-__device__ __forceinline__ Fetched fetch_block(const __nv_bfloat16* block, int64_t ld, const RowBlock& b, int lane) {
+// `array` has m rows of n elements, `block` begins at one of them
+__device__ __forceinline__ Fetched fetch_block(const __nv_bfloat16* array, int64_t ld, int m, int n, const __nv_bfloat16* block,
+                                               const RowBlock& b, int lane) {
     Fetched f = {};
     if (b.vec) {
         const int piece = lane & 3;
@@ -81,30 +87,65 @@ __device__ __forceinline__ Fetched fetch_block(const __nv_bfloat16* block, int64
                 f.w[4 * i] = q.x; f.w[4 * i + 1] = q.y; f.w[4 * i + 2] = q.z; f.w[4 * i + 3] = q.w;
             }
         }
-    } else if (lane < b.cols) {
-        const uint16_t* src = reinterpret_cast<const uint16_t*>(block) + lane;
+        return f;
+    }
+    const char *lo = reinterpret_cast<const char*>(array), *hi = reinterpret_cast<const char*>(array + (m - 1) * ld + n);
+    const int bytes = 2 * min(b.cols, 32);
+    f.skew = (int)(reinterpret_cast<uintptr_t>(block + lane * ld) & 15);
+    // granule i of this lane, or null where no row needs it
+    auto granule = [&](int i) -> const char* {
+        const int g = 32 * i + lane, row = g / 5, piece = g - 5 * row;
+        const char* src = reinterpret_cast<const char*>(block + row * ld);
+        const int skew = (int)(reinterpret_cast<uintptr_t>(src) & 15);
+        return row < b.rows && 16 * piece < skew + bytes ? src + 16 * piece - skew : nullptr;
+    };
+    unsigned edges = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            const uint32_t lo = 2 * i < b.rows ? src[(2 * i) * ld] : 0u, hi = 2 * i + 1 < b.rows ? src[(2 * i + 1) * ld] : 0u;
-            f.w[i] = lo | (hi << 16);
+    for (int i = 0; i < 5; ++i) {
+        const char* src = granule(i);
+        if (src == nullptr) continue;
+        if (src >= lo && src + 16 <= hi) {
+            const uint4 q = *reinterpret_cast<const uint4*>(src);
+            f.w[4 * i] = q.x; f.w[4 * i + 1] = q.y; f.w[4 * i + 2] = q.z; f.w[4 * i + 3] = q.w;
+        } else {
+            edges |= 1u << i;
+        }
+    }
+#pragma unroll 1
+    for (int k = 0; edges >> k; ++k) {   // one of a lane's granules, but for arrays a few elements wide
+        if (!((edges >> k) & 1)) continue;
+        const char* src = granule(k);
+        uint32_t e[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const char* at = src + 4 * j;
+            const uint32_t l = at >= lo && at < hi ? *reinterpret_cast<const uint16_t*>(at) : 0u;
+            const uint32_t h = at + 2 >= lo && at + 2 < hi ? *reinterpret_cast<const uint16_t*>(at + 2) : 0u;
+            e[j] = l | (h << 16);
+        }
+#pragma unroll
+        for (int i = 0; i < 5; ++i) {
+            if (i == k) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f.w[4 * i + j] = e[j];
+            }
         }
     }
     return f;
 }
-__device__ __forceinline__ Row32 arrange_block(const Fetched& f, bool vec, uint32_t* stage, int lane) {
+__device__ __forceinline__ Row32 arrange_block(const Fetched& f, const RowBlock& b, uint32_t* stage, int lane) {
     __syncwarp();
-    if (vec) {
+    if (b.vec) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
             *reinterpret_cast<uint4*>(stage + (8 * i + (lane >> 2)) * kStagePitch + 4 * (lane & 3)) =
                 make_uint4(f.w[4 * i], f.w[4 * i + 1], f.w[4 * i + 2], f.w[4 * i + 3]);
     } else {
-        uint16_t* s16 = reinterpret_cast<uint16_t*>(stage);
+        static_assert(kStagePitch == 20, "five granules are a staged row");
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            s16[(2 * i) * (2 * kStagePitch) + lane] = (uint16_t)(f.w[i] & 0xffffu);
-            s16[(2 * i + 1) * (2 * kStagePitch) + lane] = (uint16_t)(f.w[i] >> 16);
-        }
+        for (int i = 0; i < 5; ++i)
+            *reinterpret_cast<uint4*>(stage + (32 * i + lane) * 4) =
+                make_uint4(f.w[4 * i], f.w[4 * i + 1], f.w[4 * i + 2], f.w[4 * i + 3]);
     }
     __syncwarp();
     Row32 r;
@@ -112,6 +153,26 @@ __device__ __forceinline__ Row32 arrange_block(const Fetched& f, bool vec, uint3
     for (int j = 0; j < 4; ++j) {
         const uint4 q = *reinterpret_cast<const uint4*>(stage + lane * kStagePitch + 4 * j);
         r.w[4 * j] = q.x; r.w[4 * j + 1] = q.y; r.w[4 * j + 2] = q.z; r.w[4 * j + 3] = q.w;
+    }
+    if (!b.vec) {
+        // 80 bytes of the lane's row, shifted by `skew`: four-word, then two-byte steps
+        const uint4 q = *reinterpret_cast<const uint4*>(stage + lane * kStagePitch + 16);
+        uint32_t w[20];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) w[j] = r.w[j];
+        w[16] = q.x; w[17] = q.y; w[18] = q.z; w[19] = q.w;
+        const bool by2 = f.skew & 8, by1 = f.skew & 4;
+#pragma unroll
+        for (int j = 0; j < 18; ++j) w[j] = by2 ? w[j + 2] : w[j];
+#pragma unroll
+        for (int j = 0; j < 17; ++j) w[j] = by1 ? w[j + 1] : w[j];
+        const uint32_t half = (f.skew & 2) * 8;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r.w[j] = __funnelshift_r(w[j], w[j + 1], half);
+        if (b.cols < 32) {   // what follows the row is not zero
+#pragma unroll
+            for (int j = 0; j < 16; ++j) r.w[j] &= 2 * j + 1 < b.cols ? 0xffffffffu : 2 * j < b.cols ? 0xffffu : 0u;
+        }
     }
     return r;
 }

@@ -239,7 +239,7 @@ gemm_i8_fused_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
             auto fetch = [&](int cc) {
                 const int n = n0 + cc * 32;
                 if (EPI == kEpiGated || (!kGrad && !has_res) || cc >= chunks || n >= p.N || rows <= 0) return Fetched{};
-                return fetch_block(p.resid + (int64_t)row0 * p.ldr + n, p.ldr, {rows, p.N - n, in_vec}, lane);
+                return fetch_block(p.resid, p.ldr, p.M, p.N, p.resid + (int64_t)row0 * p.ldr + n, {rows, p.N - n, in_vec}, lane);
             };
             Fetched fetched = fetch(turn);
             const float sa = row_ok ? __ldg(p.sa + row) : 0.0f;
@@ -262,7 +262,7 @@ gemm_i8_fused_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
                 ptx::tmem_ld_32x32b_x32(t_lane + cc * 32, r);
                 if constexpr (kGated) ptx::tmem_ld_32x32b_x32(t_lane + half_n + cc * 32, u);
                 Row32 in = {};
-                if (kGrad || (EPI == kEpiLinear && has_res)) in = arrange_block(fetched, in_vec, stage, lane);
+                if (kGrad || (EPI == kEpiLinear && has_res)) in = arrange_block(fetched, {rows, p.N - n, in_vec}, stage, lane);
                 fetched = fetch(cc + 2);
                 ptx::tmem_ld_wait();
                 if constexpr (!kGrad) {
