@@ -39,7 +39,10 @@ def check_db(db, db64, dz, dz_err):
 
 
 SHAPES = [(1, 8, 16), (3, 40, 48), (17, 127, 128), (64, 128, 144), (100, 257, 272), (129, 320, 1040), (256, 256, 256),
-          (257, 1000, 400), (300, 129, 2064), (513, 600, 528), (700, 2305, 784)]
+          (257, 1000, 400), (300, 129, 2064), (513, 600, 528), (700, 2305, 784),
+          # sums split over clusters for 16, 32, 64 and 128 rows and several blocks of them; rows of a few elements
+          (1, 2000, 2064), (16, 1500, 1040), (30, 4000, 144), (40, 3000, 528), (128, 4100, 400), (300, 2600, 400),
+          (200, 300, 6160), (500, 3, 400), (260, 1, 48)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)

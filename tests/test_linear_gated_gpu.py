@@ -1,5 +1,6 @@
 """The fused W8A8 linear and the gated projection against 64 bits on the CPU, at sizes that reach every kernel behind them
-(weight streaming for up to 16, 32, 64, 128 and 256 tokens, CTA pairs, one CTA per tile) and end inside their tiles.
+(weight streaming for up to 16, 32, 64, 128 and 256 tokens, the same by CTA pairs, tiles of CTA pairs) and end inside their
+tiles.
 
 Tolerances: the integer sum is exact; its conversion, two products and the bias add round once each (4 * 2^-24 of
 |acc*sa*sb| + |bias|), the activations have slopes of at most 1.13 and are off by 2^-18 of their value where the fast
@@ -26,7 +27,10 @@ def cuda(*ts):
 
 SHAPES = [(1, 8, 16), (1, 257, 144), (5, 40, 48), (16, 384, 2064), (17, 127, 128), (33, 1000, 272), (64, 129, 1040),
           (100, 320, 256), (128, 100, 528), (129, 255, 160), (200, 256, 2064), (256, 1001, 144), (257, 8, 64), (300, 1000, 400),
-          (300, 7700, 144), (513, 5129, 272), (1100, 2304, 1040)]
+          (300, 7700, 144), (513, 5129, 272), (1100, 2304, 1040),
+          # K split over pairs, one block of tokens and several; few tokens by tiles; rows of a few elements
+          (140, 600, 6160), (200, 100, 5520), (300, 260, 7200), (600, 1000, 5520), (70, 900, 528), (80, 20000, 144),
+          (128, 19001, 272), (900, 3, 144), (400, 1, 32), (270, 5, 6000)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
