@@ -189,38 +189,6 @@ int launch_variant(const CUtensorMap& tmA, const CUtensorMap& tmB, const Params&
     return check_launch("w8a8_gemm");
 }
 
-template <int NTOK, int EPI>
-int launch_stream_variant(const CUtensorMap& tmW, const CUtensorMap& tmX, const Params& p, int n_tiles, int splits,
-                          bool follows, cudaStream_t st) {
-    using L = StreamSmem<NTOK>;
-    static_assert(L::kDynamic <= 227 * 1024, "shared memory limit");
-    static bool opted_in[64] = {};
-    if (!opt_in_shared_memory(gemm_i8_stream_kernel<NTOK, EPI>, L::kDynamic, opted_in))
-        return fail(DSV4_ERR_LAUNCH, "w8a8_gemm: cannot raise the dynamic shared memory limit");
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(n_tiles * splits), 1, 1);
-    cfg.blockDim = dim3(kThreads, 1, 1);
-    cfg.dynamicSmemBytes = L::kDynamic;
-    cfg.stream = st;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = (unsigned)splits;
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = overlap_previous_kernel() || follows ? 2 : 1;
-    const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_stream_kernel<NTOK, EPI>, tmW, tmX, p);
-    if (err != cudaSuccess) {
-        cudaGetLastError();  // clear the sticky launch error
-        static thread_local char msg[160];
-        snprintf(msg, sizeof msg, "w8a8_gemm (weight streaming): %s", cudaGetErrorString(err));
-        return fail(DSV4_ERR_LAUNCH, msg);
-    }
-    return check_launch("w8a8_gemm (weight streaming)");
-}
-
 // How many clusters of `size` (at most eight) CTAs of a kernel the device can run at once (one CTA per SM, a cluster inside one
 // GPC); asked once per kernel, device and cluster size, of a kernel that has its shared memory opted in (the answer is
 // none otherwise).
@@ -250,6 +218,44 @@ int active_clusters(Kernel kernel, int size, int smem, ClusterCounts& cached) {
     }
     return cached[dev][size] > 0 ? cached[dev][size] : 0;
 }
+template <int NTOK, int EPI>
+int launch_stream_variant(const CUtensorMap& tmW, const CUtensorMap& tmX, const Params& p, int n_tiles, int splits,
+                          bool follows, cudaStream_t st) {
+    using L = StreamSmem<NTOK>;
+    static_assert(L::kDynamic <= 227 * 1024, "shared memory limit");
+    static bool opted_in[64] = {};
+    if (!opt_in_shared_memory(gemm_i8_stream_kernel<NTOK, EPI>, L::kDynamic, opted_in))
+        return fail(DSV4_ERR_LAUNCH, "w8a8_gemm: cannot raise the dynamic shared memory limit");
+    // fused epilogues: no wider a split than lets all clusters run at once (17 x 3000 x 1024, 24 tiles: 9.7 us split over six
+    // CTAs, 5.6 over five)
+    if constexpr (EPI != kEpiPlain) {
+        static ClusterCounts cached = {};
+        while (splits > 1 && active_clusters(gemm_i8_stream_kernel<NTOK, EPI>, splits, L::kDynamic, cached) < n_tiles) --splits;
+    }
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(n_tiles * splits), 1, 1);
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = L::kDynamic;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)splits;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = overlap_previous_kernel() || follows ? 2 : 1;
+    const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_stream_kernel<NTOK, EPI>, tmW, tmX, p);
+    if (err != cudaSuccess) {
+        cudaGetLastError();  // clear the sticky launch error
+        static thread_local char msg[160];
+        snprintf(msg, sizeof msg, "w8a8_gemm (weight streaming): %s", cudaGetErrorString(err));
+        return fail(DSV4_ERR_LAUNCH, msg);
+    }
+    return check_launch("w8a8_gemm (weight streaming)");
+}
+
 template <int EPI>
 int stream_pair_active_clusters(int splits) {
     static ClusterCounts cached = {};
@@ -425,14 +431,15 @@ int launch_stream_blocks(const GemmArgs& a, Params p, int blocks, int pair_tiles
 // tokens than the tile kernel's drain.
 bool split_pays(int tokens, int splits, int k_blocks) { return k_blocks * (splits - 1) >= tokens / 8 * splits; }
 
-// Whether few tokens with a fused epilogue go to the weight-streaming kernel rather than the tiles of 256 tokens.  Up to
-// 64 tokens always.  Measured (tiles / streaming, with bias, GELU, residual): 128 x 4096 x 1024 5.6 / 9.0 us, x 7168 14.7 /
-// 14.8; 128 x 18432 x 4096 28.2 / 29.2; 65 x 18432 x 4096 27.2 / 24.0; 65 x 4096 x 1024 6.2 / 7.6; 33 x 18432 x 1024 14.4 / 9.7;
-// 200 x 200 x 7168 15.3 (pairs) / 12.4.
-bool fused_few(int M, int w_rows, int splits, int k_blocks) {
-    if (M <= 64) return true;
+// Whether few tokens with a fused epilogue go to the weight-streaming kernel rather than the tiles of 256 tokens, whose drain
+// is faster and whose tiles are as narrow as 64 outputs.  Measured (tiles / streaming, with bias, GELU, residual): 128 x 4096
+// x 1024 5.6 / 9.0 us, x 7168 14.7 / 14.8; 128 x 18432 x 4096 28.2 / 29.2; 65 x 18432 x 4096 27.2 / 24.0; 65 x 4096 x 1024
+// 6.2 / 7.6; 59 x 3000 x 64 6.6 / 9.0, x 512 7.3 / 6.6; 33 x 18432 x 1024 14.4 / 9.7; 200 x 200 x 7168 15.3 (pairs) / 12.4.
+bool fused_few(int M, int w_rows, int n_tiles, int splits, int k_blocks) {
+    const bool few_tiles = n_tiles <= 37;
+    if (M <= 64) return M <= 32 || k_blocks > 2 || !few_tiles;
     if (M > 128 && w_rows >= 256) return false;
-    return splits == 1 ? M <= 96 : split_pays(M, splits, k_blocks);
+    return few_tiles ? split_pays(M, splits, k_blocks) : M <= 96;
 }
 
 // K split of more tokens over the streaming kernel's pairs, or 0 where the tile kernel is faster.  Measured (tiles / this
@@ -473,7 +480,7 @@ int gemm_i8_dense(const GemmArgs& a, const Params& p, int bn, cudaStream_t st) {
         if (splits > 8) splits = 8;
         if (splits > k_blocks) splits = k_blocks;
         if (splits < 1) splits = 1;
-        if (EPI == kEpiPlain || fused_few(a.M, w_rows, splits, k_blocks)) {
+        if (EPI == kEpiPlain || fused_few(a.M, w_rows, n_tiles, splits, k_blocks)) {
             const int ntok = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : a.M <= 128 ? 128 : 256;
             int rc4 = make_tile_map(&tmA, a.B, (uint64_t)w_rows, (uint64_t)a.K, kGated ? 64 : 128);   // weights
             if (rc4) return rc4;

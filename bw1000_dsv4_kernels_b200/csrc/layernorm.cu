@@ -277,12 +277,40 @@ struct NormArgs {
     float eps;
 };
 
+// Eight consecutive elements of an array whose base is 16-byte aligned, from any column c on: the two 16-byte words that hold
+// them, shifted; by elements where the second would reach past the array's K elements.
+__device__ __forceinline__ Pack<8> load_shifted(const __nv_bfloat16* w, int c, int K) {
+    Pack<8> o;
+    const int s = c & 7;
+    if (c - s + 16 <= K) {
+        const Pack<8> lo = load_pack<8>(w + c - s), hi = load_pack<8>(w + c - s + 8);
+        uint32_t v[8] = {lo.w[0], lo.w[1], lo.w[2], lo.w[3], hi.w[0], hi.w[1], hi.w[2], hi.w[3]};
+#pragma unroll
+        for (int j = 0; j < 6; ++j) v[j] = s & 4 ? v[j + 2] : v[j];
+#pragma unroll
+        for (int j = 0; j < 5; ++j) v[j] = s & 2 ? v[j + 1] : v[j];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o.w[j] = __funnelshift_r(v[j], v[j + 1], (s & 1) * 16);
+    } else {
+        const uint16_t* e = reinterpret_cast<const uint16_t*>(w + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o.w[j] = e[2 * j] | ((uint32_t)e[2 * j + 1] << 16);
+    }
+    return o;
+}
+
 // ---- forward: blockDim = R groups of G threads, one row per group, V accesses of W elements per thread ---------------
 // The row stays packed (four registers per eight elements) and is widened again for each pass; the row's pointers are
 // formed once (inside the access loops every access had a 64-bit product of its own, and spilled).  8192 x 7168 with the
 // residual: 98 us with spills, 76-82 us without, 72 us at the measured copy rate.
-template <int W, int V, int THREADS, int CTAS, bool ADD, bool QUANT>
+//
+// SHIFT (W = 8): rows at any offset of the 16 bytes, the same in every array.  The 16-byte words that lie inside the row go
+// the ordinary way, from the row's first aligned column on, weight and bias shifted to them; the up to seven elements on
+// either side are the business of one thread each.  8192 x 7165 with the residual: 267 us by elements,
+// 102 us this way; 8192 x 15157 917 and 283 us.
+template <int W, int V, int THREADS, int CTAS, bool ADD, bool QUANT, bool SHIFT = false>
 __global__ void __launch_bounds__(THREADS, CTAS) layernorm_kernel(const NormArgs p) {
+    static_assert(!SHIFT || W == 8, "16-byte words");
     using T = typename Vals<W>::T;
     constexpr int N = Vals<W>::kN;
     __shared__ __align__(16) float2 red_all[8 * 128];   // a CTA holds at most eight groups
@@ -291,24 +319,35 @@ __global__ void __launch_bounds__(THREADS, CTAS) layernorm_kernel(const NormArgs
     const int64_t row = (int64_t)blockIdx.x * (blockDim.x / G) + g;
     if (row >= p.M) return;  // whole groups: nobody is left waiting at the group's barrier
     Group grp{red_all + 128 * g, G, 1 + g};
-    const int K = p.K;
-    const __nv_bfloat16* x = p.x + row * K;
-    __nv_bfloat16* res_row = p.res + row * K;
-    __nv_bfloat16* y_row = p.y + row * K;
-    int8_t* q_row = p.q + row * K;
+    // columns [c0, c0 + K) in accesses of W
+    const int c0 = SHIFT ? min(p.K, (int)(-(reinterpret_cast<intptr_t>(p.x + row * p.K) >> 1) & 7)) : 0;
+    const int K = SHIFT ? (p.K - c0) & ~7 : p.K;
+    const __nv_bfloat16* x = p.x + row * p.K + c0;
+    __nv_bfloat16* res_row = p.res + row * p.K + c0;
+    __nv_bfloat16* y_row = p.y + row * p.K + c0;
+    int8_t* q_row = p.q + row * p.K + c0;
+    // SHIFT: this thread's single element, as an offset from c0: the head's for threads 0..7, the tail's for 8..15
+    const int single = t < 8 ? t - c0 : K + t - 8;
+    const bool has_single = SHIFT && (t < 8 ? t < c0 : t < 16 && c0 + single < p.K);
+    float one = 0.0f;
     Pack<W> a[V];
     Pack<W> w1, b1;                      // a thread with one access has its weight and bias requested with the row
+    auto weights_of = [&](const __nv_bfloat16* w, int c) -> Pack<W> {
+        if constexpr (SHIFT) return load_shifted(w, c0 + c, p.K);
+        else return load_pack<W>(w + c);
+    };
 #pragma unroll
     for (int j = 0; j < V; ++j) {
         const int c = (t + j * G) * W;
         if (c < K) {
             a[j] = load_pack<W>(x + c);
             if constexpr (V == 1) {
-                w1 = load_pack<W>(p.w + c);
-                b1 = load_pack<W>(p.b + c);
+                w1 = weights_of(p.w, c);
+                b1 = weights_of(p.b, c);
             }
         }
     }
+    if (has_single) one = __bfloat162float(x[single]);
     T acc = all<T>(0.0f);
     if constexpr (ADD) {
         Pack<W> r[V];
@@ -326,6 +365,11 @@ __global__ void __launch_bounds__(THREADS, CTAS) layernorm_kernel(const NormArgs
                 store_pack<W>(res_row + c, a[j]);
             }
         }
+        if (has_single) {
+            const __nv_bfloat16 sum = __float2bfloat16_rn(add(__bfloat162float(res_row[single]), one));
+            res_row[single] = sum;
+            one = __bfloat162float(sum);
+        }
     }
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -334,7 +378,9 @@ __global__ void __launch_bounds__(THREADS, CTAS) layernorm_kernel(const NormArgs
             for (int i = 0; i < N; ++i) acc = add(acc, value<W>(a[j], i));
         }
     }
-    const float mean = __fdiv_rn(grp.sum(total(acc)), (float)K);
+    float part = total(acc);
+    if (SHIFT) part = add(part, one);
+    const float mean = __fdiv_rn(grp.sum(part), (float)p.K);
     acc = all<T>(0.0f);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -346,14 +392,20 @@ __global__ void __launch_bounds__(THREADS, CTAS) layernorm_kernel(const NormArgs
             }
         }
     }
-    const float rstd = rstd_of(grp.sum(total(acc)), K, p.eps);
+    part = total(acc);
+    if (has_single) part = fma(add(one, -mean), add(one, -mean), part);
+    const float rstd = rstd_of(grp.sum(part), p.K, p.eps);
     if (t == 0) {
         p.mean[row] = mean;
         p.rstd[row] = rstd;
     }
+    if (has_single) {
+        const int c = c0 + single;
+        one = fma(mul(add(one, -mean), rstd), __bfloat162float(p.w[c]), __bfloat162float(p.b[c]));   // y from here on
+    }
     // y of access j; the quantiser evaluates it twice (largest magnitude, codes) rather than hold it
     auto y_of = [&](int j, int c, T (&y)[N]) {
-        const Pack<W> w = V == 1 ? w1 : load_pack<W>(p.w + c), b = V == 1 ? b1 : load_pack<W>(p.b + c);
+        const Pack<W> w = V == 1 ? w1 : weights_of(p.w, c), b = V == 1 ? b1 : weights_of(p.b, c);
 #pragma unroll
         for (int i = 0; i < N; ++i)
             y[i] = fma(mul(add(value<W>(a[j], i), all<T>(-mean)), all<T>(rstd)), value<W>(w, i), value<W>(b, i));
@@ -371,8 +423,9 @@ __global__ void __launch_bounds__(THREADS, CTAS) layernorm_kernel(const NormArgs
                 store_pack<W>(y_row + c, o);
             }
         }
+        if (has_single) y_row[single] = __float2bfloat16_rn(one);
     } else {
-        float top = 0.0f;
+        float top = has_single ? fabsf(one) : 0.0f;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             const int c = (t + j * G) * W;
@@ -395,6 +448,7 @@ __global__ void __launch_bounds__(THREADS, CTAS) layernorm_kernel(const NormArgs
                 store_codes<W>(q_row + c, y, inv);
             }
         }
+        if (has_single) q_row[single] = (int8_t)quant_rn(one, inv);
     }
 }
 
@@ -694,12 +748,12 @@ int access_width(int K, const P*... ptrs) {
     return K % 8 == 0 && bits % 16 == 0 ? 8 : K % 2 == 0 && bits % 4 == 0 ? 2 : 1;
 }
 
-template <int W, int V, int THREADS, int CTAS, bool ADD, bool QUANT>
+template <int W, int V, int THREADS, int CTAS, bool ADD, bool QUANT, bool SHIFT = false>
 int launch_norm(NormArgs p, cudaStream_t st) {
     p.T = group_threads((p.K + W - 1) / W, V);
     // narrow rows share a CTA of up to 256 threads: one row each, at most 8 rows
     const int R = p.T >= 256 ? 1 : 256 / p.T;
-    layernorm_kernel<W, V, THREADS, CTAS, ADD, QUANT><<<(unsigned)(((int64_t)p.M + R - 1) / R), R * p.T, 0, st>>>(p);
+    layernorm_kernel<W, V, THREADS, CTAS, ADD, QUANT, SHIFT><<<(unsigned)(((int64_t)p.M + R - 1) / R), R * p.T, 0, st>>>(p);
     return check_launch("layernorm");
 }
 
@@ -733,17 +787,31 @@ int opt_in(Kernel kernel, bool (&done)[64], const char* what) {
     return 0;
 }
 
-// Few rows (no more than two per SM) take one wide access per thread, for latency (8 x 7168 with the quantiser: 7.3 us with
-// four accesses, 4 us with one); more rows take four (8192 x 7168 with the residual: 121 us with one, 83-99 with two,
-// 76-82 with four).
+// Whether a row begins at the same offset of the 16 bytes in all arrays (the codes': of 8 bytes), and weight and bias at 0
+template <bool ADD, bool QUANT>
+bool same_offset(const NormArgs& p) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(p.x), wb = reinterpret_cast<uintptr_t>(p.w) | reinterpret_cast<uintptr_t>(p.b);
+    auto differs = [&](const void* q) { return ((x ^ reinterpret_cast<uintptr_t>(q)) & 15) != 0; };
+    if ((wb & 15) || (ADD && differs(p.res))) return false;
+    return QUANT ? (((x >> 1) ^ reinterpret_cast<uintptr_t>(p.q)) & 7) == 0 : !differs(p.y);
+}
+
+// Few rows (no more than two per SM, or 6144 elements per SM) take one wide access per thread, for latency (8 x 7168 with
+// the quantiser: 7.3 us with four accesses, 4 us with one; 600 x 1000: 4.2 and 3.6 us); more rows take four (8192 x 7168 with
+// the residual: 121 us with one, 83-99 with two, 76-82 with four; 2000 x 1000: 5.9 us with one, 4.9 with four).
 template <bool ADD, bool QUANT>
 int dispatch_norm(const NormArgs& p, cudaStream_t st) {
     int w = access_width(p.K, p.x, p.w, p.b, (const __nv_bfloat16*)p.res, (const __nv_bfloat16*)p.y);
     if (QUANT && w == 8 && (reinterpret_cast<uintptr_t>(p.q) & 7)) w = 2;
     if (QUANT && w == 2 && (reinterpret_cast<uintptr_t>(p.q) & 1)) w = 1;
+    const int sms = sm_count();
+    const bool few = p.M <= 2 * sms || (int64_t)p.M * p.K <= (int64_t)6144 * sms;
     if (w == 8) {
-        if (p.K <= 8192 && p.M <= 2 * sm_count()) return launch_norm<8, 1, 1024, 1, ADD, QUANT>(p, st);
+        if (p.K <= 8192 && few) return launch_norm<8, 1, 1024, 1, ADD, QUANT>(p, st);
         if (p.K <= 16384) return launch_norm<8, 4, 512, 2, ADD, QUANT>(p, st);
+    } else if (p.K >= 64 && p.K <= 16384 && same_offset<ADD, QUANT>(p)) {
+        if (p.K <= 8192 && few) return launch_norm<8, 1, 1024, 1, ADD, QUANT, true>(p, st);
+        return launch_norm<8, 4, 512, 1, ADD, QUANT, true>(p, st);
     } else if (w == 2) {
         if (p.K <= 8192) return launch_norm<2, 4, 1024, 1, ADD, QUANT>(p, st);
         if (p.K <= 16384) return launch_norm<2, 8, 1024, 1, ADD, QUANT>(p, st);

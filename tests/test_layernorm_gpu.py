@@ -31,7 +31,7 @@ def weights(k, seed):
 
 SHAPES = [(1, 1), (1, 8), (3, 7), (5, 16), (2, 255), (33, 256), (7, 1001), (9, 1000), (4, 2047), (3, 4096), (3, 4104),
           (2, 4099), (65, 7168), (2, 8192), (2, 8200), (2, 8193), (1, 16384), (2, 16383), (2, 16392), (1, 20001), (1000, 40),
-          (300, 128), (40, 520)]
+          (300, 128), (40, 520), (400, 1001), (1300, 1003), (700, 2066), (333, 4097), (5, 65), (2, 71)]
 
 
 def y_slack(a, mean, rstd, w, b, k):
@@ -79,7 +79,8 @@ def test_constant_rows_have_the_bias_as_output(ext):
     assert ((rstd.cpu().double() * EPS ** 0.5 - 1).abs() <= 8 * U).all()
 
 
-@pytest.mark.parametrize("m,k", [(1, 8), (3, 7), (9, 1000), (7, 1001), (5, 7168), (2, 16392), (1, 20001)])
+@pytest.mark.parametrize("m,k", [(1, 8), (3, 7), (9, 1000), (7, 1001), (5, 7168), (2, 16392), (1, 20001), (1300, 1003),
+                                 (700, 2066), (4, 8195)])
 @pytest.mark.parametrize("add", [False, True])
 def test_layernorm_quant_codes_and_scales(ext, m, k, add):
     x, (w, b) = rows(m, k, 11), weights(k, 12)
