@@ -67,6 +67,13 @@ int to_int(int64_t v, const char* what) {
 Tensor fresh(const Tensor& like, at::IntArrayRef sizes, c10::ScalarType dtype) {
     return Tensor(at::detail::empty_cuda(sizes, dtype, like.device(), c10::nullopt));
 }
+// Dense piece of an allocation that several small outputs share: each allocation of its own costs a call about a microsecond.
+Tensor piece(const Tensor& whole, int64_t offset, at::IntArrayRef sizes) {
+    auto impl = c10::make_intrusive<c10::TensorImpl>(c10::Storage(whole.storage()), whole.key_set(), whole.dtype());
+    impl->set_storage_offset(offset);
+    impl->set_sizes_contiguous(sizes);
+    return Tensor(std::move(impl));
+}
 
 struct Rows {
     int M, N;
@@ -737,7 +744,8 @@ std::vector<Tensor> layernorm_impl(c10::optional<Tensor> res, Tensor x, Tensor w
     const NormShape n = check_norm(x, w, b, res);
     c10::cuda::CUDAGuard guard(x.device());
     auto y = fresh(x, x.sizes(), torch::kBFloat16);
-    auto mean = fresh(x, {n.M}, torch::kFloat32), rstd = fresh(x, {n.M}, torch::kFloat32);
+    const Tensor stats = fresh(x, {2 * (int64_t)n.M}, torch::kFloat32);
+    Tensor mean = piece(stats, 0, {n.M}), rstd = piece(stats, n.M, {n.M});
     check_status(launch_layernorm(res.has_value() ? res->data_ptr() : nullptr, x.data_ptr(), w.data_ptr(), b.data_ptr(),
                                   y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), n.M, n.N, (float)eps, as_stream(stream_ptr)));
     return {y, mean, rstd};
@@ -754,8 +762,8 @@ std::vector<Tensor> layernorm_quant_impl(c10::optional<Tensor> res, Tensor x, Te
     const NormShape n = check_norm(x, w, b, res);
     c10::cuda::CUDAGuard guard(x.device());
     auto q = fresh(x, x.sizes(), torch::kInt8);
-    auto s = fresh(x, {n.M, 1}, torch::kFloat32);
-    auto mean = fresh(x, {n.M}, torch::kFloat32), rstd = fresh(x, {n.M}, torch::kFloat32);
+    const Tensor stats = fresh(x, {3 * (int64_t)n.M}, torch::kFloat32);
+    Tensor s = piece(stats, 0, {n.M, 1}), mean = piece(stats, n.M, {n.M}), rstd = piece(stats, 2 * (int64_t)n.M, {n.M});
     check_status(launch_layernorm_quant(res.has_value() ? res->data_ptr() : nullptr, x.data_ptr(), w.data_ptr(), b.data_ptr(),
                                         q.data_ptr(), s.data_ptr(), mean.data_ptr(), rstd.data_ptr(), n.M, n.N, (float)eps,
                                         as_stream(stream_ptr)));
@@ -779,7 +787,8 @@ std::vector<Tensor> layernorm_backward_stream(Tensor dy, Tensor x, Tensor mean, 
     const Tensor& rstd_c = flat_scale(rstd, n.M, "rstd", x);
     c10::cuda::CUDAGuard guard(x.device());
     auto dx = fresh(x, x.sizes(), torch::kBFloat16);
-    auto dw = fresh(x, {n.N}, torch::kFloat32), db = fresh(x, {n.N}, torch::kFloat32);
+    const Tensor sums = fresh(x, {2 * (int64_t)n.N}, torch::kFloat32);
+    Tensor dw = piece(sums, 0, {n.N}), db = piece(sums, n.N, {n.N});
     const dsv4_stream_t st = as_stream(stream_ptr);
     const int64_t bytes = dsv4_layernorm_backward_workspace(n.M, n.N);
     Tensor ws = workspace_on(st, bytes, x);
