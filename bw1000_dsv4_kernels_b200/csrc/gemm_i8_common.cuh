@@ -75,9 +75,10 @@ struct Params {
     int act;
     int inter;
     // gradient epilogues: resid is the incoming gradient (dy or dh), C the fp32 gradient of z with row stride ldc (a
-    // multiple of four; a gated problem's ups start at column `up_col`), and row_top[row] collects the largest |dz * sb| of
-    // the row as the bits of a non-negative float
+    // multiple of four; a gated problem's ups start at column `up_col`), and row_top[row][slot] gets the largest |dz * sb|
+    // that the tile (or half of one) of that slot has in the row, as the bits of a non-negative float; every slot is written
     unsigned* row_top;
+    int top_slots;
     int up_col;
     // fused CTA-pair kernel: rows of B per tile, gates and ups together (a multiple of 32, of 64 when gated)
     int tile_n;

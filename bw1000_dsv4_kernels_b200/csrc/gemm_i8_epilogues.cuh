@@ -443,7 +443,8 @@ __device__ __forceinline__ void reduce_partials_fused(const Params& p, const uin
                 }
 #pragma unroll
                 for (int o = kGroups >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-                if (g == 0 && top != 0) atomicMax(p.row_top + m0 + c, top);
+                if (g == 0 && it < items && n0 < p.N)
+                    p.row_top[(int64_t)(m0 + c) * p.top_slots + n0 / (kGated ? 64 : 128)] = top;
             } else if (ok) {
                 if (kReads && p.resid != nullptr) {
                     const float2 r0 = bf16x2_to_f32x2(res[u].x), r1 = bf16x2_to_f32x2(res[u].y);

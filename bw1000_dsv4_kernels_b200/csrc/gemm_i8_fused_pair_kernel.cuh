@@ -1,5 +1,5 @@
-// Private part of gemm_i8_sm100.cu: the CTA-pair kernel behind w8a8_linear, w8a8_gated and their gradients for more than
-// 256 tokens.  Pairs, pipeline and barriers are those of gemm_i8_pair_kernel; what differs:
+// Private part of gemm_i8_sm100.cu: the CTA-pair kernel behind w8a8_linear, w8a8_gated and their gradients wherever
+// the weight-streaming kernels are not faster (fused_few, stream_blocks_splits).  Pairs, pipeline and barriers are those of gemm_i8_pair_kernel; what differs:
 //
 //   * The tile is 256 rows by p.tile_n rows of B, chosen per launch (fused_tile_n): with one tile per pair at a time, a
 //     problem of 224 tiles on 74 pairs takes four rounds for 3.03 rounds of work at a width of 256.
@@ -282,7 +282,7 @@ gemm_i8_fused_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
                 }
             }
             if constexpr (kGrad) {
-                if (row_ok && top != 0) atomicMax(p.row_top + row, top);
+                if (row_ok) p.row_top[(int64_t)row * p.top_slots + 2 * nt + turn] = top;
             }
             ptx::tc_fence_before_sync();  // the accumulator reads above are ordered before the release below
             __syncwarp();

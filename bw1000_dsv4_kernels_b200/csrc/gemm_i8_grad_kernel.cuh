@@ -14,7 +14,7 @@
 //
 // Pairs of CTAs, tiles of 256 x 256, pipeline and barriers as in gemm_i8_pair_kernel; a tile walks the K blocks twice.
 // With both accumulators taken by one tile, the drain does not overlap the next tile's MMAs (its loads do).  Short sums feel
-// it: at N = 134, K = 7568 the kernel takes 24 us for 37 MB of dx.  4096 x 7168 over N = 4096: 187 us = 2.57 POPS of int8 work.
+// it: at N = 134, K = 7568 the kernel takes 24 us for 37 MB of dx.  4096 x 7168 over N = 4096: 174 us = 2.8 POPS of int8 work.
 #ifndef W8A8_GEMM_I8_GRAD_KERNEL_CUH
 #define W8A8_GEMM_I8_GRAD_KERNEL_CUH
 

@@ -220,7 +220,7 @@ int active_clusters(Kernel kernel, int size, int smem, ClusterCounts& cached) {
 }
 template <int NTOK, int EPI>
 int launch_stream_variant(const CUtensorMap& tmW, const CUtensorMap& tmX, const Params& p, int n_tiles, int splits,
-                          bool follows, cudaStream_t st) {
+                          cudaStream_t st) {
     using L = StreamSmem<NTOK>;
     static_assert(L::kDynamic <= 227 * 1024, "shared memory limit");
     static bool opted_in[64] = {};
@@ -245,7 +245,7 @@ int launch_stream_variant(const CUtensorMap& tmW, const CUtensorMap& tmX, const 
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = overlap_previous_kernel() || follows ? 2 : 1;
+    cfg.numAttrs = overlap_previous_kernel() ? 2 : 1;
     const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_stream_kernel<NTOK, EPI>, tmW, tmX, p);
     if (err != cudaSuccess) {
         cudaGetLastError();  // clear the sticky launch error
@@ -264,7 +264,7 @@ int stream_pair_active_clusters(int splits) {
 
 template <int EPI>
 int launch_stream_pair(const CUtensorMap& tmW, const CUtensorMap& tmX, const Params& p, int n_tiles, int splits,
-                       bool follows, cudaStream_t st) {
+                       cudaStream_t st) {
     using L = StreamPairSmem;
     static_assert(L::kDynamic <= 227 * 1024, "shared memory limit");
     static bool opted_in[64] = {};
@@ -285,7 +285,7 @@ int launch_stream_pair(const CUtensorMap& tmW, const CUtensorMap& tmX, const Par
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = overlap_previous_kernel() || follows ? 2 : 1;
+    cfg.numAttrs = overlap_previous_kernel() ? 2 : 1;
     const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_stream_pair_kernel<EPI>, tmW, tmX, p);
     if (err != cudaSuccess) {
         cudaGetLastError();  // clear the sticky launch error
@@ -388,6 +388,8 @@ int launch_fused_pair(const GemmArgs& a, Params p, cudaStream_t st) {
     const int w_rows = is_gated(EPI) ? 2 * a.N : a.N, tiles_m = (a.M + 255) / 256;
     p.tile_n = fused_tile_n(tiles_m, w_rows, is_gated(EPI) ? 64 : 32, pairs);
     const int out_n = is_gated(EPI) ? p.tile_n / 2 : p.tile_n;
+    p.top_slots = 2 * ((a.N + out_n - 1) / out_n);   // a tile's chunks go to two warps per row in turn
+    if (a.top_slots != nullptr) *a.top_slots = p.top_slots;
     CUtensorMap tmA, tmB;
     if (int rc = make_tile_map(&tmA, a.A, (uint64_t)a.M, (uint64_t)a.K, BM)) return rc;
     if (int rc = make_tile_map(&tmB, a.B, (uint64_t)w_rows, (uint64_t)a.K, (uint32_t)(p.tile_n / 2))) return rc;
@@ -403,7 +405,7 @@ int launch_fused_pair(const GemmArgs& a, Params p, cudaStream_t st) {
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = overlap_previous_kernel() || a.follows ? 1 : 0;
+    cfg.numAttrs = overlap_previous_kernel() ? 1 : 0;
     const cudaError_t err = cudaLaunchKernelEx(&cfg, gemm_i8_fused_pair_kernel<EPI, ACT>, tmA, tmB, p);
     if (err != cudaSuccess) {
         cudaGetLastError();  // clear the sticky launch error
@@ -423,7 +425,7 @@ int launch_stream_blocks(const GemmArgs& a, Params p, int blocks, int pair_tiles
     CUtensorMap tmW, tmX;
     if (int rc = make_tile_map(&tmW, a.B, (uint64_t)w_rows, (uint64_t)a.K, is_gated(EPI) ? 64 : 128)) return rc;
     if (int rc = make_tile_map(&tmX, a.A, (uint64_t)a.M, (uint64_t)a.K, (uint32_t)(p.block_m / 2))) return rc;  // a CTA's half of the tokens
-    return launch_stream_pair<EPI>(tmW, tmX, p, pair_tiles * blocks, splits, a.follows, st);
+    return launch_stream_pair<EPI>(tmW, tmX, p, pair_tiles * blocks, splits, st);
 }
 
 // Whether a K split over `splits` CTAs or pairs pays for a block of so many tokens: a K block costs 0.3 us, the split saves
@@ -458,12 +460,14 @@ int stream_blocks_splits(int M, int pair_tiles, int blocks, int k_blocks) {
 // Dense problems: the kernel by the number of tokens and tiles.  A gated weight [2 N, K] gives N outputs, and each weight
 // tile takes half its rows from the gates and half from the ups, so its N counts twice.
 template <int EPI>
-int gemm_i8_dense(const GemmArgs& a, const Params& p, int bn, cudaStream_t st) {
+int gemm_i8_dense(const GemmArgs& a, Params p, int bn, cudaStream_t st) {
     constexpr bool kGated = is_gated(EPI);
     const int sms = sm_count();
     const int w_rows = kGated ? 2 * a.N : a.N;
     CUtensorMap tmA, tmB;
     const int k_blocks = (a.K + BK - 1) / BK;
+    p.top_slots = kGated ? (a.N + 63) / 64 : (a.N + 127) / 128;   // the streaming kernels' tiles; launch_fused_pair has its own
+    if (a.top_slots != nullptr) *a.top_slots = p.top_slots;
     // Few tokens: stream the weight once, tokens on the MMA's N axis, K split over a cluster
     if (a.M <= 256 && a.npeers == 0) {
         if (EPI == kEpiPlain && a.M > 128 && a.N >= 256) {
@@ -487,11 +491,11 @@ int gemm_i8_dense(const GemmArgs& a, const Params& p, int bn, cudaStream_t st) {
             rc4 = make_tile_map(&tmB, a.A, (uint64_t)a.M, (uint64_t)a.K, (uint32_t)ntok);  // tokens
             if (rc4) return rc4;
             switch (ntok) {
-                case 16: return launch_stream_variant<16, EPI>(tmA, tmB, p, n_tiles, splits, a.follows, st);
-                case 32: return launch_stream_variant<32, EPI>(tmA, tmB, p, n_tiles, splits, a.follows, st);
-                case 64: return launch_stream_variant<64, EPI>(tmA, tmB, p, n_tiles, splits, a.follows, st);
-                case 128: return launch_stream_variant<128, EPI>(tmA, tmB, p, n_tiles, splits, a.follows, st);
-                default: return launch_stream_variant<256, EPI>(tmA, tmB, p, n_tiles, splits, a.follows, st);
+                case 16: return launch_stream_variant<16, EPI>(tmA, tmB, p, n_tiles, splits, st);
+                case 32: return launch_stream_variant<32, EPI>(tmA, tmB, p, n_tiles, splits, st);
+                case 64: return launch_stream_variant<64, EPI>(tmA, tmB, p, n_tiles, splits, st);
+                case 128: return launch_stream_variant<128, EPI>(tmA, tmB, p, n_tiles, splits, st);
+                default: return launch_stream_variant<256, EPI>(tmA, tmB, p, n_tiles, splits, st);
             }
         }
     }

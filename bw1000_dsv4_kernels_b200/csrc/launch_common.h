@@ -73,8 +73,8 @@ struct GemmArgs {
     int64_t ldr = 0;
     int act = 0;                   // enum Activation in activations.cuh
     unsigned* row_top = nullptr;   // gradient epilogues (3 linear, 4 gated; resid is the incoming gradient, C is fp32)
+    int* top_slots = nullptr;      // where to say how many slots each row of row_top has (two per 64 rows of B at most)
     int up_col = 0;                // gated gradient: first column of the ups in C
-    bool follows = false;          // launched to overlap the kernel before it, whatever the thread's option says
     // Test hook, zero through every public entry point: the tile producers of the launch issue no
     // loads and every bounded wait gives up after test_wait_limit_ns, so the kernel's give-up path runs.
     int test_withhold_loads = 0;

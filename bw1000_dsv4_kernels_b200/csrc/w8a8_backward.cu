@@ -4,12 +4,12 @@
 //   dx    = (dz * sb) W                      the gradient of the dequantised activations
 //   dbias = sum over rows of dz              fp32
 //
-// Three steps: the forward's GEMM with a gradient epilogue writes dz in fp32 and each row's largest |dz * sb|
+// Three steps: the forward's GEMM with a gradient epilogue writes dz in fp32 and, per row and tile, the largest |dz * sb|
 // (gemm_i8_epilogues.cuh); split_gradient_kernel puts dz * sb into two int8 digits per element and sums the columns;
-// gemm_i8_grad_kernel multiplies the digits with W and adds the column sums up.  The codes and scales of the forward are
-// all that has to be kept for it.  Each kernel is launched to start while the one before it drains: 333 x 1001 x 1040 with
-// bias takes 34 us, 41 us as five launches in a row.  Without an activation dz is dy itself: the first step is a pass over
-// dy for the rows' largest magnitudes.
+// gemm_i8_grad_kernel, or gemm_i8_grad_stream_kernel for few rows, multiplies the digits with W and adds the column sums up.
+// The codes and scales of the forward are all that has to be kept for it.  Each kernel is launched to start while the one
+// before it drains.  Without an activation dz is dy itself: the first step is a pass over dy for the rows' largest
+// magnitudes.
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 #include <cstdint>
@@ -47,12 +47,6 @@ __device__ __forceinline__ void load8(const __nv_bfloat16* p, int left, bool vec
     }
 }
 
-__global__ void __launch_bounds__(256) clear_row_top_kernel(unsigned* row_top, int M) {
-    ptx::grid_launch_dependents();
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < M) row_top[i] = 0u;
-}
-
 // row_top[row] = largest |dy * sb| of the row, as float bits: one CTA per row
 __global__ void __launch_bounds__(256) row_top_kernel(const __nv_bfloat16* dy, int64_t ldy, const float* __restrict__ sb, int N,
                                                       bool vec, unsigned* row_top) {
@@ -85,13 +79,14 @@ struct Columns {
     __host__ __device__ int pitch() const { return parts * part_pitch; }
 };
 
+// tops[row][slots] -> each row's largest magnitude, by every warp that needs it; row_top, where it is wanted, gets it once.
 // dz -> digits int8 [2][M][pitch] (hi, then lo; zeros behind each range), and with SUM the column sums of every block of
 // kSplitRows rows.  A warp takes 256 columns of every eighth row of the block, all its rows' loads at once.
 constexpr int kSplitRows = 32;
 constexpr int kSplitWarps = 8;
 template <typename T, bool SUM>
 __global__ void __launch_bounds__(32 * kSplitWarps) split_gradient_kernel(const T* dz, int64_t ld, const float* __restrict__ sb,
-                                                                          const unsigned* __restrict__ row_top, int M,
+                                                                          const unsigned* tops, int slots, unsigned* row_top, int M,
                                                                           Columns cols, bool vec, int8_t* digits,
                                                                           float* partial) {
     __shared__ float sums[SUM ? kSplitWarps : 1][SUM ? 264 : 1];
@@ -113,10 +108,26 @@ __global__ void __launch_bounds__(32 * kSplitWarps) split_gradient_kernel(const 
         const int r = r0 + i * kSplitWarps;
         const bool ok = r < M;
         load8(dz + (int64_t)(ok ? r : 0) * ld + c, ok ? left : 0, vec, v[i]);
-        inv[i] = ok ? digit_inverse(__uint_as_float(__ldcg(row_top + r))) : 0.0f;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) scale[j] = j < left ? __ldg(sb + w_row + j) : 0.0f;
+    // the rows' largest magnitudes, all rows' loads at once
+    unsigned top[kRows] = {};
+#pragma unroll 1
+    for (int s = lane; s < slots; s += 32) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int r = r0 + i * kSplitWarps;
+            if (r < M) top[i] = max(top[i], __ldcg(tops + (int64_t)r * slots + s));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+        const int r = r0 + i * kSplitWarps;
+        top[i] = __reduce_max_sync(0xffffffffu, top[i]);
+        inv[i] = r < M ? digit_inverse(__uint_as_float(top[i])) : 0.0f;
+        if (row_top != nullptr && col_block == 0 && lane == 0 && r < M) row_top[r] = top[i];
+    }
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
         const int r = r0 + i * kSplitWarps;
@@ -157,7 +168,7 @@ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 
 struct Layout {
     Columns cols;
     int row_blocks;
-    int64_t digits, dz, row_top, partial, total;   // offsets and size in bytes
+    int64_t digits, dz, tops, row_top, partial, total;   // offsets and size in bytes
 };
 Layout layout(int M, int N, bool gated, bool recompute, bool dbias) {
     auto up = [](int64_t v) { return (v + 255) / 256 * 256; };
@@ -169,24 +180,23 @@ Layout layout(int M, int N, bool gated, bool recompute, bool dbias) {
     const int64_t pitch = l.cols.pitch();
     l.digits = 0;
     l.dz = l.digits + up(2 * (int64_t)M * pitch);
-    l.row_top = l.dz + (recompute ? up(4 * (int64_t)M * pitch) : 0);
+    l.tops = l.dz + (recompute ? up(4 * (int64_t)M * pitch) : 0);
+    // the narrowest tile has 64 rows of W and two slots
+    l.row_top = l.tops + (recompute ? up(4 * (int64_t)M * 2 * ((N + 63) / 64)) : 0);
     l.partial = l.row_top + up(4 * (int64_t)M);
     l.total = l.partial + (dbias ? up(4 * (int64_t)l.row_blocks * N) : 0);
     return l;
 }
 
 template <typename T>
-int split(const T* dz, int64_t ld, const BackwardArgs& a, const Layout& l, const unsigned* row_top, int8_t* digits,
-          float* partial, cudaStream_t st) {
+int split(const T* dz, int64_t ld, const BackwardArgs& a, const Layout& l, const unsigned* tops, int slots, unsigned* row_top,
+          int8_t* digits, float* partial, cudaStream_t st) {
     const bool vec = (ld * sizeof(T)) % 16 == 0 && aligned16(dz);
     const int64_t blocks = (int64_t)((l.cols.pitch() + 255) / 256) * l.row_blocks;
     if (blocks > INT32_MAX) return fail(DSV4_ERR_ARG, "w8a8 backward: too many rows");
-    const dim3 grid((unsigned)blocks);
-    return a.dbias != nullptr
-               ? launch_after(split_gradient_kernel<T, true>, grid, dim3(32 * kSplitWarps), 0, st, "w8a8 backward", dz, ld, a.sb,
-                              row_top, a.M, l.cols, vec, digits, partial)
-               : launch_after(split_gradient_kernel<T, false>, grid, dim3(32 * kSplitWarps), 0, st, "w8a8 backward", dz, ld, a.sb,
-                              row_top, a.M, l.cols, vec, digits, partial);
+    auto kernel = a.dbias != nullptr ? split_gradient_kernel<T, true> : split_gradient_kernel<T, false>;
+    return launch_after(kernel, dim3((unsigned)blocks), dim3(32 * kSplitWarps), 0, st, "w8a8 backward", dz, ld, a.sb, tops, slots,
+                        row_top, a.M, l.cols, vec, digits, partial);
 }
 
 }  // namespace
@@ -205,20 +215,21 @@ int w8a8_backward(const BackwardArgs& a, void* workspace, cudaStream_t st) {
     const __nv_bfloat16* dy = static_cast<const __nv_bfloat16*>(a.dy);
     if (recompute) {
         float* dz = reinterpret_cast<float*>(ws + l.dz);
-        clear_row_top_kernel<<<(a.M + 255) / 256, 256, 0, st>>>(row_top, a.M);
-        if (int rc = check_launch("w8a8 backward")) return rc;
         GemmArgs g{};
         g.A = a.A; g.B = a.B; g.sa = a.sa; g.sb = a.sb; g.C = dz;
         g.M = a.M; g.N = l.cols.part_rows; g.K = a.K; g.E = 1; g.ldc = l.cols.pitch(); g.sa_groups = 1;
-        g.epilogue = a.gated ? 4 : 3; g.bias = a.bias; g.resid = a.dy; g.ldr = a.ldy; g.act = a.act; g.row_top = row_top;
+        g.epilogue = a.gated ? 4 : 3; g.bias = a.bias; g.resid = a.dy; g.ldr = a.ldy; g.act = a.act;
         g.up_col = l.cols.part_pitch;
-        g.follows = true;
+        unsigned* tops = reinterpret_cast<unsigned*>(ws + l.tops);
+        int slots = 0;
+        g.row_top = tops;
+        g.top_slots = &slots;
         if (int rc = gemm_i8(g, st)) return rc;
-        if (int rc = split(dz, (int64_t)l.cols.pitch(), a, l, row_top, digits, partial, st)) return rc;
+        if (int rc = split(dz, (int64_t)l.cols.pitch(), a, l, tops, slots, row_top, digits, partial, st)) return rc;
     } else {
         row_top_kernel<<<a.M, 256, 0, st>>>(dy, a.ldy, a.sb, a.N, a.ldy % 8 == 0 && aligned16(dy), row_top);
         if (int rc = check_launch("w8a8 backward")) return rc;
-        if (int rc = split(dy, a.ldy, a, l, row_top, digits, partial, st)) return rc;
+        if (int rc = split(dy, a.ldy, a, l, row_top, 1, nullptr, digits, partial, st)) return rc;
     }
     GradientArgs d;
     d.digits = digits; d.row_top = row_top; d.W = a.B; d.dx = a.dx;
