@@ -739,11 +739,15 @@ int gemm_i8_gradient(const GradientArgs& a, cudaStream_t st) {
     p.partial = a.partial;
     p.row_blocks = a.row_blocks;
     p.dbias = a.dbias;
+    // rows of a block: as few as still fill half the SMs with clusters of eight, since a CTA's load is its digits' (83 rows,
+    // gated 15696 x 96: 49 us with 128, 42 with 16; 128 rows, 4096 x 512: 26 and 22)
+    int rows = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : 128;
+    while (rows > 16 && (int64_t)((a.K + 127) / 128) * ((a.M + rows - 1) / rows) * 16 <= sm_count()) rows /= 2;
     bool launched;
-    const int rc = a.M <= 16   ? launch_grad_stream<16>(a, p, st, launched)
-                   : a.M <= 32 ? launch_grad_stream<32>(a, p, st, launched)
-                   : a.M <= 64 ? launch_grad_stream<64>(a, p, st, launched)
-                               : launch_grad_stream<128>(a, p, st, launched);
+    const int rc = rows == 16   ? launch_grad_stream<16>(a, p, st, launched)
+                   : rows == 32 ? launch_grad_stream<32>(a, p, st, launched)
+                   : rows == 64 ? launch_grad_stream<64>(a, p, st, launched)
+                                : launch_grad_stream<128>(a, p, st, launched);
     if (rc != 0 || launched) return rc;
     CUtensorMap tmD, tmW;
     if (int rc = make_tile_map(&tmD, a.digits, (uint64_t)2 * a.M, (uint64_t)pitch, BM)) return rc;

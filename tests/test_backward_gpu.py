@@ -42,7 +42,7 @@ SHAPES = [(1, 8, 16), (3, 40, 48), (17, 127, 128), (64, 128, 144), (100, 257, 27
           (257, 1000, 400), (300, 129, 2064), (513, 600, 528), (700, 2305, 784),
           # sums split over clusters for 16, 32, 64 and 128 rows and several blocks of them; rows of a few elements
           (1, 2000, 2064), (16, 1500, 1040), (30, 4000, 144), (40, 3000, 528), (128, 4100, 400), (300, 2600, 400),
-          (200, 300, 6160), (500, 3, 400), (260, 1, 48)]
+          (200, 300, 6160), (500, 3, 400), (260, 1, 48), (83, 5000, 96), (50, 2600, 256)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -182,12 +182,12 @@ def test_more_rows_than_a_grid_dimension_of_row_blocks(ext):
     want = ref.linear_backward(dy.cpu()[pick], a.cpu()[pick], sa.cpu()[pick], w, sw, b, "silu")[0]
     assert ((dx.cpu()[pick].double() - want).norm(dim=1) <= 4e-3 * want.norm(dim=1)).all()
     dz = (dy.double() * ref.dact((a.double() @ w.cuda().double().T) * sa.double() * sw.cuda().double() + b.cuda().double(), "silu"))
-    # 65537 block sums in four chains of 16384 additions, 32 rows each
-    assert ((db.double() - dz.sum(0)).abs() <= U * (16384 + 60) * dz.abs().sum(0)).all()
+    # 65537 block sums in sixteen chains of at most 4097 additions, 32 rows each
+    assert ((db.double() - dz.sum(0)).abs() <= U * (4097 + 60) * dz.abs().sum(0)).all()
 
 
-def test_two_runs_other_streams_and_captured_replays(ext):
-    m, i, k = 200, 136, 272
+@pytest.mark.parametrize("m,i,k", [(200, 136, 272), (16, 700, 528), (700, 136, 272)])
+def test_two_runs_other_streams_and_captured_replays(ext, m, i, k):
     (a, sa), (w, sw) = ref.tokens(m, k, 1), ref.weight(2 * i, k, 2)
     b = ref.bf16((2 * i,), 3)
     a, sa, w, sw, b = cuda(a, sa, w, sw, b)
