@@ -436,12 +436,12 @@ bool split_pays(int tokens, int splits, int k_blocks) { return k_blocks * (split
 // Whether few tokens with a fused epilogue go to the weight-streaming kernel rather than the tiles of 256 tokens, whose drain
 // is faster and whose tiles are as narrow as 64 outputs.  Measured (tiles / streaming, with bias, GELU, residual): 128 x 4096
 // x 1024 5.6 / 9.0 us, x 7168 14.7 / 14.8; 128 x 18432 x 4096 28.2 / 29.2; 65 x 18432 x 4096 27.2 / 24.0; 65 x 4096 x 1024
-// 6.2 / 7.6; 59 x 3000 x 64 6.6 / 9.0, x 512 7.3 / 6.6; 33 x 18432 x 1024 14.4 / 9.7; 200 x 200 x 7168 15.3 (pairs) / 12.4.
-bool fused_few(int M, int w_rows, int n_tiles, int splits, int k_blocks) {
+// 6.2 / 7.6; 59 x 3000 x 64 6.6 / 9.0, x 512 7.3 / 6.6; 33 x 18432 x 1024 14.4 / 9.7; 256 x 400 x 4096 12.4 / 8.3 (blocks of 32).
+bool fused_few(int M, int ntok, int w_rows, int n_tiles, int splits, int k_blocks) {
     const bool few_tiles = n_tiles <= 37;
     if (M <= 64) return M <= 32 || k_blocks > 2 || !few_tiles;
-    if (M > 128 && w_rows >= 256) return false;
-    return few_tiles ? split_pays(M, splits, k_blocks) : M <= 96;
+    if (M > 128 && w_rows >= 256 && ntok > 64) return false;
+    return few_tiles ? split_pays(min(M, ntok), splits, k_blocks) : M <= 96;
 }
 
 // K split of more tokens over the streaming kernel's pairs, or 0 where the tile kernel is faster.  Measured (tiles / this
@@ -484,18 +484,26 @@ int gemm_i8_dense(const GemmArgs& a, Params p, int bn, cudaStream_t st) {
         if (splits > 8) splits = 8;
         if (splits > k_blocks) splits = k_blocks;
         if (splits < 1) splits = 1;
-        if (EPI == kEpiPlain || fused_few(a.M, w_rows, n_tiles, splits, k_blocks)) {
-            const int ntok = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : a.M <= 128 ? 128 : 256;
+        int ntok = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : a.M <= 128 ? 128 : 256, tiles = n_tiles;
+        if constexpr (EPI != kEpiPlain) {
+            // blocks of fewer tokens while the clusters would fill less than half the SMs (200 x 200 x 8192 12.7 -> 7.3 us,
+            // 90 x 60 x 2048 7.6 -> 5.5; 17 x 1000 x 4096 5.9 -> 6.2 with 16, hence not below 32)
+            while (ntok > 32 && tiles * splits * 2 <= sms) {
+                ntok /= 2;
+                tiles = n_tiles * ((a.M + ntok - 1) / ntok);
+            }
+        }
+        if (EPI == kEpiPlain || fused_few(a.M, ntok, w_rows, n_tiles, splits, k_blocks)) {
             int rc4 = make_tile_map(&tmA, a.B, (uint64_t)w_rows, (uint64_t)a.K, kGated ? 64 : 128);   // weights
             if (rc4) return rc4;
             rc4 = make_tile_map(&tmB, a.A, (uint64_t)a.M, (uint64_t)a.K, (uint32_t)ntok);  // tokens
             if (rc4) return rc4;
             switch (ntok) {
-                case 16: return launch_stream_variant<16, EPI>(tmA, tmB, p, n_tiles, splits, st);
-                case 32: return launch_stream_variant<32, EPI>(tmA, tmB, p, n_tiles, splits, st);
-                case 64: return launch_stream_variant<64, EPI>(tmA, tmB, p, n_tiles, splits, st);
-                case 128: return launch_stream_variant<128, EPI>(tmA, tmB, p, n_tiles, splits, st);
-                default: return launch_stream_variant<256, EPI>(tmA, tmB, p, n_tiles, splits, st);
+                case 16: return launch_stream_variant<16, EPI>(tmA, tmB, p, tiles, splits, st);
+                case 32: return launch_stream_variant<32, EPI>(tmA, tmB, p, tiles, splits, st);
+                case 64: return launch_stream_variant<64, EPI>(tmA, tmB, p, tiles, splits, st);
+                case 128: return launch_stream_variant<128, EPI>(tmA, tmB, p, tiles, splits, st);
+                default: return launch_stream_variant<256, EPI>(tmA, tmB, p, tiles, splits, st);
             }
         }
     }
