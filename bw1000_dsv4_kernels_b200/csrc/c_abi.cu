@@ -425,8 +425,8 @@ int launch_layernorm_backward(const void* dy, const void* x, const void* mean, c
     DSV4_REQUIRE_PTR("layernorm_backward", w);
     DSV4_REQUIRE_PTR("layernorm_backward", dx);
     DSV4_REQUIRE_PTR("layernorm_backward", workspace);
-    if (workspace_bytes < layernorm_backward_workspace(M, N) || (reinterpret_cast<uintptr_t>(workspace) & 3))
-        return fail(DSV4_ERR_ARG, "layernorm_backward: the workspace is smaller than dsv4_layernorm_backward_workspace or not 4-byte aligned");
+    if (workspace_bytes < layernorm_backward_workspace(M, N) || (reinterpret_cast<uintptr_t>(workspace) & 15))
+        return fail(DSV4_ERR_ARG, "layernorm_backward: the workspace is smaller than dsv4_layernorm_backward_workspace or not 16-byte aligned");
     return layernorm_backward(dy, x, mean, rstd, w, dres, dx, dw, db, workspace, M, N, cs(stream));
 }
 

@@ -501,7 +501,7 @@ struct NormBwdArgs {
     const __nv_bfloat16* w;
     const __nv_bfloat16* dres;   // null: none
     __nv_bfloat16* dx;
-    float* partial;              // [gridDim.x][2][K]: this CTA's share of dw and db
+    float* partial;              // [gridDim.x][2][K]: this CTA's share of dw and db; 16-byte aligned
     int M, K, T;
     int slot_bytes;
 };
@@ -649,7 +649,7 @@ __global__ void __launch_bounds__(THREADS, 1) layernorm_backward_kernel(const No
                 if constexpr (W == 1) {
                     to[c] = dw[j][i];
                     to[K + c] = db[j][i];
-                } else {   // c and K are even: 8-byte aligned
+                } else {   // c, K and the partial's alignment allow 8 bytes
                     *reinterpret_cast<float2*>(to + c + 2 * i) = dw[j][i];
                     *reinterpret_cast<float2*>(to + K + c + 2 * i) = db[j][i];
                 }

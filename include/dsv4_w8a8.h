@@ -299,7 +299,8 @@ DSV4_API int launch_layernorm_quant(void* res, const void* x, const void* w, con
 /* Gradients of launch_layernorm: x bf16 [M,N] is the row that was normalised (the updated residual where there was
  * one), dy bf16 [M,N]; dres bf16 [M,N] or null is the gradient that reaches the same row past the norm and is added.
  * dx bf16 [M,N]; dw, db fp32 [N], summed over the rows in an order that depends on M, N and the device only.
- * workspace: dsv4_layernorm_backward_workspace(M, N) bytes of device memory, free again once the launch has run. */
+ * workspace: dsv4_layernorm_backward_workspace(M, N) bytes of device memory, 16-byte aligned, free again once the launches
+ * have run. */
 DSV4_API int64_t dsv4_layernorm_backward_workspace(int M, int N);
 DSV4_API int launch_layernorm_backward(const void* dy, const void* x, const void* mean, const void* rstd, const void* w,
                        const void* dres, void* dx, void* dw, void* db, void* workspace, int64_t workspace_bytes, int M,

@@ -102,6 +102,20 @@ def test_c_abi_refuses_before_it_touches_a_device():
         assert nback(**bad) == 1
 
 
+def test_layernorm_backward_refuses_a_workspace_that_its_stores_do_not_fit():
+    """shares of the column sums are stored eight bytes at a time, so four-byte alignment is not enough"""
+    lib = pkg.c_abi()
+    lib.dsv4_last_error.restype = ctypes.c_char_p
+    lib.dsv4_layernorm_backward_workspace.restype = ctypes.c_int64
+    one, null = ctypes.c_void_p(16), ctypes.c_void_p(0)
+    size = lib.dsv4_layernorm_backward_workspace(4, 8)
+
+    for offset in (1, 2, 4, 8, 12):
+        rc = lib.launch_layernorm_backward(one, one, one, one, one, null, one, one, one, ctypes.c_void_p(4096 + offset),
+                                           ctypes.c_longlong(size), 4, 8, null)
+        assert rc == 1 and b"16-byte aligned" in lib.dsv4_last_error(), (offset, rc, lib.dsv4_last_error())
+
+
 def test_operators_refuse_cpu_tensors():
     ext = pkg.dsv4_native_ext
     (a, sa), (w, sw) = ref.tokens(2, 16, 1), ref.weight(4, 16, 2)
