@@ -8,6 +8,7 @@
 #include <cuda_runtime.h>
 #include <cuda_bf16.h>
 #include <cstdint>
+#include "gradient_digits.cuh"
 #include "launch_common.h"
 #include "sm100_ptx.cuh"
 #include "w8a8_arith.cuh"
@@ -75,10 +76,10 @@ struct Params {
     int act;
     int inter;
     // gradient epilogues: resid is the incoming gradient (dy or dh), C the fp32 gradient of z with row stride ldc (a
-    // multiple of four; a gated problem's ups start at column `up_col`), and row_top[row][slot] gets the largest |dz * sb|
-    // that the tile (or half of one) of that slot has in the row, as the bits of a non-negative float; every slot is written
-    unsigned* row_top;
-    int top_slots;
+    // multiple of four; a gated problem's ups start at column `up_col`), and row_sizes[row][slot] gets the size of dz * sb
+    // in the columns that the tile (or half of one) of that slot has; every slot is written
+    RowSize* row_sizes;
+    int size_slots;
     int up_col;
     // fused CTA-pair kernel: rows of B per tile, gates and ups together (a multiple of 32, of 64 when gated)
     int tile_n;

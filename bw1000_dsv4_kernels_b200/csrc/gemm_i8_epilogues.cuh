@@ -4,8 +4,8 @@
 //   gated        the tile holds a block of gate columns and the same block of up columns (two loads of weight rows, I
 //                rows apart), so one thread has g and u of the same output: h = act(zg) * zu   -> bf16
 //   gradients    z is computed again from the same codes and scales: dz = dy * act'(z), or dg = dh * zu * act'(zg) and
-//                du = dh * act(zg), stored in fp32, together with each row's largest |dz * sb| (the scale of the
-//                fixed-point form in which the gradient product takes it)
+//                du = dh * act(zg), stored in fp32, together with each row's size (largest |dz * sb| and their sum: the
+//                scale and the number of digits of the fixed-point form in which the gradient product takes it)
 //
 // Without bias, activation and residual, linear gives the bits of the plain epilogue.
 #ifndef W8A8_GEMM_I8_EPILOGUES_CUH
@@ -195,9 +195,6 @@ __device__ __forceinline__ void store_block(__nv_bfloat16* block, int64_t ld, co
     }
 }
 
-// larger magnitude, as bits: unlike fmaxf it keeps a NaN, which then reaches the whole row of the result
-__device__ __forceinline__ unsigned top_bits(unsigned top, float v) { return max(top, __float_as_uint(v) & 0x7fffffffu); }
-
 // 32 columns of scales or biases in this warp's shared memory (16-byte aligned), four at a time: the tensor cores take
 // nearly all of the shared memory's bandwidth for their operands, and one access per column and row made the GEMM 12 %
 // slower than its plain form.
@@ -251,16 +248,12 @@ __device__ __forceinline__ Row32 gated_values(const uint32_t (&g)[32], const uin
 __device__ __forceinline__ uint4 bits4(const float2& a, const float2& b) {
     return make_uint4(__float_as_uint(a.x), __float_as_uint(a.y), __float_as_uint(b.x), __float_as_uint(b.y));
 }
-__device__ __forceinline__ unsigned top_bits2(unsigned top, const float2& v, const float2& s) {
-    const float2 t = __fmul2_rn(v, s);
-    return top_bits(top_bits(top, t.x), t.y);
-}
 
-// dz of 32 columns -> the warp's block of dz (fp32, rows 16-byte aligned with room for whole chunks); returns the row's
-// largest |dz * sb| as bits, together with `top`
+// dz of 32 columns -> the warp's block of dz (fp32, rows 16-byte aligned with room for whole chunks); dz * sb is added to the
+// row's size
 template <int ACT>
-__device__ __forceinline__ unsigned linear_gradients(const uint32_t (&r)[32], float sa, Cols32 sb, Cols32 bias, const Row32& dy,
-                                                     float* block, int64_t ld, int rows, uint32_t* stage, int lane, unsigned top) {
+__device__ __forceinline__ void linear_gradients(const uint32_t (&r)[32], float sa, Cols32 sb, Cols32 bias, const Row32& dy,
+                                                     float* block, int64_t ld, int rows, uint32_t* stage, int lane, RowSize& size) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         uint4 out[4];
@@ -275,20 +268,19 @@ __device__ __forceinline__ unsigned linear_gradients(const uint32_t (&r)[32], fl
                 float2 slope;
                 act_value_slope2<ACT>(scaled2(r[e], r[e + 1], sa, two(s4, k), two(b4, k)), slope);
                 v[k] = __fmul2_rn(bf16x2_to_f32x2(dy.w[e >> 1]), slope);
-                top = top_bits2(top, v[k], two(s4, k));
+                size.add(__fmul2_rn(v[k], two(s4, k)));
             }
             out[i] = bits4(v[0], v[1]);
         }
         store_pieces(reinterpret_cast<char*>(block + 16 * half), 4 * ld, out, rows, 4, stage, lane);
     }
-    return top;
 }
 
 // dg and du of 32 outputs
 template <int ACT>
-__device__ __forceinline__ unsigned gated_gradients(const uint32_t (&g)[32], const uint32_t (&u)[32], float sa, Cols32 sg,
+__device__ __forceinline__ void gated_gradients(const uint32_t (&g)[32], const uint32_t (&u)[32], float sa, Cols32 sg,
                                                     Cols32 bg, Cols32 su, Cols32 bu, const Row32& dh, float* block_g,
-                                                    float* block_u, int64_t ld, int rows, uint32_t* stage, int lane, unsigned top) {
+                                                    float* block_u, int64_t ld, int rows, uint32_t* stage, int lane, RowSize& size) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         uint4 out_g[4], out_u[4];
@@ -305,7 +297,8 @@ __device__ __forceinline__ unsigned gated_gradients(const uint32_t (&g)[32], con
                 const float2 d = bf16x2_to_f32x2(dh.w[e >> 1]);
                 vg[k] = __fmul2_rn(__fmul2_rn(d, scaled2(u[e], u[e + 1], sa, two(su4, k), two(bu4, k))), slope);
                 vu[k] = __fmul2_rn(d, value);
-                top = top_bits2(top_bits2(top, vg[k], two(sg4, k)), vu[k], two(su4, k));
+                size.add(__fmul2_rn(vg[k], two(sg4, k)));
+                size.add(__fmul2_rn(vu[k], two(su4, k)));
             }
             out_g[i] = bits4(vg[0], vg[1]);
             out_u[i] = bits4(vu[0], vu[1]);
@@ -313,7 +306,6 @@ __device__ __forceinline__ unsigned gated_gradients(const uint32_t (&g)[32], con
         store_pieces(reinterpret_cast<char*>(block_g + 16 * half), 4 * ld, out_g, rows, 4, stage, lane);
         store_pieces(reinterpret_cast<char*>(block_u + 16 * half), 4 * ld, out_u, rows, 4, stage, lane);
     }
-    return top;
 }
 
 // Split-K epilogues of the weight-streaming kernels (see reduce_partials_and_store): the item's partials come through
@@ -343,7 +335,7 @@ __device__ __forceinline__ void reduce_partials_fused(const Params& p, const uin
     const bool vec_store = (p.ldc % 4 == 0) && ((reinterpret_cast<uintptr_t>(p.C) & 7) == 0);
     const bool res_vec = (p.ldr % 4 == 0) && ((reinterpret_cast<uintptr_t>(p.resid) & 7) == 0);
     const int items = (cols_hi - cols_lo) * kGroups;
-    // a warp's lanes stay together: the gradients' largest magnitudes are exchanged between them
+    // a warp's lanes stay together: the gradients' sizes are exchanged between them
     for (int it0 = tid; (it0 & ~31) < items; it0 += nthreads * U) {
         uint4 v[U][kHalves][MAXS];
         uint2 res[U];
@@ -428,7 +420,7 @@ __device__ __forceinline__ void reduce_partials_fused(const Params& p, const uin
             const bool ok = it < items && n < p.N;
             if constexpr (kGrad) {
                 // dz rows have room for whole tiles: four columns are stored, those at or beyond N with zeros
-                unsigned top = 0;
+                RowSize size = RowSize::none();
                 if (ok) {
                     float* dz = static_cast<float*>(p.C) + (int64_t)(m0 + c) * p.ldc + n;
 #pragma unroll
@@ -437,14 +429,14 @@ __device__ __forceinline__ void reduce_partials_fused(const Params& p, const uin
 #pragma unroll
                         for (int j = 0; j < 2; ++j) {
                             const int col = h * 64 + g * 4 + 2 * j;
-                            top = top_bits2(top, z[u][h][j], make_float2(sb_s[col], sb_s[col + 1]));
+                            size.add(__fmul2_rn(z[u][h][j], make_float2(sb_s[col], sb_s[col + 1])));
                         }
                     }
                 }
 #pragma unroll
-                for (int o = kGroups >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                for (int o = kGroups >> 1; o > 0; o >>= 1) size.add_lane(o);
                 if (g == 0 && it < items && n0 < p.N)
-                    p.row_top[(int64_t)(m0 + c) * p.top_slots + n0 / (kGated ? 64 : 128)] = top;
+                    p.row_sizes[(int64_t)(m0 + c) * p.size_slots + n0 / (kGated ? 64 : 128)] = size;
             } else if (ok) {
                 if (kReads && p.resid != nullptr) {
                     const float2 r0 = bf16x2_to_f32x2(res[u].x), r1 = bf16x2_to_f32x2(res[u].y);

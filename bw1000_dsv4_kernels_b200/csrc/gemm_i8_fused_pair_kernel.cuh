@@ -251,7 +251,7 @@ gemm_i8_fused_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
             }
             ptx::tc_fence_after_sync();
             const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + acc * 256;
-            unsigned top = 0;
+            RowSize size = RowSize::none();
             const float* col = cols;
 #pragma unroll 1
             for (int cc = turn; cc < chunks; cc += 2, col += kGated ? 64 : 32) {
@@ -275,14 +275,14 @@ gemm_i8_fused_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_
                     // dz has room for whole chunks; columns at or beyond N get zeros (their gradient was read as zero)
                     float* dz = static_cast<float*>(p.C) + (int64_t)row0 * p.ldc + n;
                     if constexpr (kGated)
-                        top = gated_gradients<ACT>(r, u, sa, {col}, {col + 128}, {col + 32}, {col + 160}, in, dz, dz + p.up_col,
-                                                   p.ldc, rows, stage, lane, top);
+                        gated_gradients<ACT>(r, u, sa, {col}, {col + 128}, {col + 32}, {col + 160}, in, dz, dz + p.up_col,
+                                             p.ldc, rows, stage, lane, size);
                     else
-                        top = linear_gradients<ACT>(r, sa, {col}, {col + 128}, in, dz, p.ldc, rows, stage, lane, top);
+                        linear_gradients<ACT>(r, sa, {col}, {col + 128}, in, dz, p.ldc, rows, stage, lane, size);
                 }
             }
             if constexpr (kGrad) {
-                if (row_ok) p.row_top[(int64_t)row * p.top_slots + 2 * nt + turn] = top;
+                if (row_ok) p.row_sizes[(int64_t)row * p.size_slots + 2 * nt + turn] = size;
             }
             ptx::tc_fence_before_sync();  // the accumulator reads above are ordered before the release below
             __syncwarp();

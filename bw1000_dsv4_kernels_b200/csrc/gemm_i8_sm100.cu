@@ -388,8 +388,8 @@ int launch_fused_pair(const GemmArgs& a, Params p, cudaStream_t st) {
     const int w_rows = is_gated(EPI) ? 2 * a.N : a.N, tiles_m = (a.M + 255) / 256;
     p.tile_n = fused_tile_n(tiles_m, w_rows, is_gated(EPI) ? 64 : 32, pairs);
     const int out_n = is_gated(EPI) ? p.tile_n / 2 : p.tile_n;
-    p.top_slots = 2 * ((a.N + out_n - 1) / out_n);   // a tile's chunks go to two warps per row in turn
-    if (a.top_slots != nullptr) *a.top_slots = p.top_slots;
+    p.size_slots = 2 * ((a.N + out_n - 1) / out_n);   // a tile's chunks go to two warps per row in turn
+    if (a.size_slots != nullptr) *a.size_slots = p.size_slots;
     CUtensorMap tmA, tmB;
     if (int rc = make_tile_map(&tmA, a.A, (uint64_t)a.M, (uint64_t)a.K, BM)) return rc;
     if (int rc = make_tile_map(&tmB, a.B, (uint64_t)w_rows, (uint64_t)a.K, (uint32_t)(p.tile_n / 2))) return rc;
@@ -466,8 +466,8 @@ int gemm_i8_dense(const GemmArgs& a, Params p, int bn, cudaStream_t st) {
     const int w_rows = kGated ? 2 * a.N : a.N;
     CUtensorMap tmA, tmB;
     const int k_blocks = (a.K + BK - 1) / BK;
-    p.top_slots = kGated ? (a.N + 63) / 64 : (a.N + 127) / 128;   // the streaming kernels' tiles; launch_fused_pair has its own
-    if (a.top_slots != nullptr) *a.top_slots = p.top_slots;
+    p.size_slots = kGated ? (a.N + 63) / 64 : (a.N + 127) / 128;   // the streaming kernels' tiles; launch_fused_pair has its own
+    if (a.size_slots != nullptr) *a.size_slots = p.size_slots;
     // Few tokens: stream the weight once, tokens on the MMA's N axis, K split over a cluster
     if (a.M <= 256 && a.npeers == 0) {
         if (EPI == kEpiPlain && a.M > 128 && a.N >= 256) {
@@ -604,7 +604,7 @@ int gemm_i8(const GemmArgs& a, cudaStream_t st) {
     if (p.ldc < a.N) return fail(DSV4_ERR_ARG, "w8a8_gemm: ldc smaller than N");
     p.bias = static_cast<const __nv_bfloat16*>(a.bias);
     p.resid = static_cast<const __nv_bfloat16*>(a.resid);
-    p.ldr = a.ldr; p.act = a.act; p.inter = a.N; p.row_top = a.row_top;
+    p.ldr = a.ldr; p.act = a.act; p.inter = a.N; p.row_sizes = static_cast<RowSize*>(a.row_sizes);
     p.up_col = a.up_col; p.tile_n = 256;
     if (a.epilogue != kEpiPlain && (grouped || a.out_i32 || a.npeers != 0))
         return fail(DSV4_ERR_ARG, "w8a8_linear: the fused epilogues exist for the dense GEMM with bf16 output");
@@ -700,7 +700,7 @@ int launch_grad_stream(const GradientArgs& a, const GradParams& p, cudaStream_t 
     if (blocks * (3 * splits - 2) < 20 * splits || splits == 0) return 0;
     launched = true;
     CUtensorMap tmD, tmW;
-    if (int rc = make_tile_map(&tmD, a.digits, (uint64_t)2 * a.M, (uint64_t)a.parts * a.part_pitch, ROWS)) return rc;
+    if (int rc = make_tile_map(&tmD, a.digits, (uint64_t)3 * a.M, (uint64_t)a.parts * a.part_pitch, ROWS)) return rc;
     if (int rc = make_tile_map(&tmW, a.W, (uint64_t)a.parts * a.part_rows, (uint64_t)a.K, 128)) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(clusters * splits), 1, 1);
@@ -732,7 +732,8 @@ int gemm_i8_gradient(const GradientArgs& a, cudaStream_t st) {
     if (!opt_in_shared_memory(gemm_i8_grad_kernel, L::kDynamic, opted_in))
         return fail(DSV4_ERR_LAUNCH, "w8a8 backward: cannot raise the dynamic shared memory limit");
     GradParams p = {};
-    p.row_top = a.row_top;
+    p.row_size = a.row_size;
+    p.wide = a.wide;
     p.dx = static_cast<__nv_bfloat16*>(a.dx);
     p.M = a.M; p.K = a.K;
     p.parts = a.parts; p.part_rows = a.part_rows; p.part_blocks = a.part_pitch / BK;
@@ -758,7 +759,7 @@ int gemm_i8_gradient(const GradientArgs& a, cudaStream_t st) {
                                 : launch_grad_stream<128>(a, p, st, launched);
     if (rc != 0 || launched) return rc;
     CUtensorMap tmD, tmW;
-    if (int rc = make_tile_map(&tmD, a.digits, (uint64_t)2 * a.M, (uint64_t)pitch, BM)) return rc;
+    if (int rc = make_tile_map(&tmD, a.digits, (uint64_t)3 * a.M, (uint64_t)pitch, BM)) return rc;
     if (int rc = make_tile_map(&tmW, a.W, (uint64_t)a.parts * a.part_rows, (uint64_t)a.K, 128)) return rc;
     const int64_t tiles = (int64_t)tiles_m * ((a.K + 255) / 256);
     int pairs = sm_count() / 2;

@@ -72,8 +72,8 @@ struct GemmArgs {
     const void* resid = nullptr;   // bf16 [M, N] with row stride ldr
     int64_t ldr = 0;
     int act = 0;                   // enum Activation in activations.cuh
-    unsigned* row_top = nullptr;   // gradient epilogues (3 linear, 4 gated; resid is the incoming gradient, C is fp32)
-    int* top_slots = nullptr;      // where to say how many slots each row of row_top has (two per 64 rows of B at most)
+    void* row_sizes = nullptr;     // gradient epilogues (3 linear, 4 gated; resid is the incoming gradient, C is fp32): RowSize
+    int* size_slots = nullptr;     // where to say how many slots each row of row_sizes has (two per 64 rows of B at most)
     int up_col = 0;                // gated gradient: first column of the ups in C
     // Test hook, zero through every public entry point: the tile producers of the launch issue no
     // loads and every bounded wait gives up after test_wait_limit_ns, so the kernel's give-up path runs.
@@ -82,8 +82,9 @@ struct GemmArgs {
 };
 int gemm_i8(const GemmArgs& a, cudaStream_t st);
 struct GradientArgs {
-    const void* digits;         // int8 [2][M][parts * part_pitch]: hi, then lo
-    const unsigned* row_top;    // [M] float bits
+    const void* digits;         // int8 [3][M][parts * part_pitch]: hi, mid, and lo for wide rows only
+    const unsigned* row_size;   // [M] packed_size (gradient_digits.cuh)
+    const unsigned char* wide;  // per block of 32 rows: whether it has a wide row; 8-byte aligned, zeros up to a multiple of eight
     const void* W;              // int8 [parts * part_rows, K]
     void* dx;                   // bf16 [M, K]
     int M, K, parts, part_rows, part_pitch;   // part_pitch: multiple of 128, zeros behind part_rows

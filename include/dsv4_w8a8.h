@@ -273,8 +273,9 @@ DSV4_API int launch_w8a8_gated(const void* A, const void* B, const void* sa, con
  * it has to keep); z is computed again from them.  dy bf16 [M, N] (gated: [M, I]) with row stride ldy.
  * dx bf16 [M,K]: the gradient of the dequantised activations A * sa (the quantiser is passed straight through);
  * dbias fp32 [N] (gated: [2*I]) or null: sums of dz over the rows.  The residual's gradient is dy itself.
- * Inside, each row of dz * sb is in 16-bit fixed point relative to its largest magnitude (a row that holds an infinity or
- * a NaN therefore gives a row of NaN); dz, the sums and the scales are fp32.  With DSV4_ACT_NONE A and sa are not read
+ * Inside, each row of dz * sb is in fixed point relative to its largest magnitude (a row that holds an infinity or a NaN
+ * therefore gives a row of NaN): off by at most 2^-16 of it, or by 2^-24 of it in rows whose typical magnitude (the square
+ * of the mean square root) is less than about 1 / 256 of it.  dz, the sums and the scales are fp32.  With DSV4_ACT_NONE A and sa are not read
  * and may be null.  At most 131071 weight rows.  Every result depends on the inputs, sizes and device only.
  * workspace: dsv4_w8a8_backward_workspace(M, weight rows, gated, act, dbias != null) bytes of device memory, 16-byte
  * aligned, free again once the launches have run. */

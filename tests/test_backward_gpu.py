@@ -134,6 +134,103 @@ def test_rows_are_scaled_by_themselves(ext):
         assert db.cpu()[11].isnan() and not db.cpu()[12].isfinite()
 
 
+def outlier_rows(m, n, w, seed):
+    """gradients of unit size with one element of 3000 in some rows, where the weight has a row of zeros: nothing of the
+    outlier reaches dx"""
+    w = w.clone()
+    w[5 % n] = 0
+    dy = ref.bf16((m, n), seed).float()
+    some = torch.arange(m) % 3 == 1
+    dy[some, 5 % n] = 3000.0
+    return dy.to(torch.bfloat16), w, some
+
+
+def check_dx_by_typical_size(dx, dx64, t, t_err, w):
+    """Half a step of the fixed point: two digits, or three where the typical size (the square of the mean root, every root
+    within 6 %) is below top / 256; either way at most 2^-8 of the typical size, or 2^-24 of top where that is more.  The
+    latter is what fp32 sums lose wherever the outlier meets a code that is not zero."""
+    top = t.abs().amax(1, keepdim=True)
+    typical = 1.06 ** 2 * t.abs().sqrt().mean(1, keepdim=True) ** 2
+    half_step = torch.maximum(torch.minimum(top * 2.0 ** -16, typical * 2.0 ** -8), top * 2.0 ** -24) * 1.01
+    wsum = w.double().abs()
+    slack = half_step * wsum.sum(0, keepdim=True) + (t_err + 4 * U * t.abs()) @ wsum
+    err = (dx.cpu().double() - dx64).abs()
+    assert (err <= ref.UBF * (dx64.abs() + slack) + slack).all(), float((err - ref.UBF * dx64.abs() - slack).max())
+    # in the 2-norm of a row: half a bf16 step, and twice the root mean square of the fixed point's error, which is uniform
+    # and independent from element to element (a third of half a step's square, times the codes' squares)
+    spread = half_step.squeeze(1) / 3 ** 0.5 * w.double().norm() + ((t_err + 4 * U * t.abs()) @ wsum).norm(dim=1)
+    assert (err.norm(dim=1) <= ref.UBF * dx64.norm(dim=1) + 2 * spread).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 600, 256), (14, 400, 528), (30, 700, 272), (64, 520, 400), (128, 4100, 400), (200, 300, 6160),
+                                   (300, 2600, 400), (257, 1000, 400), (700, 2305, 784), (1030, 400, 512), (5, 40, 48)])
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_rows_with_outliers_are_as_exact_as_the_others(ext, m, n, k, act):
+    """dx against the magnitudes that really enter it, as everywhere else, and the rows without outliers bit for bit what they
+    are without those neighbours"""
+    (a, sa), (w, sw) = ref.tokens(m, k, m), ref.weight(n, k, n)
+    dy, w, some = outlier_rows(m, n, w, 4)
+    b = torch.zeros(n, dtype=torch.bfloat16)
+    if act != "none":
+        b[5 % n] = 4.0   # the weight row of zeros: z is the bias, whose slope is about one
+    dx64, db64, t, dz = ref.linear_backward(dy, a, sa, w, sw, b, act)
+    dx, db = ext.w8a8_linear_backward(dy.cuda(), *cuda(a, w, sa, sw, b), act)
+    _, size = ref.project(a, sa, w, sw, b)
+    dz_err = dy.double().abs() * (DZ + 1.2 * 4 * U * size) if act != "none" else torch.zeros_like(dz)
+    check_db(db, db64, dz, dz_err)
+    check_dx_by_typical_size(dx, dx64, t, dz_err * sw.double(), w)
+    assert ((dx.cpu().double() - dx64).norm(dim=1) <= 4e-3 * dx64.norm(dim=1)).all()
+    calm = torch.where(some[:, None], torch.zeros_like(dy), dy)
+    dx2, _ = ext.w8a8_linear_backward(calm.cuda(), *cuda(a, w, sa, sw, b), act)
+    assert torch.equal(dx2.cpu()[~some].view(torch.int16), dx.cpu()[~some].view(torch.int16))
+
+
+@pytest.mark.parametrize("m,i,k", [(20, 300, 272), (300, 700, 528), (700, 1100, 784)])
+def test_gated_rows_with_outliers(ext, m, i, k):
+    """an outlier in the incoming gradient, whose gate and up rows of the weight are zero"""
+    (a, sa), (w, sw) = ref.tokens(m, k, m), ref.weight(2 * i, k, i)
+    w[7], w[i + 7] = 0, 0
+    b = torch.zeros(2 * i, dtype=torch.bfloat16)
+    b[7], b[i + 7] = 2.0, 1.0
+    dh = ref.bf16((m, i), 4).float()
+    dh[::2, 7] = 30000.0
+    dh = dh.to(torch.bfloat16)
+    dx64, db64, t, dz = ref.gated_backward(dh, a, sa, w, sw, b, "silu")
+    dx, db = ext.w8a8_gated_backward(dh.cuda(), *cuda(a, w, sa, sw, b), "silu")
+    z, size = ref.project(a, sa, w, sw, b)
+    g, u, size_g, size_u, d = z[:, :i], z[:, i:], size[:, :i], size[:, i:], dh.double().abs()
+    err_g = d * u.abs() * (DZ + 1.2 * 4 * U * size_g) + d * 1.13 * 4 * U * size_u
+    err_u = d * (DZ * (ref.act(g, "silu").abs() + 1e-6) + 1.13 * 4 * U * size_g)
+    check_dx_by_typical_size(dx, dx64, t, (torch.cat([err_g, err_u], 1) + 4 * U * dz.abs()) * sw.double(), w)
+    again = ext.w8a8_gated_backward(dh.cuda(), *cuda(a, w, sa, sw, b), "silu")
+    assert torch.equal(again[0].view(torch.int16), dx.view(torch.int16)) and torch.equal(again[1], db)
+
+
+def test_every_row_wide_at_many_tiles(ext):
+    """more tiles than pairs of CTAs, wide and calm blocks of rows in turn, captured and replayed"""
+    m, n, k = 5200, 520, 1808
+    (w, sw) = ref.weight(n, k, 2)
+    w[5] = 0
+    (a, sa) = ref.tokens(m, k, 3)
+    dy = ref.bf16((m, n), 4).float()
+    wide = (torch.arange(m) // 700) % 2 == 0
+    dy[wide, 5] = 3000.0
+    dy = dy.to(torch.bfloat16)
+    ad, wd, sad, swd, dyd = cuda(a, w, sa, sw, dy)
+    dx, _ = ext.w8a8_linear_backward(dyd, ad, wd, sad, swd)
+    want = ref.linear_backward(dy, a, sa, w, sw)[0]
+    assert ((dx.cpu().double() - want).norm(dim=1) <= 4e-3 * want.norm(dim=1)).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, _ = ext.w8a8_linear_backward(dyd, ad, wd, sad, swd)
+    for flip in (True, False):
+        dyd.copy_(dy.flip(0) if flip else dy)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.view(torch.int16), ext.w8a8_linear_backward(dyd, ad, wd, sad, swd)[0].view(torch.int16))
+    assert torch.equal(out.view(torch.int16), dx.view(torch.int16)) and ext.device_status() == 0
+
+
 def test_directional_difference_of_the_forward(ext):
     """dx and dbias of the kernels against central differences of the 64-bit forward, in the dequantised activations"""
     m, i, k, h = 9, 40, 96, 1e-5

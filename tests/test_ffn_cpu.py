@@ -55,6 +55,17 @@ def test_every_digit_pair_is_int8_and_gives_its_value_back():
     assert 131071 * 128 * 128 < 2 ** 31
 
 
+def test_three_digits_are_the_bytes_of_a_shifted_sum():
+    """w = 65536 hi + 256 mid + lo with signed digits: the bytes of w + 0x8080 are hi, mid + 128 and lo + 128 (mod 256)"""
+    top = 32639 * 256
+    w = torch.cat([torch.arange(-32639, 32640) * 256, torch.arange(-top - 2, top + 3, 61), torch.tensor([-top - 2, top + 2])])
+    s = w + 0x8080
+    signed = lambda b: torch.where(b >= 128, b - 256, b)   # noqa: E731
+    hi, mid, lo = signed((s >> 16) & 255), signed(((s >> 8) & 255) ^ 128), signed((s & 255) ^ 128)
+    assert torch.equal(65536 * hi + 256 * mid + lo, w)
+    assert hi.abs().max() <= 127 and (lo[:2 * 32639 + 1] == 0).all()
+
+
 def test_c_abi_refuses_before_it_touches_a_device():
     lib = pkg.c_abi()
     lib.dsv4_last_error.restype = ctypes.c_char_p
