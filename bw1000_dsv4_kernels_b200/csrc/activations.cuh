@@ -1,7 +1,9 @@
 // Activations of the fused linear and gated epilogues and their derivatives, fp32, two elements at a time: products and
-// sums as packed f32x2 instructions, exponential and reciprocal as the hardware's approximations, whose relative error
-// (about 2^-21 at the arguments where the result still matters) is far below the bf16 step of every output they reach.
-// A tile's epilogue evaluates 32768 of them per SM beside the tensor cores, so their instructions count.
+// sums as packed f32x2 instructions, exponential and reciprocal as the hardware's approximations.  Relative to itself a
+// value is off by at most 2^-15, most of it the rounding of the exponential's argument far from zero, and so is each of the
+// two terms of a slope: a bf16 result is rounded by 2^-8.  Values below about 1e-36, where the exponential or its
+// reciprocal leaves the normal numbers, become zero.  A tile's epilogue evaluates 32768 of them per SM beside the tensor
+// cores, so their instructions count.
 #pragma once
 #include <cuda_runtime.h>
 #include "w8a8_arith.cuh"
@@ -11,7 +13,6 @@ namespace w8a8 {
 // matches the order of the names in torch_ext.cpp and the DSV4_ACT_* constants
 enum Activation : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
 
-constexpr float kSqrtHalf = 0.70710678f;
 constexpr float kInvSqrt2Pi = 0.39894228f;
 constexpr float kGeluTanhC = 1.59576912f;   // 2 * sqrt(2 / pi): 0.5 * (1 + tanh(a)) = sigmoid(2 a)
 constexpr float kGeluCubic = 0.044715f;
@@ -35,20 +36,25 @@ __device__ __forceinline__ float2 sigmoid2(float2 z, float a) {
 }
 
 // Phi(z), the normal distribution function, and e = exp(-z^2 / 2), which Phi's formula needs anyway and the density is
-// made of.  1 - Phi(|z|) = 0.5 * erfc(|z| / sqrt 2) by Abramowitz and Stegun, Handbook of Mathematical Functions, formula
-// 7.1.26: a polynomial of degree five in 1 / (1 + 0.3275911 x) times exp(-x^2), off by at most 0.75e-7.  erfcf is exact
-// to the last bits but takes four times the instructions and branches on its argument, which made the drain of a
-// 7168-deep tile longer than its tensor-core work.
+// made of.  1 - Phi(|z|) = 0.5 * erfc(x) = exp(-x^2) * 0.5 * erfcx(x), x = |z| / sqrt 2, with 0.5 * erfcx as t times a
+// polynomial of degree six in t = 1 / (1 + 0.37339598 x) (the form of Hastings' approximations).  Constant and coefficients
+// were fitted here to the smallest largest relative error on 0 <= x <= 9.5, a linear program over them: 4.9e-7, 9e-7 with
+// fp32's roundings.  It is the relative error that counts: GELU far below zero is z times the tail, and a polynomial with an
+// absolute bound (0.75e-7) was off by 3.6e-3 of the value at -6, about what bf16 rounds.  erfcf is exact to the last bits
+// but takes four times the instructions and branches on its argument, which made the drain of a 7168-deep tile longer than
+// its tensor-core work.
 __device__ __forceinline__ float2 normal_cdf2(float2 z, float2& e) {
     const float2 a = make_float2(fabsf(z.x), fabsf(z.y));
-    const float2 d = __ffma2_rn(a, splat2(0.3275911f * kSqrtHalf), splat2(1.0f));
+    const float2 d = __ffma2_rn(a, splat2(0.26403083f), splat2(1.0f));
     const float2 t = make_float2(rcp_fast(d.x), rcp_fast(d.y));
     const float2 s = __fmul2_rn(__fmul2_rn(z, z), splat2(-0.5f * kLog2e));
     e = make_float2(exp2_fast(s.x), exp2_fast(s.y));
-    float2 q = __ffma2_rn(t, splat2(0.5f * 1.061405429f), splat2(0.5f * -1.453152027f));
-    q = __ffma2_rn(t, q, splat2(0.5f * 1.421413741f));
-    q = __ffma2_rn(t, q, splat2(0.5f * -0.284496736f));
-    q = __ffma2_rn(t, q, splat2(0.5f * 0.254829592f));
+    float2 q = __ffma2_rn(t, splat2(-0.0693054696f), splat2(0.203423122f));
+    q = __ffma2_rn(t, q, splat2(-0.0763239056f));
+    q = __ffma2_rn(t, q, splat2(0.148744691f));
+    q = __ffma2_rn(t, q, splat2(0.0804328837f));
+    q = __ffma2_rn(t, q, splat2(0.107843366f));
+    q = __ffma2_rn(t, q, splat2(0.105185018f));
     q = __fmul2_rn(__fmul2_rn(q, t), e);
     return make_float2(z.x > 0.0f ? 1.0f - q.x : q.x, z.y > 0.0f ? 1.0f - q.y : q.y);
 }

@@ -231,6 +231,41 @@ def test_every_row_wide_at_many_tiles(ext):
     assert torch.equal(out.view(torch.int16), dx.view(torch.int16)) and ext.device_status() == 0
 
 
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_slopes_keep_their_digits_far_from_zero(ext, act):
+    """act'(z) of one element per row, to bf16 of its two terms' magnitude: z is the bias, dx the element's digits times 127.
+    Each term has the relative error of the exponential, 2^-15.6 (arguments up to 88, four roundings), and less than 2^-19
+    beside it."""
+    hi = {"gelu": 9.0, "gelu_tanh": 9.0, "silu": 60.0}[act]
+    bits = torch.arange(0, 0x7F80, 8, dtype=torch.int32)
+    v = (bits << 16).view(torch.float32)
+    v = v[(v >= 2.0 ** -20) & (v <= hi)]
+    z = torch.cat([-v.flip(0), v])
+    z = torch.cat([z, torch.zeros(-z.numel() % 16)])
+    n = z.numel()
+    zd = z.double()
+    if act == "gelu":
+        terms = (0.5 * torch.erfc(-zd / 2 ** 0.5), zd * torch.exp(-0.5 * zd * zd) / (2 * torch.pi) ** 0.5)
+    else:
+        c = 2 * (2 / torch.pi) ** 0.5
+        arg, slope = (zd, 1.0) if act == "silu" else (c * (zd + 0.044715 * zd ** 3), c * (1 + 3 * 0.044715 * zd * zd))
+        p = torch.sigmoid(arg)
+        terms = (p, zd * p * torch.sigmoid(-arg) * slope)
+    want, size = sum(terms), sum(t.abs() for t in terms)
+    w = torch.diag(torch.full((n,), 127, dtype=torch.int8)).cuda()
+    one = torch.ones(n, device="cuda")
+    for rows in (range(0, n, n // 40), range(n)):   # weight streaming and tiles
+        rows = torch.tensor(list(rows))
+        m = rows.numel()
+        dy = torch.zeros((m, n), dtype=torch.bfloat16)
+        dy[torch.arange(m), rows] = 1.0
+        a = torch.zeros((m, n), dtype=torch.int8)
+        dx, _ = ext.w8a8_linear_backward(dy.cuda(), a.cuda(), w, one[:m].contiguous(), one, z.to(torch.bfloat16).cuda(), act)
+        got = dx.cpu().double()[torch.arange(m), rows] / 127
+        err = (got - want[rows]).abs()
+        assert (err <= ref.UBF * want[rows].abs() + 1.01 * 2.0 ** -15 * size[rows]).all(), float((err / size[rows]).max())
+
+
 def test_directional_difference_of_the_forward(ext):
     """dx and dbias of the kernels against central differences of the 64-bit forward, in the dequantised activations"""
     m, i, k, h = 9, 40, 96, 1e-5

@@ -112,6 +112,35 @@ def test_large_scales_and_special_values_pass_through(ext):
     assert ((huge - torch.clamp(z, min=0)).abs() <= 2.0 ** -8 * z.abs() + 1.0).all()
 
 
+def tail_arguments(lo, hi):
+    """every fourth bf16 number from -hi to hi with magnitudes from lo on"""
+    bits = torch.arange(0, 0x7F80, 4, dtype=torch.int32)
+    v = (bits << 16).view(torch.float32)
+    v = v[(v >= lo) & (v <= hi)]
+    return torch.cat([-v.flip(0), v])
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_activations_keep_their_digits_far_from_zero(ext, act):
+    """the value itself to bf16, also where it is tiny: z is the bias, the weight is zero.  Relative error of the value:
+    the exponential's argument is at most 88 with four roundings of 2^-24, which is 2^-15.6 of the exponential; the reciprocal
+    and the polynomial add less than 2^-19."""
+    z = tail_arguments(2.0 ** -20, {"gelu": 12.0, "gelu_tanh": 9.0, "silu": 80.0}[act])
+    n = z.numel()
+    b = z.to(torch.bfloat16).cuda()
+    for m in (1, 300):   # weight streaming and tiles
+        a, w = torch.zeros((m, 16), dtype=torch.int8, device="cuda"), torch.zeros((n, 16), dtype=torch.int8, device="cuda")
+        y = ext.w8a8_linear(a, w, torch.ones((m, 1), device="cuda"), torch.ones(n, device="cuda"), b, act)
+        zd = z.double()
+        if act == "gelu_tanh":   # 1 + tanh loses every digit far below zero
+            want = zd * torch.sigmoid(2 * (2 / torch.pi) ** 0.5 * (zd + 0.044715 * zd ** 3))
+        else:
+            want = ref.act(zd, act)
+        err = (y.cpu().double() - want).abs()
+        bad = err > (ref.UBF + 1.01 * 2.0 ** -15) * want.abs()
+        assert not bad.any(), (z[bad[0]][:5], (err / want.abs())[0].max())
+
+
 def test_residual_rows_of_a_broadcast_or_wrong_shape_are_refused(ext):
     (a, sa), (w, sw) = ref.tokens(4, 64, 1), ref.weight(32, 64, 2)
     a, sa, w, sw = cuda(a, sa, w, sw)
