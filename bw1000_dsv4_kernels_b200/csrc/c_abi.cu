@@ -179,6 +179,32 @@ DSV4_API int dsv4_test_gemm_wait_expiry(const void* A, const void* B, const void
     return gemm_i8(a, cs(stream));
 }
 
+// The same for launch_w8a8_linear (nothing is written by the kernel for more than 256 rows) and for the gradient product of
+// launch_w8a8_linear_backward without an activation (nothing by the kernel for many rows, dx is unspecified after the one
+// for few rows).
+DSV4_API int dsv4_test_linear_wait_expiry(const void* A, const void* B, const void* sa, const void* sb, int act, void* C, int M,
+                                          int N, int K, unsigned long long wait_limit_ns, dsv4_stream_t stream) {
+    GemmArgs a{};
+    a.A = A; a.B = B; a.sa = static_cast<const float*>(sa); a.sb = static_cast<const float*>(sb); a.C = C;
+    a.offsets = nullptr; a.M = M; a.N = N; a.K = K; a.E = 1; a.sa_groups = 1; a.out_i32 = 0;
+    a.epilogue = 1; a.act = act;
+    a.test_withhold_loads = 1;
+    a.test_wait_limit_ns = wait_limit_ns ? wait_limit_ns : 1000000ull;
+    return gemm_i8(a, cs(stream));
+}
+DSV4_API int dsv4_test_backward_wait_expiry(const void* dy, const void* B, const void* sb, void* dx, void* workspace,
+                                            int64_t workspace_bytes, int M, int N, int K, unsigned long long wait_limit_ns,
+                                            dsv4_stream_t stream) {
+    if (workspace_bytes < w8a8_backward_workspace(M, N, false, false, false) || K % 16 != 0 || N > 131071)
+        return fail(DSV4_ERR_ARG, "dsv4_test_backward_wait_expiry: sizes");
+    BackwardArgs a{};
+    a.dy = dy; a.ldy = N; a.B = B; a.sb = static_cast<const float*>(sb); a.dx = dx;
+    a.M = M; a.N = N; a.K = K;
+    a.test_withhold_loads = 1;
+    a.test_wait_limit_ns = wait_limit_ns ? wait_limit_ns : 1000000ull;
+    return w8a8_backward(a, workspace, cs(stream));
+}
+
 int launch_w8a8_gemm_v5(const void* A, const void* B, const void* sa, const void* sb, void* C, int M, int N,
                         int K, dsv4_stream_t stream) {
     return launch_w8a8_gemm(A, B, sa, sb, C, M, N, K, stream);

@@ -46,6 +46,7 @@ struct GradParams {
     int row_blocks;
     float* dbias;
     unsigned long long wait_limit_ns;
+    int withhold_loads;        // as in Params
 };
 
 // Not zero if one of the rows [row0, row0 + ROWS) is in a block of 32 with a wide row; row0 is a multiple of ROWS.  One load:
@@ -136,7 +137,7 @@ gemm_i8_grad_kernel(const __grid_constant__ CUtensorMap tmD, const __grid_consta
 
     if (warp == 0) {
         // ---------------- TMA producer (both CTAs) ----------------
-        if (ptx::elect_one()) {
+        if (!p.withhold_loads && ptx::elect_one()) {
             ptx::grid_dependency_wait();   // the digits come from the kernel before
             int stage = 0;
             uint32_t phase = 0;
@@ -428,7 +429,7 @@ gemm_i8_grad_stream_kernel(const __grid_constant__ CUtensorMap tmD, const __grid
 
     const int blocks = p.parts * p.part_blocks;
     const int nb0 = (int)((int64_t)blocks * split / S), nb1 = (int)((int64_t)blocks * (split + 1) / S);
-    const int prologue = (nb1 - nb0) < STAGES ? (nb1 - nb0) : STAGES;
+    const int prologue = p.withhold_loads ? 0 : (nb1 - nb0) < STAGES ? (nb1 - nb0) : STAGES;
     auto load_weight = [&](uint32_t dst, int nb, uint32_t bar) {
         const int part = nb >= p.part_blocks ? 1 : 0;
         ptx::tma_load_2d(dst, &tmW, k0, part * p.part_rows + (nb - part * p.part_blocks) * BK, bar);
@@ -470,7 +471,7 @@ gemm_i8_grad_stream_kernel(const __grid_constant__ CUtensorMap tmD, const __grid
     const int passes = wide ? 2 : 1;   // both first digits at once, then the third
 
     if (warp == 0) {
-        if (ptx::elect_one()) {
+        if (!p.withhold_loads && ptx::elect_one()) {
             int stage = prologue == STAGES ? 0 : prologue;
             uint32_t phase = prologue == STAGES ? 1u : 0u;
             for (int it = prologue; it < passes * (nb1 - nb0); ++it) {

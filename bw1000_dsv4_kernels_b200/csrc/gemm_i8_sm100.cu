@@ -146,6 +146,12 @@ volatile int* host_status_mirror() {
     if (mirror[dev] != nullptr) return mirror[dev];
     std::lock_guard<std::mutex> lock(mu);
     if (mirror[dev] != nullptr) return mirror[dev];
+    // a stream under capture (any thread's) must not be disturbed by what follows, none of which is for the graph
+    struct Relaxed {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        Relaxed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+        ~Relaxed() { cudaThreadExchangeStreamCaptureMode(&mode); }
+    } relaxed;
     int* host = nullptr;
     int* device_view = nullptr;
     if (cudaHostAlloc(reinterpret_cast<void**>(&host), sizeof(int), cudaHostAllocMapped) != cudaSuccess ||
@@ -559,6 +565,17 @@ int gemm_i8_dense(const GemmArgs& a, Params p, int bn, cudaStream_t st) {
 
 }  // namespace
 
+int refuse_after_failed_wait() {
+    volatile int* mirror = host_status_mirror();
+    const int site = mirror != nullptr ? *mirror : 0;
+    if (site == 0) return 0;
+    *mirror = 0;
+    static thread_local char msg[160];
+    snprintf(msg, sizeof msg, "w8a8_gemm: an earlier kernel on this device gave up a bounded wait (site %d); "
+             "nothing was launched; dsv4_device_status reads and clears the device's word", site);
+    return fail(DSV4_ERR_DEVICE_WAIT, msg);
+}
+
 int gemm_i8(const GemmArgs& a, cudaStream_t st) {
     const bool grouped = a.offsets != nullptr || a.masked_m != nullptr;
     if (a.M < 0 || a.N < 0 || a.K < 0) return fail(DSV4_ERR_ARG, "w8a8_gemm: negative size");
@@ -580,17 +597,7 @@ int gemm_i8(const GemmArgs& a, cudaStream_t st) {
             return fail(DSV4_ERR_ARG, "grouped_gemm: group scales need K % 128 == 0 and sa_groups == K / 128");
     }
 
-    // a kernel launched earlier on this device gave up a bounded wait: say so once instead of launching
-    if (volatile int* mirror = host_status_mirror()) {
-        const int site = *mirror;
-        if (site != 0) {
-            *mirror = 0;
-            static thread_local char msg[160];
-            snprintf(msg, sizeof msg, "w8a8_gemm: an earlier kernel on this device gave up a bounded wait (site %d); "
-                     "nothing was launched; dsv4_device_status reads and clears the device's word", site);
-            return fail(DSV4_ERR_DEVICE_WAIT, msg);
-        }
-    }
+    if (int rc = refuse_after_failed_wait()) return rc;
 
     Params p;
     p.wait_limit_ns = a.test_wait_limit_ns ? a.test_wait_limit_ns : ptx::kWaitLimitNs;
@@ -737,7 +744,8 @@ int gemm_i8_gradient(const GradientArgs& a, cudaStream_t st) {
     p.dx = static_cast<__nv_bfloat16*>(a.dx);
     p.M = a.M; p.K = a.K;
     p.parts = a.parts; p.part_rows = a.part_rows; p.part_blocks = a.part_pitch / BK;
-    p.wait_limit_ns = ptx::kWaitLimitNs;
+    p.wait_limit_ns = a.test_wait_limit_ns ? a.test_wait_limit_ns : ptx::kWaitLimitNs;
+    p.withhold_loads = a.test_withhold_loads;
     const int pitch = a.parts * a.part_pitch;
     // groups of m-tiles whose two digits take at most 32 MB, as in gemm_i8
     const int tiles_m = (a.M + 255) / 256;

@@ -81,6 +81,9 @@ struct GemmArgs {
     unsigned long long test_wait_limit_ns = 0;
 };
 int gemm_i8(const GemmArgs& a, cudaStream_t st);
+// Before the launches of an operator whose kernels wait on barriers: if one launched earlier on this device gave up such a
+// wait, says so once (DSV4_ERR_DEVICE_WAIT).  The device's word has its mirror in host memory from the first call on.
+int refuse_after_failed_wait();
 struct GradientArgs {
     const void* digits;         // int8 [3][M][parts * part_pitch]: hi, mid, and lo for wide rows only
     const unsigned* row_size;   // [M] packed_size (gradient_digits.cuh)
@@ -91,6 +94,8 @@ struct GradientArgs {
     const float* partial;       // null, or [row_blocks][parts * part_rows]: column sums of blocks of rows
     int row_blocks;
     float* dbias;               // their sums
+    int test_withhold_loads = 0;                   // as in GemmArgs
+    unsigned long long test_wait_limit_ns = 0;
 };
 int gemm_i8_gradient(const GradientArgs& a, cudaStream_t st);
 int scale_convert(const void* acc, const void* sa, const void* sb, void* out, int M, int N,
@@ -135,6 +140,8 @@ struct BackwardArgs {
     void* dx;              // bf16 [M, K]
     float* dbias;          // fp32 [N] or null
     int M, N, K;
+    int test_withhold_loads = 0;                   // of the gradient product, as in GemmArgs
+    unsigned long long test_wait_limit_ns = 0;
 };
 int64_t w8a8_backward_workspace(int M, int N, bool gated, bool recompute, bool dbias);
 int w8a8_backward(const BackwardArgs& a, void* workspace, cudaStream_t st);

@@ -228,6 +228,7 @@ int64_t w8a8_backward_workspace(int M, int N, bool gated, bool recompute, bool d
 }
 
 int w8a8_backward(const BackwardArgs& a, void* workspace, cudaStream_t st) {
+    if (int rc = refuse_after_failed_wait()) return rc;
     const bool recompute = a.act != kActNone;
     const Layout l = layout(a.M, a.N, a.gated, recompute, a.dbias != nullptr);
     char* ws = static_cast<char*>(workspace);
@@ -258,6 +259,7 @@ int w8a8_backward(const BackwardArgs& a, void* workspace, cudaStream_t st) {
     d.digits = digits; d.row_size = row_size; d.wide = wide; d.W = a.B; d.dx = a.dx;
     d.M = a.M; d.K = a.K; d.parts = l.cols.parts; d.part_rows = l.cols.part_rows; d.part_pitch = l.cols.part_pitch;
     d.partial = a.dbias != nullptr ? partial : nullptr; d.row_blocks = l.row_blocks; d.dbias = a.dbias;
+    d.test_withhold_loads = a.test_withhold_loads; d.test_wait_limit_ns = a.test_wait_limit_ns;
     return gemm_i8_gradient(d, st);
 }
 

@@ -36,8 +36,9 @@ enum {
     DSV4_ERR_ARG = 1,         /* null pointer, negative size, unsupported stride/alignment */
     DSV4_ERR_LAUNCH = 2,      /* the CUDA runtime rejected the launch */
     DSV4_ERR_DRIVER = 3,      /* tensor-map creation failed / driver entry point missing */
-    DSV4_ERR_DEVICE_WAIT = 4  /* a bounded wait in an earlier GEMM kernel on this device gave up; returned once by
-                                 the next GEMM launch, which launches nothing (see dsv4_device_status) */
+    DSV4_ERR_DEVICE_WAIT = 4  /* a bounded wait in an earlier GEMM or gradient kernel on this device gave up (what that
+                                 launch writes is unspecified); returned once by the next GEMM or backward launch, which
+                                 launches nothing (see dsv4_device_status) */
 };
 
 #define DSV4_ABI_VERSION 1
