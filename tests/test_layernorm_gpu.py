@@ -229,3 +229,128 @@ def test_a_row_with_nan_or_infinity_keeps_it(ext, m, k):
     assert torch.equal(y[fine], y0[fine]) and torch.equal(q[fine], q0[fine]) and torch.equal(s[fine], s0[fine])
     b[k - 1] = float("nan")
     assert ext.layernorm_quant(*(t.cuda() for t in (clean, w, b)), EPS)[1].isnan().all()
+
+
+def view_at(t, offset):
+    """the same values on the device, `offset` elements into a buffer whose elements around them are NaN"""
+    if t is None:
+        return None
+    buf = torch.full((t.numel() + 32,), float("nan"), dtype=t.dtype, device="cuda")
+    v = buf[offset:offset + t.numel()].view(t.shape)
+    v.copy_(t)
+    return v
+
+
+def check_forward(a, w, b, k, y, mean, rstd):
+    y64, mean64, rstd64 = ref.layernorm(a, w, b, EPS)
+    big = a.double().abs().amax(1)
+    assert ((mean.cpu().double() - mean64).abs() <= U * seq(k) * big).all()
+    var_err = 2 * seq(k) * U + (U * seq(k) * big * rstd64) ** 2 + 4 * U * seq(k) * big * rstd64
+    assert ((rstd.cpu().double() / rstd64 - 1).abs() <= var_err).all()
+    slack = y_slack(a, mean64, rstd64, w, b, k) + var_err[:, None] * (2 * y64.abs() + b.double().abs())
+    assert ((y.cpu().double() - y64).abs() <= ref.UBF * (y64.abs() + slack) + slack).all()
+
+
+def check_codes(a, w, b, k, q, s):
+    y64, mean64, rstd64 = ref.layernorm(a, w, b, EPS)
+    big = a.double().abs().amax(1)
+    var_err = 2 * seq(k) * U + 4 * U * seq(k) * big * rstd64
+    err = y_slack(a, mean64, rstd64, w, b, k) + var_err[:, None] * (y64.abs() + b.double().abs()) * 2
+    top = y64.abs().amax(1, keepdim=True).clamp_min(1e-10)
+    assert ((s.cpu().double() * 127 - top).abs() <= err.amax(1, keepdim=True) + 2 * U * top).all()
+    exact = y64 * 127 / top
+    slack = err * 127 / top + exact.abs() * (err.amax(1, keepdim=True) / top + 4 * U)
+    assert ((q.cpu().double() - exact).abs() <= 0.5 + slack).all()
+
+
+def check_backward(dy, x, mean, rstd, w, dres, k, dx, dw, db):
+    m = x.shape[0]
+    dx64, dw64, db64 = ref.layernorm_backward(dy, x, mean, rstd, w, dres)
+    xh = (x.double() - mean.double()[:, None]) * rstd.double()[:, None]
+    t = dy.double() * w.double()
+    size = rstd.double()[:, None] * (t.abs() + t.abs().mean(1, keepdim=True) + xh.abs() * (t * xh).abs().mean(1, keepdim=True))
+    slack = U * 2 * seq(k) * size + (0 if dres is None else U * dres.double().abs())
+    assert ((dx.cpu().double() - dx64).abs() <= ref.UBF * (dx64.abs() + slack) + slack).all()
+    adds = U * (min(m, 400) + 8)
+    assert ((dw.cpu().double() - dw64).abs() <= adds * (dy.double() * xh).abs().sum(0) + 1e-30).all()
+    assert ((db.cpu().double() - db64).abs() <= adds * dy.double().abs().sum(0) + 1e-30).all()
+
+
+# arrays at offsets of their own: x, residual (or the gradient past the norm), output side (dy), weight, bias
+OFFSETS = [(0, 0, 0, 0, 0), (2, 2, 2, 0, 0), (1, 1, 1, 0, 0), (2, 0, 4, 2, 6), (1, 2, 3, 0, 1), (8, 5, 0, 8, 8)]
+
+
+@pytest.mark.parametrize("m,k", [(3, 4098), (2, 8190), (3, 8191), (2, 8192), (2, 12290), (2, 16383), (2, 16384), (300, 4098),
+                                 (5, 61), (700, 65), (40, 16386)])
+@pytest.mark.parametrize("offsets", OFFSETS)
+@pytest.mark.parametrize("add", [False, True])
+def test_forward_of_arrays_at_any_offset(ext, m, k, offsets, add):
+    ox, orr, _, ow, ob = offsets
+    x, (w, b) = rows(m, k, 81), weights(k, 82)
+    res = rows(m, k, 83) if add else None
+    a = (res.float() + x.float()).to(torch.bfloat16) if add else x
+    xd, wd, bd = view_at(x, ox), view_at(w, ow), view_at(b, ob)
+    if add:
+        res_d = view_at(res, orr)
+        y, mean, rstd = ext.add_layernorm(res_d, xd, wd, bd, EPS)
+        assert torch.equal(res_d.cpu().view(torch.int16), a.view(torch.int16))
+        around = res_d._base
+        assert around[:orr].isnan().all() and around[orr + m * k:].isnan().all()
+        res_d.copy_(res)
+        q, s, mean2, rstd2 = ext.add_layernorm_quant(res_d, xd, wd, bd, EPS)
+        assert torch.equal(res_d.cpu().view(torch.int16), a.view(torch.int16))
+    else:
+        y, mean, rstd = ext.layernorm(xd, wd, bd, EPS)
+        q, s, mean2, rstd2 = ext.layernorm_quant(xd, wd, bd, EPS)
+    check_forward(a, w, b, k, y, mean, rstd)
+    check_forward(a, w, b, k, y, mean2, rstd2)
+    check_codes(a, w, b, k, q, s)
+
+
+@pytest.mark.parametrize("m,k", [(3, 7170), (2, 7176), (2, 8190), (3, 8191), (1, 8184), (2, 8194), (3, 16382), (2, 16383), (400, 7170),
+                                 (300, 8191), (330, 8190), (160, 16382), (700, 12289), (5, 61), (900, 65), (300, 4098)])
+@pytest.mark.parametrize("offsets", OFFSETS)
+@pytest.mark.parametrize("add", [False, True])
+def test_backward_of_arrays_at_any_offset(ext, m, k, offsets, add):
+    ox, orr, oy, ow, _ = offsets
+    x, (w, b) = rows(m, k, 91), weights(k, 92)
+    dy, dres = wl.randn_bf16((m, k), seed=93), wl.randn_bf16((m, k), seed=94) if add else None
+    _, mean, rstd = ref.layernorm(x, w, b, EPS)
+    mean, rstd = mean.float(), rstd.float()
+    dx, dw, db = ext.layernorm_backward(view_at(dy, oy), view_at(x, ox), mean.cuda(), rstd.cuda(), view_at(w, ow), view_at(dres, orr))
+    check_backward(dy, x, mean, rstd, w, dres, k, dx, dw, db)
+
+
+@pytest.mark.parametrize("m,k,off", [(5, 4104, 4), (3, 8190, 1), (4, 8191, 3), (2, 12290, 2), (3, 16383, 5), (300, 1000, 7), (40, 7170, 2)])
+def test_outputs_at_any_offset_through_the_c_abi(ext, m, k, off):
+    """torch's own outputs are always aligned; a C caller's need not be.  Nothing around them is written."""
+    import ctypes
+    import bw1000_dsv4_kernels_b200 as pkg
+    lib = pkg.c_abi()
+    p = lambda t: ctypes.c_void_p(t.data_ptr())   # noqa: E731
+    st = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    x, (w, b) = rows(m, k, 101), weights(k, 102)
+    xd, wd, bd = x.cuda(), w.cuda(), b.cuda()
+    mean, rstd, s = (torch.empty(m, device="cuda") for _ in range(3))
+    y = view_at(torch.zeros((m, k), dtype=torch.bfloat16), off)
+    eps = ctypes.c_float(EPS)
+    assert lib.launch_layernorm(None, p(xd), p(wd), p(bd), p(y), p(mean), p(rstd), m, k, eps, st) == 0
+    check_forward(x, w, b, k, y, mean, rstd)
+    assert y._base[:off].isnan().all() and y._base[off + m * k:].isnan().all()
+    codes = torch.full((m * k + 64,), 99, dtype=torch.int8, device="cuda")
+    q = codes[off:off + m * k].view(m, k)
+    assert lib.launch_layernorm_quant(None, p(xd), p(wd), p(bd), p(q), p(s), p(mean), p(rstd), m, k, eps, st) == 0
+    check_codes(x, w, b, k, q, s.unsqueeze(1))
+    assert (codes[:off] == 99).all() and (codes[off + m * k:] == 99).all()
+    dy = wl.randn_bf16((m, k), seed=103)
+    _, mean64, rstd64 = ref.layernorm(x, w, b, EPS)
+    mean, rstd = mean64.float(), rstd64.float()
+    dx, dw, db = view_at(torch.zeros((m, k), dtype=torch.bfloat16), off), torch.empty(k, device="cuda"), torch.empty(k, device="cuda")
+    lib.dsv4_layernorm_backward_workspace.restype = ctypes.c_int64
+    size = lib.dsv4_layernorm_backward_workspace(m, k)
+    ws = torch.empty(size, dtype=torch.uint8, device="cuda")
+    md, rd, yd = mean.cuda(), rstd.cuda(), dy.cuda()
+    assert lib.launch_layernorm_backward(p(yd), p(xd), p(md), p(rd), p(wd), None, p(dx), p(dw), p(db), p(ws),
+                                         ctypes.c_longlong(size), m, k, st) == 0
+    check_backward(dy, x, mean, rstd, w, None, k, dx, dw, db)
+    assert dx._base[:off].isnan().all() and dx._base[off + m * k:].isnan().all()
