@@ -11,7 +11,8 @@
 // The sum that is normalised is the ROUNDED one, the residual as it is stored: the backward pass has only that row,
 // and differentiates exactly the function that ran (add_rmsnorm_quant, which has no backward pass, normalises the
 // unrounded sum).  The variance comes from the deviations, not from sum(a^2) - mean^2, which loses every digit of a row
-// with a large mean.  All statistics and sums are fp32.
+// with a large mean.  All statistics and sums are fp32, in an order that sizes, device and the arrays' alignment decide: the
+// width of the accesses decides which columns a thread adds up.
 //
 // Everything here is bound by HBM.  A row belongs to a group of G threads and is read once.
 //   * Forward: a row per group, straight from HBM, several CTAs per SM.

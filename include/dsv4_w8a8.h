@@ -300,7 +300,9 @@ DSV4_API int launch_layernorm_quant(void* res, const void* x, const void* w, con
                        void* rstd, int M, int N, float eps, dsv4_stream_t stream);
 /* Gradients of launch_layernorm: x bf16 [M,N] is the row that was normalised (the updated residual where there was
  * one), dy bf16 [M,N]; dres bf16 [M,N] or null is the gradient that reaches the same row past the norm and is added.
- * dx bf16 [M,N]; dw, db fp32 [N], summed over the rows in an order that depends on M, N and the device only.
+ * dx bf16 [M,N]; dw, db fp32 [N].  Here and in the forward pass the order of the fp32 sums depends on M, N, the device and
+ * the arrays' alignment (which decides how wide the accesses are): a call repeats its bits, the same values at addresses of
+ * another alignment can differ in the last ones.
  * workspace: dsv4_layernorm_backward_workspace(M, N) bytes of device memory, 16-byte aligned, free again once the launches
  * have run. */
 DSV4_API int64_t dsv4_layernorm_backward_workspace(int M, int N);
