@@ -59,18 +59,6 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                    CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
-// More than 48 KB of dynamic shared memory needs an opt-in per kernel and per device; done on the
-// first launch of each kernel on each device.
-template <typename Kernel>
-bool opt_in_shared_memory(Kernel kernel, int bytes, bool (&done)[64]) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev >= 0 && dev < 64 && done[dev]) return true;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) return false;
-    if (dev >= 0 && dev < 64) done[dev] = true;
-    return true;
-}
-
 EncodeTiledFn encode_tiled_fn() {
     static EncodeTiledFn fn = nullptr;
     static std::once_flag once;
@@ -168,17 +156,6 @@ volatile int* host_status_mirror() {
     return mirror[dev];
 }
 
-int sm_count() {
-    static thread_local int cached_dev = -1, cached = 0;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    if (dev != cached_dev) {
-        cudaDeviceGetAttribute(&cached, cudaDevAttrMultiProcessorCount, dev);
-        cached_dev = dev;
-    }
-    return cached;
-}
-
 template <int BN, int STAGES>
 int launch_variant(const CUtensorMap& tmA, const CUtensorMap& tmB, const Params& p, int max_tiles,
                    cudaStream_t st) {
@@ -263,6 +240,11 @@ int launch_stream_variant(const CUtensorMap& tmW, const CUtensorMap& tmX, const 
 }
 
 template <int EPI>
+bool stream_pair_opted_in() {
+    static bool opted_in[64] = {};
+    return opt_in_shared_memory(gemm_i8_stream_pair_kernel<EPI>, StreamPairSmem::kDynamic, opted_in);
+}
+template <int EPI>
 int stream_pair_active_clusters(int splits) {
     static ClusterCounts cached = {};
     return active_clusters(gemm_i8_stream_pair_kernel<EPI>, 2 * splits, StreamPairSmem::kDynamic, cached);
@@ -273,8 +255,7 @@ int launch_stream_pair(const CUtensorMap& tmW, const CUtensorMap& tmX, const Par
                        cudaStream_t st) {
     using L = StreamPairSmem;
     static_assert(L::kDynamic <= 227 * 1024, "shared memory limit");
-    static bool opted_in[64] = {};
-    if (!opt_in_shared_memory(gemm_i8_stream_pair_kernel<EPI>, L::kDynamic, opted_in))
+    if (!stream_pair_opted_in<EPI>())
         return fail(DSV4_ERR_LAUNCH, "w8a8_gemm: cannot raise the dynamic shared memory limit");
     // a cluster must fit into one GPC: take the widest K split whose clusters all run in one wave
     while (splits > 1 && stream_pair_active_clusters<EPI>(splits) < n_tiles) --splits;
@@ -439,15 +420,18 @@ int launch_stream_blocks(const GemmArgs& a, Params p, int blocks, int pair_tiles
 // tokens than the tile kernel's drain.
 bool split_pays(int tokens, int splits, int k_blocks) { return k_blocks * (splits - 1) >= tokens / 8 * splits; }
 
+// Half as many tiles as there are pairs of SMs (37 on a B200): with so few, a tile's K is worth splitting
+int few_tiles() { return sm_count() / 4; }
+
 // Whether few tokens with a fused epilogue go to the weight-streaming kernel rather than the tiles of 256 tokens, whose drain
 // is faster and whose tiles are as narrow as 64 outputs.  Measured (tiles / streaming, with bias, GELU, residual): 128 x 4096
 // x 1024 5.6 / 9.0 us, x 7168 14.7 / 14.8; 128 x 18432 x 4096 28.2 / 29.2; 65 x 18432 x 4096 27.2 / 24.0; 65 x 4096 x 1024
 // 6.2 / 7.6; 59 x 3000 x 64 6.6 / 9.0, x 512 7.3 / 6.6; 33 x 18432 x 1024 14.4 / 9.7; 256 x 400 x 4096 12.4 / 8.3 (blocks of 32).
 bool fused_few(int M, int ntok, int w_rows, int n_tiles, int splits, int k_blocks) {
-    const bool few_tiles = n_tiles <= 37;
-    if (M <= 64) return M <= 32 || k_blocks > 2 || !few_tiles;
+    const bool few = n_tiles <= few_tiles();
+    if (M <= 64) return M <= 32 || k_blocks > 2 || !few;
     if (M > 128 && w_rows >= 256 && ntok > 64) return false;
-    return few_tiles ? split_pays(min(M, ntok), splits, k_blocks) : M <= 96;
+    return few ? split_pays(min(M, ntok), splits, k_blocks) : M <= 96;
 }
 
 // K split of more tokens over the streaming kernel's pairs, or 0 where the tile kernel is faster.  Measured (tiles / this
@@ -456,8 +440,7 @@ bool fused_few(int M, int ntok, int w_rows, int n_tiles, int splits, int k_block
 template <int EPI>
 int stream_blocks_splits(int M, int pair_tiles, int blocks, int k_blocks) {
     const int64_t clusters = (int64_t)pair_tiles * blocks;
-    static bool opted_in[64] = {};
-    if (clusters > 37 || !opt_in_shared_memory(gemm_i8_stream_pair_kernel<EPI>, StreamPairSmem::kDynamic, opted_in)) return 0;
+    if (clusters > few_tiles() || !stream_pair_opted_in<EPI>()) return 0;
     for (int s = k_blocks < 4 ? k_blocks : 4; s > 1; --s)
         if (stream_pair_active_clusters<EPI>(s) >= clusters) return split_pays(stream_block_tokens(M, blocks), s, k_blocks) ? s : 0;
     return 0;
@@ -490,8 +473,11 @@ int gemm_i8_dense(const GemmArgs& a, Params p, int bn, cudaStream_t st) {
         if (splits > 8) splits = 8;
         if (splits > k_blocks) splits = k_blocks;
         if (splits < 1) splits = 1;
-        int ntok = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : a.M <= 128 ? 128 : 256, tiles = n_tiles;
+        // fused epilogues: blocks of at most 128 tokens, several clusters of them for more
+        int ntok = a.M <= 16 ? 16 : a.M <= 32 ? 32 : a.M <= 64 ? 64 : a.M <= 128 || EPI != kEpiPlain ? 128 : 256;
+        int tiles = n_tiles;
         if constexpr (EPI != kEpiPlain) {
+            if (a.M > 128) tiles *= 2;
             // blocks of fewer tokens while the clusters would fill less than half the SMs (200 x 200 x 8192 12.7 -> 7.3 us,
             // 90 x 60 x 2048 7.6 -> 5.5; 17 x 1000 x 4096 5.9 -> 6.2 with 16, hence not below 32)
             while (ntok > 32 && tiles * splits * 2 <= sms) {
@@ -509,7 +495,9 @@ int gemm_i8_dense(const GemmArgs& a, Params p, int bn, cudaStream_t st) {
                 case 32: return launch_stream_variant<32, EPI>(tmA, tmB, p, tiles, splits, st);
                 case 64: return launch_stream_variant<64, EPI>(tmA, tmB, p, tiles, splits, st);
                 case 128: return launch_stream_variant<128, EPI>(tmA, tmB, p, tiles, splits, st);
-                default: return launch_stream_variant<256, EPI>(tmA, tmB, p, tiles, splits, st);
+                default:
+                    if constexpr (EPI == kEpiPlain) return launch_stream_variant<256, EPI>(tmA, tmB, p, tiles, splits, st);
+                    return fail(DSV4_ERR_ARG, "w8a8_linear: more tokens than a block has");   // ntok is one of those above
             }
         }
     }

@@ -13,6 +13,33 @@ int fail(int code, const char* msg);
 int check_launch(const char* what);
 
 #ifdef __CUDACC__
+// SMs of the current device; 0 without one
+inline int sm_count() {
+    static thread_local int cached_dev = -1, cached = 0;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (dev != cached_dev) {
+        cudaDeviceGetAttribute(&cached, cudaDevAttrMultiProcessorCount, dev);
+        cached_dev = dev;
+    }
+    return cached;
+}
+
+// More than 48 KB of dynamic shared memory needs an opt-in per kernel and per device; done on the
+// first launch of each kernel on each device.
+template <typename Kernel>
+bool opt_in_shared_memory(Kernel kernel, int bytes, bool (&done)[64]) {
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (dev >= 0 && dev < 64 && done[dev]) return true;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess) {
+        cudaGetLastError();  // clear the sticky error
+        return false;
+    }
+    if (dev >= 0 && dev < 64) done[dev] = true;
+    return true;
+}
+
 // Launches a kernel that may start while the one before it on the stream still runs (programmatic dependent launch); it
 // has to wait (griddepcontrol.wait) before it touches anything that kernel, or one before it, reads or writes.
 template <typename... P, typename... A>

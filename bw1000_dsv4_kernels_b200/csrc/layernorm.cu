@@ -728,17 +728,6 @@ __global__ void __launch_bounds__(256) layernorm_column_sum_kernel(const float* 
 }
 
 // ---- host side -----------------------------------------------------------------------------------------------------
-int sm_count() {
-    static thread_local int cached_dev = -1, cached = 0;
-    int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    if (dev != cached_dev) {
-        cudaDeviceGetAttribute(&cached, cudaDevAttrMultiProcessorCount, dev);
-        cached_dev = dev;
-    }
-    return cached;
-}
-
 // threads per row (multiple of 32) when each thread makes at most `v` accesses
 int group_threads(int accesses, int v) { return ((accesses + v - 1) / v + 31) / 32 * 32; }
 
@@ -775,19 +764,6 @@ RowsShape rows_shape(int K, int arrays, int threads, int column_floats) {
     s.smem = s.R * per_group;
     return s;
 }
-template <typename Kernel>
-int opt_in(Kernel kernel, bool (&done)[64], const char* what) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (dev >= 0 && dev < 64 && done[dev]) return 0;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kRowsSmem) != cudaSuccess) {
-        cudaGetLastError();
-        return fail(DSV4_ERR_LAUNCH, what);
-    }
-    if (dev >= 0 && dev < 64) done[dev] = true;
-    return 0;
-}
-
 // Whether a row begins at the same offset of the 16 bytes in all arrays (the codes': of 8 bytes), and weight and bias at 0
 template <bool ADD, bool QUANT>
 bool same_offset(const NormArgs& p) {
@@ -832,8 +808,8 @@ constexpr int kMaxParts = 160;
 template <int W, int V, int B, int DEPTH, int THREADS, bool RES>
 int launch_norm_backward(NormBwdArgs p, float* dw, float* db, int parts, cudaStream_t st) {
     static bool opted_in[64] = {};
-    if (int rc = opt_in(layernorm_backward_kernel<W, V, B, DEPTH, THREADS, RES>, opted_in, "layernorm_backward: cannot raise the dynamic shared memory limit"))
-        return rc;
+    if (!opt_in_shared_memory(layernorm_backward_kernel<W, V, B, DEPTH, THREADS, RES>, kRowsSmem, opted_in))
+        return fail(DSV4_ERR_LAUNCH, "layernorm_backward: cannot raise the dynamic shared memory limit");
     RowsShape s = rows_shape<W, V, DEPTH * B>(p.K, RES ? 3 : 2, THREADS, 2 * p.K);
     p.T = s.G;
     p.slot_bytes = s.slot_bytes;
