@@ -12,6 +12,11 @@
 // them to the CURRENT stream: a caller that passes another stream keeps the outputs alive (or calls
 // record_stream on them) until that stream has run the kernel, as with any tensor used across streams.
 //
+// Small outputs of one call share an allocation: mean, rstd and scales of a layer norm, dw and db of its gradient.  Each is a
+// dense tensor with a version counter of its own, not a view of the others; keeping one keeps the memory of all.
+// per_token_quant_int8, w8a8_scaled_gemm and the feed-forward operators take their outputs from the caching allocator without
+// torch's dispatcher, so dispatch modes do not see these allocations.
+//
 // Differences from the reference, all additive or stricter:
 //   * `name(...)` launches on torch's current stream rather than on stream 0;
 //   * dtype / device / shape / alignment are checked (the reference checks contiguity only);
@@ -720,7 +725,7 @@ std::vector<c10::optional<Tensor>> w8a8_gated_backward_stream(Tensor dh, Tensor 
 struct NormShape {
     int M, N;
 };
-NormShape check_norm(const Tensor& x, const Tensor& w, const Tensor& b, const c10::optional<Tensor>& res) {
+NormShape check_norm(const Tensor& x, const Tensor& w, const Tensor& b, const c10::optional<Tensor>& res, const char* res_name = "res") {
     check_cuda(x, "x", torch::kBFloat16);
     check_cuda(w, "w", torch::kBFloat16);
     check_cuda(b, "b", torch::kBFloat16);
@@ -730,10 +735,10 @@ NormShape check_norm(const Tensor& x, const Tensor& w, const Tensor& b, const c1
     TORCH_CHECK(x.dim() >= 1 && x.size(-1) > 0, "x must have at least one column");
     TORCH_CHECK(w.numel() == x.size(-1) && b.numel() == x.size(-1), "w and b must have one entry per column of x");
     if (res.has_value()) {
-        check_cuda(*res, "res", torch::kBFloat16);
-        check_same_device(x, *res, "x/res");
-        TORCH_CHECK(res->is_contiguous(), "res must be contiguous");
-        TORCH_CHECK(res->sizes() == x.sizes(), "res and x must have the same shape");
+        check_cuda(*res, res_name, torch::kBFloat16);
+        check_same_device(x, *res, res_name);
+        TORCH_CHECK(res->is_contiguous(), res_name, " must be contiguous");
+        TORCH_CHECK(res->sizes() == x.sizes(), res_name, " and x must have the same shape");
     }
     const Rows r = rows_of(x);
     return {r.M, r.N};
@@ -779,7 +784,7 @@ std::vector<Tensor> add_layernorm_quant_stream(Tensor res, Tensor x, Tensor w, T
 // -> dx, dw fp32, db fp32; x is the row that was normalised (the updated residual where there was one)
 std::vector<Tensor> layernorm_backward_stream(Tensor dy, Tensor x, Tensor mean, Tensor rstd, Tensor w,
                                               c10::optional<Tensor> dres, int64_t stream_ptr) {
-    const NormShape n = check_norm(x, w, w, dres);
+    const NormShape n = check_norm(x, w, w, dres, "dres");
     check_cuda(dy, "dy", torch::kBFloat16);
     check_same_device(x, dy, "x/dy");
     TORCH_CHECK(dy.is_contiguous() && dy.sizes() == x.sizes(), "dy must be contiguous with the shape of x");
