@@ -75,8 +75,8 @@ __device__ __forceinline__ int quant_trunc_div(float x, float scale) {
 // The same quotient without a division per element: with rcp = RN(1/scale) computed once per
 // group, q0 = RN(x*rcp), r = fma(-q0, scale, x) (the exact residual, rounded once) and
 // q1 = fma(r, rcp, q0) is the correctly rounded x/scale for operands in the normal range
-// (the final step of the standard division algorithm); below 1 in magnitude the truncation is
-// zero whatever the last bit.  Checked against true division in the GPU tests.
+// (one correction with a fused remainder: P. W. Markstein, "Computation of elementary functions on the IBM RISC
+// System/6000 processor", 1990); below 1 in magnitude the truncation is zero whatever the last bit.  Checked against true division in the GPU tests.
 // Returns the code in the low byte of the result (two's complement).  No clamp: for a finite group
 // |x| <= amax and scale = RN(amax/127), so |x/scale| <= 127*(1+2^-23) and the truncation is within
 // [-127, 127]; groups containing Inf or NaN give unspecified codes.
@@ -121,6 +121,8 @@ __device__ __forceinline__ uint32_t pack_i8x4(int a, int b, int c, int d) {
 //   r = fma(n, -ln2_hi, x); r = fma(n, -ln2_lo, r)
 //   p = 1 + r*(1 + r*(c2 + r*(c3 + r*(c4 + r*(c5 + r*c6)))))   (Horner, all fma)
 //   result = p * 2^n   (added to the exponent field; p*2^n stays a normal number)
+// The reduction with ln 2 in two parts is W. J. Cody and W. Waite's ("Software Manual for the Elementary Functions", 1980),
+// the polynomial is the Taylor series.
 // Maximum observed error against a double-precision exp: 2.6 ulp of the result.
 constexpr float kExpClamp = 87.0f;
 constexpr float kLog2e = 1.44269502162933349609375f;        // 0x3FB8AA3B

@@ -124,6 +124,7 @@ class NormFFN:
         return out, NormFFNSaved(saved, res, mean, rstd)
 
     def backward(self, dout, saved: NormFFNSaved) -> NormFFNGrads:
+        """dout bf16 [M, H], dense (it is also the gradient that reaches the residual past the norm)."""
         g = self.ffn.backward(dout, saved.ffn)
         dx, dgamma, dbeta = _ext().layernorm_backward(g.dx, saved.res, saved.mean, saved.rstd, self.gamma, dout)
         return NormFFNGrads(dx, dgamma, dbeta, g.db1, g.db2)
