@@ -185,6 +185,22 @@ def test_rows_with_outliers_are_as_exact_as_the_others(ext, m, n, k, act):
     assert torch.equal(dx2.cpu()[~some].view(torch.int16), dx.cpu()[~some].view(torch.int16))
 
 
+@pytest.mark.parametrize("m", [9, 120, 400])
+def test_outliers_of_every_size_stay_within_the_bound(ext, m):
+    """one and several outliers per row, from three times to 10^6 times the rest, on both sides of the rule"""
+    n, k = 1100, 400
+    (a, sa), (w, sw) = ref.tokens(m, k, m), ref.weight(n, k, n)
+    w[5], w[600], w[1099] = 0, 0, 0
+    dy = ref.bf16((m, n), 4).float()
+    size = 10.0 ** (0.5 + 5.5 * torch.arange(m) / m)
+    dy[:, 5] = size
+    dy[::2, 600], dy[::3, 1099] = size[::2], -size[::3]
+    dy = dy.to(torch.bfloat16)
+    dx64, _, t, dz = ref.linear_backward(dy, a, sa, w, sw)
+    dx, _ = ext.w8a8_linear_backward(dy.cuda(), *cuda(a, w, sa, sw))
+    check_dx_by_typical_size(dx, dx64, t, torch.zeros_like(dz), w)
+
+
 @pytest.mark.parametrize("m,i,k", [(20, 300, 272), (300, 700, 528), (700, 1100, 784)])
 def test_gated_rows_with_outliers(ext, m, i, k):
     """an outlier in the incoming gradient, whose gate and up rows of the weight are zero"""
